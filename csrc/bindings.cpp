@@ -145,6 +145,7 @@ void wait_selftest(torch::Tensor flag, int64_t target, double timeout_s, torch::
 
 void register_runtime(pybind11::module_& m);  // runtime_bindings.cpp
 void register_flash(pybind11::module_& m);    // flash_bindings.cpp
+void register_paged(pybind11::module_& m);    // paged_bindings.cpp
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "B200-native ring attention: sm_100a kernels and the native ring runtime";
@@ -164,5 +165,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("wait_selftest", &rab::wait_selftest,
         "bounded device wait on a flag word; records a timeout in the status word");
   register_flash(m);
+  register_paged(m);
   register_runtime(m);
 }

@@ -46,6 +46,15 @@ enum BoundsSite : uint32_t {
   kBoundsMergeRecord = 103,  // split partial record read by a merge kernel
 };
 
+// Sites of kStatusBadArgs: what a device tensor held that a kernel of the paged
+// cache skipped instead of following (reported as `where`, the value in `detail`).
+enum BadArgSite : uint32_t {
+  kBadPage = 201,      // page id outside the pool
+  kBadPosition = 202,  // cache position outside the page table
+  kBadPath = 203,      // accepted path not increasing, or longer than its row
+  kBadParent = 204,    // parent index not before its token
+};
+
 struct DeviceStatus {
   uint32_t code;       // StatusCode, first error wins
   uint32_t where;      // WaitSite of the first error

@@ -31,6 +31,10 @@ a call counter in device memory that the kernel itself advances, so a call
 captured once (``capture()``, or any ``torch.cuda.graph`` region) can be
 replayed; every rank must capture and replay in step, one replay being one
 ring call, with the same input and output tensors each time.
+
+Rotary positions: ``rotary=Rotary(...)`` (`ops.rotary`) turns q and k of every
+call by this rank's global token positions (``positions()``, zigzag shards
+included) before the ring; v and the inputs themselves are left alone.
 """
 from __future__ import annotations
 
@@ -39,7 +43,9 @@ from typing import Optional
 import torch
 
 from .._ext import load
+from ..ops.rotary import Rotary
 from ..parallel.dist import RingRuntime
+from .oracle import zigzag_positions
 
 _DTYPES = {torch.float32: "fp32", torch.bfloat16: "bf16"}
 
@@ -49,11 +55,13 @@ class RingAttention:
                  heads_kv: Optional[int] = None, dtype: torch.dtype = torch.float32,
                  causal: bool = False, zigzag: Optional[bool] = None, ring_mode: str = "direct",
                  runtime: Optional[RingRuntime] = None, timeout_s: float = 10.0,
-                 graph_safe: bool = False):
+                 graph_safe: bool = False, rotary: Optional[Rotary] = None):
         if dtype not in _DTYPES:
             raise ValueError("dtype must be torch.float32 or torch.bfloat16")
         if ring_mode not in ("direct", "chain"):
             raise ValueError("ring_mode must be 'direct' or 'chain'")
+        if rotary is not None and not 2 <= rotary.rotary_dim <= head_dim:
+            raise ValueError(f"rotary turns {rotary.rotary_dim} dims of a head of {head_dim}")
         C = load()
         self.seq = seq_per_rank
         self.heads = heads
@@ -81,6 +89,8 @@ class RingAttention:
         self._shape_q = torch.Size((seq_per_rank, heads, head_dim))
         self._shape_kv = torch.Size((seq_per_rank, self.heads_kv, head_dim))
         self._default_scale = head_dim ** -0.5
+        self._rotary = rotary.to(self._dev) if rotary is not None else None
+        self._positions = self.positions() if rotary is not None else None
 
     @property
     def rank(self) -> int:
@@ -89,6 +99,14 @@ class RingAttention:
     @property
     def world(self) -> int:
         return self.runtime.world
+
+    def positions(self) -> torch.Tensor:
+        """Global position of each token of this rank's shard (int64, on its GPU)."""
+        if self.zigzag:
+            pos = zigzag_positions(self.rank, self.world, self.seq)
+        else:
+            pos = torch.arange(self.rank * self.seq, (self.rank + 1) * self.seq)
+        return pos.to(self._dev)
 
     def _check_inputs(self, q, k, v, out=None):
         dev, dt = self._dev, self.dtype
@@ -119,6 +137,8 @@ class RingAttention:
             out = torch.empty_like(q)
         lse = (torch.empty(self.seq, self.heads, dtype=torch.float32, device=q.device)
                if return_lse else None)
+        if self._rotary is not None:
+            q, k = self._rotary(q.detach(), k.detach(), self._positions)
         self.engine.forward(q.contiguous(), k.contiguous(), v.contiguous(), out, lse, float(scale))
         if check:
             self.engine.check()

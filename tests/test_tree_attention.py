@@ -1,0 +1,383 @@
+"""Attention of drafted trees, single tokens and chunks over a paged cache, against 64 bits."""
+import math
+
+import pytest
+import torch
+
+import _paged_oracle as O
+from ring_attention_benchmark_b200.ops.attention import DeviceTimeout, check_status, new_status
+from ring_attention_benchmark_b200.ops.paged import pack_mask, tree_attention, tree_mask
+
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def _case(ctx, counts, H, Hk, D, page, dtype, seed=0, extra=0, spread=1.0, fill=None):
+    """Inputs on the CPU; unused rows of the pool hold `fill` (a stale cache holds anything)."""
+    g = torch.Generator().manual_seed(seed)
+    T = sum(counts)
+    q = (torch.randn(T + extra, H, D, generator=g) * spread).to(dtype)
+    need = [-(-(c + m) // page) for c, m in zip(ctx, counts)]
+    pool = sum(need) + 2
+    order = torch.randperm(pool, generator=g).tolist()
+    table = torch.zeros(len(ctx), max(max(need), 1) + 1, dtype=torch.int32)
+    kp, vp = (torch.full((pool, Hk, page, D), 0.0 if fill is None else fill).to(dtype) for _ in "kv")
+    for b, n in enumerate(need):
+        for i in range(n):
+            table[b, i] = order.pop()
+        for j in range(ctx[b] + counts[b]):
+            kp[table[b, j // page], :, j % page] = torch.randn(Hk, D, generator=g).to(dtype)
+            vp[table[b, j // page], :, j % page] = torch.randn(Hk, D, generator=g).to(dtype)
+    return q, kp, vp, table
+
+
+def _run(q, kp, vp, table, ctx, counts, uniform=False, **kw):
+    cu = None if uniform else torch.tensor([0] + counts).cumsum(0).int().cuda()
+    return tree_attention(q.cuda(), kp.cuda(), vp.cuda(), table.cuda(),
+                          torch.tensor(ctx, dtype=torch.int32).cuda(), cu, return_lse=True, **kw)
+
+
+def _check(got, lse, case, ctx, counts, masks=None, scale=None):
+    q, kp, vp, table = case
+    T = sum(counts)
+    ref, rlse, mag, smax = O.attention(q[:T], kp, vp, table, ctx, counts, masks, scale)
+    keys = max([c + m for c, m in zip(ctx, counts)] + [1])
+    bo, bl = O.attention_bound(ref, mag, smax, q.dtype, keys, q.shape[2])
+    g, gl = got[:T].cpu().double(), lse[:T].cpu().double()
+    empty = rlse == -math.inf
+    assert torch.equal(gl == -math.inf, empty)
+    assert (g[empty] == 0).all()
+    d = (g - ref).abs()
+    assert (d <= bo).all(), ((d - bo).max().item(), d.max().item())
+    dl = (gl - rlse).abs()[~empty]
+    assert (dl <= (bl + 2.0 ** -22 * rlse.abs())[~empty]).all(), dl.max().item()
+
+
+def _trees(counts, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    parents, masks, depths = [], [], []
+    for m in counts:
+        p = [-1 if i == 0 or torch.rand(1, generator=g).item() < 0.1
+             else int(torch.randint(0, i, (1,), generator=g)) for i in range(m)]
+        mask, depth = O.ancestors(p)
+        parents += p
+        masks.append(mask)
+        depths += depth
+    w = max(counts)
+    rows = torch.zeros(sum(counts), w, dtype=torch.bool)
+    first = 0
+    for m, mask in zip(counts, masks):
+        rows[first:first + m, :m] = mask
+        first += m
+    return parents, masks, rows, depths
+
+
+# ------------------------------------------------------------------ refusals (CPU)
+def _args(**kw):
+    a = dict(q=torch.zeros(2, 4, 64), k_pages=torch.zeros(3, 2, 16, 64),
+             v_pages=torch.zeros(3, 2, 16, 64), block_table=torch.zeros(1, 2, dtype=torch.int32),
+             context_lens=torch.zeros(1, dtype=torch.int32))
+    a.update(kw)
+    return a
+
+
+@pytest.mark.parametrize("kw, what", [
+    (dict(), "CUDA"),
+    (dict(q=torch.zeros(2, 4, 32), k_pages=torch.zeros(3, 2, 16, 32), v_pages=torch.zeros(3, 2, 16, 32)), "64 or 128"),
+    (dict(q=torch.zeros(2, 4, 128)), "head dim"),
+    (dict(q=torch.zeros(2, 3, 64)), "multiple"),
+    (dict(q=torch.zeros(2, 4, 64).half()), "share a dtype"),
+    (dict(k_pages=torch.zeros(3, 2, 24, 64), v_pages=torch.zeros(3, 2, 24, 64)), "page size"),
+    (dict(k_pages=torch.zeros(3, 2, 8, 64), v_pages=torch.zeros(3, 2, 8, 64)), "page size"),
+    (dict(k_pages=torch.zeros(3, 2, 512, 64), v_pages=torch.zeros(3, 2, 512, 64)), "page size"),
+    (dict(mask=torch.zeros(3, 2, dtype=torch.bool)), "row for each"),
+    (dict(mask=torch.zeros(2, 2)), "bool, or int32"),
+    (dict(mask=torch.zeros(2, 0, dtype=torch.bool)), "columns"),
+    (dict(scale=math.nan), "finite"),
+    (dict(max_q=0), "max_q"),
+    (dict(out=torch.zeros(2, 4, 128)), "shape"),
+    (dict(out=torch.zeros(2, 4, 64).half()), "dtype"),
+    (dict(out=torch.zeros(1, 4, 64).expand(2, 4, 64)), "shares memory"),
+    (dict(out=torch.zeros(2, 4, 66)[:, :, :64]), "aligned"),
+    (dict(timeout_s=0.0), "timeout_s"),
+    (dict(context_lens=torch.zeros(1, dtype=torch.int64)), "int32"),
+    (dict(context_lens=torch.zeros(3, dtype=torch.int32), block_table=torch.zeros(3, 2, dtype=torch.int32)), "evenly"),
+])
+def test_refusals(ext, kw, what):
+    with pytest.raises(RuntimeError, match=what):
+        tree_attention(**_args(**kw))
+
+
+@pytest.mark.parametrize("kw, what", [
+    (dict(parents=torch.zeros(4, dtype=torch.int32), max_q=4), "CUDA"),
+    (dict(parents=torch.zeros(4), max_q=4), "int32"),
+    (dict(parents=torch.zeros(4, dtype=torch.int32), max_q=0), "max_q"),
+    (dict(parents=torch.zeros(4, dtype=torch.int32), max_q=4, batch=3), "evenly"),
+])
+def test_tree_mask_refusals(ext, kw, what):
+    with pytest.raises(RuntimeError, match=what):
+        tree_mask(**kw)
+
+
+def test_pack_mask_refusals(ext):
+    for m in (torch.zeros(2, 2), torch.zeros(2, 0, dtype=torch.bool), torch.zeros(2, 2, dtype=torch.bool)):
+        with pytest.raises(RuntimeError, match="bool|columns|CUDA"):
+            pack_mask(m)
+
+
+# ------------------------------------------------------------------ masks (GPU)
+def _bits(words, cols):
+    j = torch.arange(cols)
+    return ((words.cpu().long()[:, j // 32] >> (j % 32)) & 1).bool()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("counts", [[1], [1, 0, 5], [33, 64, 2], [70, 7]])
+def test_tree_mask(ext, cuda_device, counts):
+    parents, _, rows, depths = _trees([c for c in counts])
+    w = max(counts)
+    cu = torch.tensor([0] + counts).cumsum(0).int().cuda()
+    st = new_status("cuda")
+    mask, depth = tree_mask(torch.tensor(parents, dtype=torch.int32).cuda(), cu, max_q=w, status=st)
+    check_status(st)
+    assert mask.shape == (sum(counts), -(-w // 32))
+    assert torch.equal(_bits(mask, w), rows) and depth.cpu().tolist() == depths
+    assert torch.equal(pack_mask(rows.cuda()), mask)
+    narrow, _ = tree_mask(torch.tensor(parents, dtype=torch.int32).cuda(), cu, max_q=1)
+    assert torch.equal(_bits(narrow, min(w, 32)), rows[:, :32])
+
+
+@pytest.mark.gpu
+def test_tree_mask_uniform_and_bad_parents(ext, cuda_device):
+    st = new_status("cuda")
+    p = torch.tensor([-1, 0, 1, -1, 0, 0], dtype=torch.int32).cuda()
+    mask, depth = tree_mask(p, batch=2, max_q=3, status=st)
+    check_status(st)
+    assert mask.flatten().tolist() == [1, 3, 7, 1, 3, 5] and depth.tolist() == [0, 1, 2, 0, 1, 1]
+    mask, _ = tree_mask(torch.tensor([-1, 1, 5, -2], dtype=torch.int32).cuda(), batch=1, max_q=4, status=st)
+    assert mask.flatten().tolist() == [1, 2, 4, 8]  # a token whose parent is no token before it is a root
+    with pytest.raises(DeviceTimeout, match="code=2"):
+        check_status(st)
+
+
+# ------------------------------------------------------------------ values (GPU)
+SHAPES = [
+    # ctx, counts, heads, kv heads, dim, page
+    ([0], [1], 1, 1, 64, 16),
+    ([1, 0, 127, 128, 129], [1, 1, 1, 1, 1], 8, 2, 128, 16),
+    ([300, 5, 64], [7, 1, 16], 7, 1, 64, 32),
+    ([33, 0, 200], [3, 0, 40], 4, 4, 128, 64),
+    ([0, 0], [130, 64], 2, 1, 64, 128),
+    ([255, 256, 900], [2, 33, 5], 16, 2, 128, 256),
+    ([70], [65], 24, 8, 64, 16),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("ctx, counts, H, Hk, D, page", SHAPES)
+def test_causal_values(ext, cuda_device, dtype, ctx, counts, H, Hk, D, page):
+    case = _case(ctx, counts, H, Hk, D, page, dtype)
+    st = new_status("cuda")
+    out, lse = _run(*case, ctx, counts, status=st)
+    check_status(st)
+    _check(out, lse, case, ctx, counts)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("ctx, counts, H, Hk, D, page", SHAPES)
+def test_tree_values(ext, cuda_device, dtype, ctx, counts, H, Hk, D, page):
+    case = _case(ctx, counts, H, Hk, D, page, dtype, seed=1)
+    parents, masks, rows, _ = _trees(counts)
+    st = new_status("cuda")
+    out, lse = _run(*case, ctx, counts, mask=rows.cuda(), max_q=max(counts), status=st)
+    _check(out, lse, case, ctx, counts, masks)
+    words, _ = tree_mask(torch.tensor(parents, dtype=torch.int32).cuda(),
+                         torch.tensor([0] + counts).cumsum(0).int().cuda(), max_q=max(counts))
+    out2, lse2 = _run(*case, ctx, counts, mask=words, max_q=1, status=st)  # the hint only steers
+    check_status(st)
+    _check(out2, lse2, case, ctx, counts, masks)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_uniform_borders_scale_and_out(ext, cuda_device, dtype):
+    ctx, counts = [40, 41, 7], [2, 2, 2]
+    case = _case(ctx, counts, 4, 2, 64, 16, dtype, seed=2)
+    big = torch.full((6, 6, 64), 5.0, dtype=dtype, device="cuda")
+    out, lse = _run(*case, ctx, counts, uniform=True, scale=0.03, out=big[:, 1:5])
+    _check(out, lse, case, ctx, counts, scale=0.03)
+    assert (big[:, 0] == 5.0).all() and (big[:, 5] == 5.0).all()
+    out, lse = _run(*case, ctx, counts, uniform=True, scale=-0.5)
+    _check(out, lse, case, ctx, counts, scale=-0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_that_see_nothing(ext, cuda_device, dtype):
+    """An empty mask row without context gives 0 and -inf; with context it sees the context."""
+    ctx, counts = [0, 50, 0], [4, 4, 3]
+    case = _case(ctx, counts, 4, 2, 128, 16, dtype, seed=3)
+    masks = [torch.zeros(m, 4, dtype=torch.bool) for m in counts]
+    masks[0][1, 0] = masks[2][2, 2] = masks[1][0, 3] = True
+    out, lse = _run(*case, ctx, counts, mask=torch.cat(masks).cuda())
+    _check(out, lse, case, ctx, counts, masks)
+    narrow = [m[:, :1] for m in masks]  # columns beyond the mask are not seen
+    out, lse = _run(*case, ctx, counts, mask=torch.cat(narrow).cuda())
+    _check(out, lse, case, ctx, counts, narrow)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_masked_places_may_hold_anything(ext, cuda_device, dtype, bad):
+    """Stale rows of the pool, and a new token that some rows see and others do not."""
+    ctx, counts = [37, 130], [5, 9]
+    for where in ("pool", "k", "v"):
+        case = _case(ctx, counts, 4, 2, 64, 32, dtype, seed=4, fill=bad if where == "pool" else None)
+        q, kp, vp, table = case
+        masks = [torch.ones(m, 9, dtype=torch.bool).tril() for m in counts]
+        for m in masks:
+            m[4, 2] = False  # row 4 does not see token 2, row 3 does
+        if where != "pool":
+            for b in range(2):
+                j = ctx[b] + 2
+                (kp if where == "k" else vp)[table[b, j // 32], 1, j % 32, 5] = bad
+        out, lse = _run(*case, ctx, counts, mask=torch.cat(masks).cuda())
+        out, lse = out.cpu(), lse.cpu()
+        blind = torch.tensor([t for t in range(14) if t in (0, 1, 4, 5, 6, 9)])
+        keep = torch.arange(14) if where == "pool" else blind
+        clean = (q, kp.nan_to_num(0.0, 0.0, 0.0), vp.nan_to_num(0.0, 0.0, 0.0), table)
+        ref, rlse, mag, smax = O.attention(*clean, ctx, counts, masks)
+        bo, bl = O.attention_bound(ref, mag, smax, dtype, 139, 64)
+        assert ((out.double() - ref).abs() <= bo)[keep].all(), where
+        assert ((lse.double() - rlse).abs() <= bl + 2.0 ** -22 * rlse.abs())[keep].all(), where
+        if where == "v":  # a row that sees it has it in its own column, and only there
+            seen = torch.tensor([t for t in range(14) if t not in blind.tolist()])
+            got = out[seen][:, 2:].float()  # the heads of kv head 1
+            assert (got[..., 5].isnan() if math.isnan(bad) else got[..., 5] == bad).all()
+            rest = torch.arange(64) != 5
+            assert torch.isfinite(got[..., rest]).all() and torch.isfinite(out[seen][:, :2]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_behind_the_last_request_are_left(ext, cuda_device, dtype):
+    ctx, counts = [10, 20], [3, 2]
+    case = _case(ctx, counts, 4, 2, 64, 16, dtype, extra=4)
+    q = case[0].clone()
+    q[5:] = math.nan
+    out = torch.full(q.shape, 2.5, dtype=dtype, device="cuda")
+    got, lse = _run(q, *case[1:], ctx, counts, out=out)
+    _check(got, lse, case, ctx, counts)
+    assert (out[5:] == 2.5).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_large_and_small_scores(ext, cuda_device, dtype):
+    """Scores of some hundreds, where one key takes all the weight, and of zero."""
+    ctx, counts = [200, 90], [4, 1]
+    case = _case(ctx, counts, 4, 1, 128, 16, dtype, seed=6, spread=40.0)
+    out, lse = _run(*case, ctx, counts)
+    _check(out, lse, case, ctx, counts)
+    zero = (case[0] * 0, *case[1:])
+    out, lse = _run(*zero, ctx, counts)
+    _check(out, lse, zero, ctx, counts)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_long_contexts_are_split_and_joined(ext, cuda_device, dtype):
+    """One request over every SM, alone and beside short ones; a repeat gives the same bits."""
+    for ctx, counts in (([9001], [1]), ([6000, 3, 1500], [9, 1, 2])):
+        case = _case(ctx, counts, 4, 2, 64, 64, dtype, seed=7)
+        out, lse = _run(*case, ctx, counts)
+        _check(out, lse, case, ctx, counts)
+        out2, lse2 = _run(*case, ctx, counts)
+        assert torch.equal(out, out2) and torch.equal(lse, lse2)
+
+
+@pytest.mark.gpu
+def test_many_requests(ext, cuda_device):
+    """More requests than threads in a block, most of them without tokens."""
+    n = 700
+    counts = [1 if b % 3 == 0 else 0 for b in range(n)]
+    ctx = [(b * 37) % 90 for b in range(n)]
+    case = _case(ctx, counts, 2, 1, 64, 16, torch.bfloat16, seed=8)
+    out, lse = _run(*case, ctx, counts)
+    _check(out, lse, case, ctx, counts)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_strided_queries_and_pools(ext, cuda_device, dtype):
+    """Queries that are a slice of a projection (aligned and not), a pool that is one layer's slice."""
+    ctx, counts = [100], [3]
+    q, kp, vp, table = _case(ctx, counts, 4, 2, 64, 16, dtype, seed=9)
+    pool = torch.zeros(kp.shape[0], 2, *kp.shape[1:], dtype=dtype)
+    pool[:, 0], pool[:, 1] = kp, vp
+    dev = pool.cuda()
+    want = tree_attention(q.cuda(), kp.cuda(), vp.cuda(), table.cuda(), torch.tensor([100], dtype=torch.int32).cuda())
+    for shift in (0, 1):
+        flat = torch.zeros(3, 4 * 64 + 72, dtype=dtype, device="cuda")
+        flat[:, shift:shift + 256] = q.flatten(1).cuda()
+        got = tree_attention(flat[:, shift:shift + 256].unflatten(1, (4, 64)), dev[:, 0], dev[:, 1],
+                             table.cuda(), torch.tensor([100], dtype=torch.int32).cuda())
+        assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_bad_pages_and_lengths_are_reported(ext, cuda_device, dtype):
+    """A page outside the pool reads as zeros, a context longer than the table ends with it; neither faults."""
+    ctx, counts = [60, 60], [2, 2]
+    q, kp, vp, table = _case(ctx, counts, 2, 1, 64, 16, dtype, seed=10)
+    good = table.clone()
+    table[0, 1] = 10 ** 6
+    table[1, 2] = -3
+    st = new_status("cuda")
+    out, _ = _run(q, kp, vp, table, ctx, counts, status=st)
+    with pytest.raises(DeviceTimeout, match="code=2"):
+        check_status(st)
+    assert torch.isfinite(out).all()
+    out, lse = _run(q, kp, vp, good[:, :4], [63, 2 ** 31 - 5], counts)  # the table has room for 64
+    assert torch.isfinite(out).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_streams_and_graphs(ext, cuda_device, dtype):
+    """Two captured calls replayed at the same time, and a call on a side stream."""
+    ctx, counts = [700, 30], [3, 6]
+    cases = [_case(ctx, counts, 8, 2, 128, 16, dtype, seed=s) for s in (11, 12)]
+    cu = torch.tensor([0] + counts).cumsum(0).int().cuda()
+    ctx_t = torch.tensor(ctx, dtype=torch.int32).cuda()
+    dev = [[x.cuda() for x in c] for c in cases]
+    want = [tree_attention(*d, ctx_t, cu) for d in dev]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in dev]
+    graphs, outs = [], []
+    for d, s in zip(dev, streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            outs.append(tree_attention(*d, ctx_t, cu))
+        graphs.append(g)
+    for _ in range(5):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        assert torch.equal(o, w)
+    with torch.cuda.stream(streams[0]):
+        got = tree_attention(*dev[1], ctx_t, cu)
+    streams[0].synchronize()
+    assert torch.equal(got, want[1])
+
+
+@pytest.mark.gpu
+def test_empty_call(ext, cuda_device):
+    case = _case([5], [0], 2, 1, 64, 16, torch.bfloat16)
+    out, lse = _run(*case, [5], [0])
+    assert out.shape == (0, 2, 64) and lse.shape == (0, 2)
