@@ -127,6 +127,8 @@ struct TreePlan {
 
 TreePlan tree_plan(Elem elem, const TreeParams& p, int max_q, int sms);
 int tree_launch(Elem elem, const TreeParams& p, const TreePlan& plan, cudaStream_t stream);
+// the tensor-core kernel of bf16 and fp16 (tree_launch calls it); 128 or 256 rows per unit
+int tree_sm100_launch(Elem elem, const TreeParams& p, int rows_per_unit, cudaStream_t stream);
 
 // ancestor bits and depths of drafted trees from parent indices
 int tree_mask_launch(const int* parents, const int* cu, int batch, int uniform, int total,

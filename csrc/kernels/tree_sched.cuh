@@ -26,7 +26,7 @@ constexpr int kMetaInts = 8;
 struct Request {
   int first;   // first packed token
   int tokens;  // new tokens (clamped to what the tensors hold)
-  int ctx;     // cached tokens before them
+  int ctx;     // cached tokens before them, at most the table's room
   int keys;    // keys that exist: ctx + tokens, at most the table's room
 };
 
@@ -41,10 +41,9 @@ __device__ __forceinline__ Request load_request(const TreeParams& p, int b) {
     end = max(r.first, min(p.cu[b + 1], p.total));
   }
   r.tokens = end - r.first;
-  r.ctx = max(0, p.ctx[b]);
-  const long long room = static_cast<long long>(p.table_w) * p.page_size;
-  const long long keys = static_cast<long long>(r.ctx) + r.tokens;
-  r.keys = static_cast<int>(keys < room ? keys : room);
+  const int room = p.table_w * p.page_size;  // at most 2^30 (checked by the bindings)
+  r.ctx = max(0, min(p.ctx[b], room));
+  r.keys = min(r.ctx + r.tokens, room);
   return r;
 }
 
@@ -56,13 +55,12 @@ __device__ __forceinline__ int row_tiles(const TreeParams& p, const Request& r, 
 // them; a mask bounds them by the request's last token.
 template <int kTile>
 __device__ __forceinline__ int unit_tiles(const TreeParams& p, const Request& r, int t, int rows) {
-  long long keys = r.keys;
+  int keys = r.keys;
   if (p.mask == nullptr) {
-    const long long last = min(static_cast<long long>(r.tokens) - 1,
-                               ((static_cast<long long>(t) + 1) * rows - 1) / p.group);
-    keys = min(keys, r.ctx + last + 1);
+    const long long last = ((static_cast<long long>(t) + 1) * rows - 1) / p.group;
+    if (last < r.tokens) keys = min(keys, r.ctx + static_cast<int>(last) + 1);
   }
-  return static_cast<int>((keys + kTile - 1) / kTile);
+  return (keys + kTile - 1) / kTile;
 }
 
 // places of one kv head of a request
@@ -117,6 +115,9 @@ __device__ __forceinline__ Range find_range(const TreeParams& p, int rows, long 
       long long mine = 0;
       if (b < p.batch) {
         const Request r = load_request(p, b);
+        if (pass == 0 && blockIdx.x == 0 && r.tokens > 0 &&
+            (p.ctx[b] < 0 || r.keys - r.tokens != p.ctx[b]))
+          st_record(p.status, kStatusBadArgs, kBadPosition, b);  // longer than its table
         mine = head_places<kTile>(p, r, rows) * p.heads_kv;
       }
       long long inc = mine;  // inclusive sum over the warp
@@ -213,8 +214,9 @@ struct Walk {
       c.ctx = r.ctx;
       c.tokens = r.tokens;
       c.keys = r.keys;
+      const int cta = 2 * static_cast<int>(blockIdx.x);
       const bool from_start = c.tile_begin == 0, to_end = c.tile_end == tiles;
-      c.record = from_start ? (to_end ? -1 : 2 * blockIdx.x + 1) : 2 * blockIdx.x;
+      c.record = from_start ? (to_end ? -1 : cta + 1) : cta;
       merges = to_end && !from_start;
       if (merges) merge_c0 = range_owner(g.total, g.grid, unit_at + kUnitCost);
       const bool have = c.tile_end > c.tile_begin || tiles == 0;

@@ -43,35 +43,11 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool v
                : "memory");
 }
 
-template <typename T>
-__device__ __forceinline__ float4 ld4(const T* p);
-template <>
-__device__ __forceinline__ float4 ld4<float>(const float* p) {
+__device__ __forceinline__ float4 ld4(const float* p) {
   return *reinterpret_cast<const float4*>(p);
 }
-template <>
-__device__ __forceinline__ float4 ld4<__nv_bfloat16>(const __nv_bfloat16* p) {
-  const uint2 u = *reinterpret_cast<const uint2*>(p);
-  const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x));
-  const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
-  return make_float4(a.x, a.y, b.x, b.y);
-}
-template <>
-__device__ __forceinline__ float4 ld4<__half>(const __half* p) {
-  const uint2 u = *reinterpret_cast<const uint2*>(p);
-  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
-  const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
-  return make_float4(a.x, a.y, b.x, b.y);
-}
-__device__ __forceinline__ float ld1(float x) { return x; }
-__device__ __forceinline__ float ld1(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float ld1(__half x) { return __half2float(x); }
 template <typename T>
 __device__ __forceinline__ T cast_out(float x);
-template <>
-__device__ __forceinline__ float cast_out<float>(float x) {
-  return x;
-}
 template <>
 __device__ __forceinline__ __nv_bfloat16 cast_out<__nv_bfloat16>(float x) {
   return __float2bfloat16_rn(x);
@@ -81,12 +57,11 @@ __device__ __forceinline__ __half cast_out<__half>(float x) {
   return __float2half_rn(x);
 }
 
-template <typename T, int D>
+template <int D>
 struct SimtCfg {
-  static constexpr int kPad = 16 / sizeof(T);  // K rows shifted by 16 bytes: lanes of 8 keys hit all banks
-  static constexpr int kKRow = D + kPad;
-  static constexpr int kKBytes = kSimtTile * kKRow * sizeof(T);
-  static constexpr int kVBytes = kSimtTile * D * sizeof(T);
+  static constexpr int kKRow = D + 4;  // K rows shifted by 16 bytes: lanes of 8 keys hit all banks
+  static constexpr int kKBytes = kSimtTile * kKRow * 4;
+  static constexpr int kVBytes = kSimtTile * D * 4;
   static constexpr int kStage = kKBytes + kVBytes;
   static constexpr int kQRow = D + 4;
   static constexpr int kQBytes = kSimtRows * kQRow * 4;
@@ -96,10 +71,10 @@ struct SimtCfg {
   static constexpr int kSmem = kStages + kQBytes + kPBytes;
 };
 
-template <typename T, int D>
+template <int D>
 __global__ void __launch_bounds__(kSimtThreads)
     tree_simt_kernel(const __grid_constant__ TreeParams p) {
-  using C = SimtCfg<T, D>;
+  using C = SimtCfg<D>;
   constexpr int kCols = D / 32;
   extern __shared__ __align__(16) uint8_t smem[];
   float* sQ = reinterpret_cast<float*>(smem + C::kStages);
@@ -128,8 +103,8 @@ __global__ void __launch_bounds__(kSimtThreads)
     __syncthreads();
     if (!s_have) break;
     const Piece c = s_piece;
-    const T* kb = static_cast<const T*>(p.k) + static_cast<int64_t>(c.head_kv) * p.page_size * D;
-    const T* vb = static_cast<const T*>(p.v) + static_cast<int64_t>(c.head_kv) * p.page_size * D;
+    const float* kb = static_cast<const float*>(p.k) + static_cast<int64_t>(c.head_kv) * p.page_size * D;
+    const float* vb = static_cast<const float*>(p.v) + static_cast<int64_t>(c.head_kv) * p.page_size * D;
     const int* table = p.table + static_cast<int64_t>(c.request) * p.table_stride;
 
     // queries, scaled to base-2 exponents
@@ -138,7 +113,7 @@ __global__ void __launch_bounds__(kSimtThreads)
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       if (r < c.rows) {
         const int row = c.row0 + r, t = row / p.group, h = c.head_kv * p.group + row % p.group;
-        v = ld4<T>(static_cast<const T*>(p.q) + (c.first + t) * p.q_t + h * p.q_h + x);
+        v = ld4(static_cast<const float*>(p.q) + (c.first + t) * p.q_t + h * p.q_h + x);
         v.x *= p.scale_log2;
         v.y *= p.scale_log2;
         v.z *= p.scale_log2;
@@ -147,7 +122,7 @@ __global__ void __launch_bounds__(kSimtThreads)
       *reinterpret_cast<float4*>(sQ + r * C::kQRow + x) = v;
     }
     auto load = [&](int tile, int stage) {
-      constexpr int kChunks = D * sizeof(T) / 16;
+      constexpr int kChunks = D * 4 / 16;
       const uint32_t sk = sm100::smem_u32(smem) + stage * C::kStage;
       const uint32_t sv = sk + C::kKBytes;
 #pragma unroll 4
@@ -167,9 +142,9 @@ __global__ void __launch_bounds__(kSimtThreads)
             page = 0;
           }
         }
-        const int at = off * D + x * (16 / static_cast<int>(sizeof(T)));
-        cp_async16(sk + r * C::kKRow * sizeof(T) + x * 16, kb + page * p.k_page + at, ok);
-        cp_async16(sv + r * D * sizeof(T) + x * 16, vb + page * p.v_page + at, ok);
+        const int at = off * D + x * 4;
+        cp_async16(sk + r * C::kKRow * 4 + x * 16, kb + page * p.k_page + at, ok);
+        cp_async16(sv + r * D * 4 + x * 16, vb + page * p.v_page + at, ok);
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -194,14 +169,14 @@ __global__ void __launch_bounds__(kSimtThreads)
         asm volatile("cp.async.wait_group 0;" ::: "memory");
       }
       __syncthreads();
-      const T* sk = reinterpret_cast<const T*>(smem + stage * C::kStage);
-      const T* sv = reinterpret_cast<const T*>(smem + stage * C::kStage + C::kKBytes);
+      const float* sk = reinterpret_cast<const float*>(smem + stage * C::kStage);
+      const float* sv = reinterpret_cast<const float*>(smem + stage * C::kStage + C::kKBytes);
       float s[4] = {0.f, 0.f, 0.f, 0.f};
-      const T* krow = sk + (warp * 16 + key) * C::kKRow;
+      const float* krow = sk + (warp * 16 + key) * C::kKRow;
       const float* qrow = sQ + half * 4 * C::kQRow;
 #pragma unroll 8
       for (int x = 0; x < D; x += 4) {
-        const float4 kv = ld4<T>(krow + x);
+        const float4 kv = ld4(krow + x);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float4 qv = *reinterpret_cast<const float4*>(qrow + i * C::kQRow + x);
@@ -251,14 +226,14 @@ __global__ void __launch_bounds__(kSimtThreads)
 #pragma unroll
         for (int x = 0; x < kCols; ++x) acc[r][x] *= a;
       }
-      const T* vcol = sv + warp * 16 * D + lane * kCols;
+      const float* vcol = sv + warp * 16 * D + lane * kCols;
 #pragma unroll
       for (int k4 = 0; k4 < 16; k4 += 4) {
         float v[4][kCols];
 #pragma unroll
         for (int u = 0; u < 4; ++u)
 #pragma unroll
-          for (int x = 0; x < kCols; ++x) v[u][x] = ld1(vcol[(k4 + u) * D + x]);
+          for (int x = 0; x < kCols; ++x) v[u][x] = vcol[(k4 + u) * D + x];
 #pragma unroll
         for (int r = 0; r < kSimtRows; ++r) {
           const float4 pr = *reinterpret_cast<const float4*>(sP + (warp * kSimtRows + r) * 16 + k4);
@@ -312,8 +287,8 @@ __global__ void __launch_bounds__(kSimtThreads)
         }
       } else {
         const int row = c.row0 + r, t = row / p.group, h = c.head_kv * p.group + row % p.group;
-        static_cast<T*>(p.out)[(c.first + t) * p.out_t + h * p.out_h + x] =
-            cast_out<T>(sum == 0.f ? 0.f : o / sum);
+        static_cast<float*>(p.out)[(c.first + t) * p.out_t + h * p.out_h + x] =
+            sum == 0.f ? 0.f : o / sum;
         if (x == 0 && p.lse != nullptr)
           p.lse[static_cast<int64_t>(c.first + t) * p.heads + h] =
               sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2f;
@@ -375,25 +350,28 @@ __global__ void __launch_bounds__(kMergeThreads)
   }
 }
 
-template <typename T, int D>
-int run_simt(const TreeParams& p, const TreePlan& plan, cudaStream_t stream) {
-  using C = SimtCfg<T, D>;
+template <int D>
+int run_simt(const TreeParams& p, cudaStream_t stream) {
+  using C = SimtCfg<D>;
   static bool done[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !done[dev]) {
     const cudaError_t err = cudaFuncSetAttribute(
-        tree_simt_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+        tree_simt_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
     if (err != cudaSuccess) return static_cast<int>(err);
     if (dev >= 0 && dev < 64) done[dev] = true;
   }
-  tree_simt_kernel<T, D><<<plan.grid, kSimtThreads, C::kSmem, stream>>>(p);
-  int err = static_cast<int>(cudaGetLastError());
-  if (err != 0) return err;
+  tree_simt_kernel<D><<<p.grid, kSimtThreads, C::kSmem, stream>>>(p);
+  return static_cast<int>(cudaGetLastError());
+}
+
+template <typename T, int D>
+int run_merge(const TreeParams& p, int rows_per_unit, cudaStream_t stream) {
   constexpr int kRows = kMergeThreads / (D / 4);
-  const int gy = (plan.rows_per_unit + kRows - 1) / kRows;
+  const int gy = (rows_per_unit + kRows - 1) / kRows;
   tree_merge_kernel<T, D>
-      <<<dim3(plan.grid, gy < 8 ? gy : 8), kMergeThreads, 0, stream>>>(p, plan.rows_per_unit);
+      <<<dim3(p.grid, gy < 8 ? gy : 8), kMergeThreads, 0, stream>>>(p, rows_per_unit);
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -452,14 +430,16 @@ __global__ void pack_mask_kernel(const uint8_t* in, int64_t in_t, int total, int
 
 TreePlan tree_plan(Elem elem, const TreeParams& p, int max_q, int sms) {
   TreePlan plan;
-  (void)max_q;
-  plan.rows_per_unit = kSimtRows;
-  const int smem = p.dim == 64 ? (elem == Elem::kF32 ? SimtCfg<float, 64>::kSmem
-                                                     : SimtCfg<__half, 64>::kSmem)
-                               : (elem == Elem::kF32 ? SimtCfg<float, 128>::kSmem
-                                                     : SimtCfg<__half, 128>::kSmem);
-  const int per_sm = (227 * 1024) / (smem + 2048);
-  plan.grid = sms * (per_sm < 1 ? 1 : (per_sm > 8 ? 8 : per_sm));
+  if (elem == Elem::kF32) {
+    plan.rows_per_unit = kSimtRows;
+    const int smem = p.dim == 64 ? SimtCfg<64>::kSmem : SimtCfg<128>::kSmem;
+    plan.grid = sms * ((227 * 1024) / (smem + 2048));
+  } else {
+    // one row tile keeps two key tiles in the air per CTA and suits what reading
+    // the cache bounds; from the second row tile on, both share every key tile
+    plan.rows_per_unit = static_cast<int64_t>(max_q) * p.group > 128 ? 256 : 128;
+    plan.grid = sms;
+  }
   const size_t rows = static_cast<size_t>(2) * plan.grid * plan.rows_per_unit;
   plan.acc_floats = rows * p.dim;
   plan.ml_floats = 2 * rows;
@@ -468,16 +448,23 @@ TreePlan tree_plan(Elem elem, const TreeParams& p, int max_q, int sms) {
 }
 
 int tree_launch(Elem elem, const TreeParams& p, const TreePlan& plan, cudaStream_t stream) {
+  const int rows = plan.rows_per_unit;
+  int err;
+  if (elem == Elem::kF32)
+    err = p.dim == 64 ? run_simt<64>(p, stream) : run_simt<128>(p, stream);
+  else
+    err = tree_sm100_launch(elem, p, rows, stream);
+  if (err != 0) return err;
   switch (elem) {
     case Elem::kBF16:
-      return p.dim == 64 ? run_simt<__nv_bfloat16, 64>(p, plan, stream)
-                         : run_simt<__nv_bfloat16, 128>(p, plan, stream);
+      return p.dim == 64 ? run_merge<__nv_bfloat16, 64>(p, rows, stream)
+                         : run_merge<__nv_bfloat16, 128>(p, rows, stream);
     case Elem::kF16:
-      return p.dim == 64 ? run_simt<__half, 64>(p, plan, stream)
-                         : run_simt<__half, 128>(p, plan, stream);
+      return p.dim == 64 ? run_merge<__half, 64>(p, rows, stream)
+                         : run_merge<__half, 128>(p, rows, stream);
     default:
-      return p.dim == 64 ? run_simt<float, 64>(p, plan, stream)
-                         : run_simt<float, 128>(p, plan, stream);
+      return p.dim == 64 ? run_merge<float, 64>(p, rows, stream)
+                         : run_merge<float, 128>(p, rows, stream);
   }
 }
 

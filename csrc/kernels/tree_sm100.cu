@@ -1,0 +1,717 @@
+// tree_sm100.cu - attention of new tokens over a paged cache on the tensor
+// cores (bf16 and fp16), for B200 (sm_100a).
+//
+// The rows of a unit are the (new token, query head) pairs that share a kv head,
+// token-major, so a decoding step of 8 query heads fills 8 of the 128 rows of an
+// MMA and K and V are still read once for all of them.  Up to 128 rows the work is
+// bound by reading the cache; a tile of 128 keys (64 KB at dim 128) takes an SM
+// about 1.5 us at the measured 6.55 TB/s, while QK, softmax and PV of the tile
+// follow one another and take longer than that in a row.  So two chains run side
+// by side in one CTA:
+//   kTwoRows = 0  (a unit is 128 rows): chain x takes the key tiles of parity x,
+//                 with its own scores, maxima, sums and outputs; the two are
+//                 joined when the piece ends, as split records are joined.
+//   kTwoRows = 1  (a unit is 256 rows): chain x takes row tile x, both use every
+//                 key tile, so a tile read once serves 256 rows (work bound by the
+//                 tensor cores: chunks of prompts, wide trees).
+//
+// CTA = 12 warps, persistent over the pieces of its even share (tree_sched.cuh):
+//   warp 0      walks the pieces, looks pages up (a lane per page) and issues the
+//               TMA loads of K and V, one box per page and 64 columns
+//   warp 1      MMA issuer (one thread), TMEM owner
+//   warps 2-3   queries: gathered rows, 16-byte asynchronous copies, swizzled
+//   warps 4-7   softmax and results of chain 0, warps 8-11 of chain 1
+// TMEM: S_0 [0,128) S_1 [128,256) O_0 [256,..) O_1 [384,..); P lies over S.
+//
+// Keys no row may see: the score is replaced by -inf, so K may hold anything.  V
+// enters a product with a weight of zero, which a NaN or infinity would survive,
+// so in the tiles that hold new tokens or the end of the cache the softmax warps
+// clean V in shared memory first: rows past the end become zeros, and what is not
+// finite among the new tokens is taken out and, for the rows that do see it, added
+// to the result at the end (a path no sane cache takes).
+//
+// Every wait is bounded; no TMA load uses cluster broadcast.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "paged.h"
+#include "sm100.cuh"
+#include "tmap.h"
+#include "tree_sched.cuh"
+
+namespace rab {
+
+using namespace sm100;
+using namespace tree_detail;
+
+namespace {
+
+constexpr int kThreads = 384;
+constexpr int kN = 128;  // keys of a tile
+constexpr int kM = 128;  // rows of a chain
+constexpr uint32_t kCols = 512;
+constexpr float kRescale = 8.0f;  // the running maximum moves when it grows by 2^8
+constexpr float kLn2 = 0.69314718055994530942f;
+constexpr uint32_t kRegsLaunch = 168;
+constexpr uint32_t kRegsLow = 72;
+constexpr uint32_t kRegsHigh = 216;
+static_assert(128 * kRegsLow + 256 * kRegsHigh <= kRegsLaunch * kThreads,
+              "register split exceeds the launch allocation");
+constexpr int kItems = 4;  // queue of pieces
+
+template <int D, bool kTwoRows>
+struct Cfg {
+  static constexpr int kTile = kN * D * 2;  // bytes of a K or V tile
+  static constexpr int kQBytes = (kTwoRows ? 2 : 1) * kM * D * 2;
+  // K and V tiles take turns in one ring: what is left of 227 KB beside the queries
+  static constexpr int kStages = D == 64 ? (kTwoRows ? 10 : 12) : (kTwoRows ? 5 : 6);
+  static constexpr int kBars = 2 * kStages + 2 + 2 + 2 + 4 + 2 * kItems;
+  static constexpr int kBarOff = kQBytes + kStages * kTile;
+  static constexpr int kMlOff = kBarOff + kBars * 8;       // float2 [2][128]
+  static constexpr int kItemOff = kMlOff + 2 * kM * 8;     // Piece [kItems]
+  static constexpr int kSumOff = kItemOff + kItems * 48;   // long long [12 + 1]
+  static constexpr int kMiscOff = kSumOff + 13 * 8;        // int [8]
+  static constexpr int kSmem = kMiscOff + 32;
+  static_assert(kMlOff % 8 == 0 && kSumOff % 8 == 0 && kSmem <= 232448, "shared memory");
+  static_assert(sizeof(Piece) <= 48, "piece");
+};
+
+template <bool kBF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (kBF16) return pack_bf16x2(lo, hi);
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+template <bool kBF16>
+__device__ __forceinline__ bool not_finite(uint32_t h) {  // the low 16 bits
+  constexpr uint32_t e = kBF16 ? 0x7f80u : 0x7c00u;
+  return (h & e) == e;
+}
+
+template <bool kBF16>
+__device__ __forceinline__ float widen(uint32_t h) {
+  if constexpr (kBF16) return __uint_as_float(h << 16);
+  float f;
+  asm("{\n\t.reg .b16 t;\n\tcvt.u16.u32 t, %1;\n\tcvt.f32.f16 %0, t;\n\t}" : "=f"(f) : "r"(h));
+  return f;
+}
+
+// The 32 columns of new tokens rel0 .. rel0 + 31 that token t of the request
+// sees, as bits; places before the new tokens (rel < 0) are cached and seen.
+__device__ __forceinline__ uint32_t seen_bits(const TreeParams& p, const Piece& c, int t,
+                                              int rel0) {
+  int n = min(c.tokens, c.keys - c.ctx) - rel0;  // columns that hold a key
+  uint32_t bits;
+  if (p.mask == nullptr) {
+    n = min(n, t - rel0 + 1);
+    bits = 0xffffffffu;
+  } else {
+    const uint32_t* row = p.mask + static_cast<int64_t>(c.first + t) * p.mask_stride;
+    const int w = rel0 >> 5, sh = rel0 & 31;
+    auto word = [&](int i) { return i < 0 ? 0xffffffffu : (i < p.mask_w ? row[i] : 0u); };
+    const uint32_t lo = word(w);
+    const uint32_t hi = sh ? word(w + 1) : 0u;
+    bits = __funnelshift_r(lo, hi, sh);
+  }
+  if (n <= 0) return 0u;
+  return n < 32 ? bits & ((1u << n) - 1u) : bits;
+}
+
+template <int D, bool kBF16, bool kTwoRows>
+__global__ void __launch_bounds__(kThreads, 1)
+    tree_attn_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap tmK,
+                     const __grid_constant__ CUtensorMap tmV) {
+  using C = Cfg<D, kTwoRows>;
+  constexpr int NS = C::kStages;
+  constexpr int kRows = kTwoRows ? 2 * kM : kM;
+  constexpr uint32_t kFmt = kBF16 ? kFmtBF16 : kFmtF16;
+  constexpr uint32_t kIdescQK = make_idesc(kFmt, kFmt, kM, kN, kMajorK, kMajorK);
+  constexpr uint32_t kIdescPV = make_idesc(kFmt, kFmt, kM, D, kMajorK, kMajorMN);
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t* sQ = smem;
+  uint8_t* sKV = smem + C::kQBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBarOff);  // [NS]
+  uint64_t* empty = full + NS;                                      // [NS]
+  uint64_t* q_full = empty + NS;
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* s_full = q_full + 2;  // [2]
+  uint64_t* p_full = q_full + 4;  // [2]
+  uint64_t* o_final = q_full + 6;
+  uint64_t* o_free = q_full + 7;
+  uint64_t* joined = q_full + 8;
+  uint64_t* drain = q_full + 9;
+  uint64_t* item_full = q_full + 10;           // [kItems]
+  uint64_t* item_empty = item_full + kItems;   // [kItems]
+  float2* s_ml = reinterpret_cast<float2*>(smem + C::kMlOff);
+  long long* s_sums = reinterpret_cast<long long*>(smem + C::kSumOff);
+  int* s_misc = reinterpret_cast<int*>(smem + C::kMiscOff);
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_misc);
+  int* s_request = s_misc + 1;
+  volatile int* s_dirty = s_misc + 2;  // [2], by the piece's parity
+  auto item_slot = [&](int w) {
+    return reinterpret_cast<Piece*>(smem + C::kItemOff + (w % kItems) * 48);
+  };
+
+  const uint32_t warp = warp_id();
+  DeviceStatus* st = p.status;
+  const uint64_t tmo = p.timeout_ns;
+  // the swizzle of the tiles counts from 1024-byte boundaries; the block has no
+  // other shared memory, so its dynamic part starts on one
+  if ((smem_u32(smem) & 1023u) != 0) {
+    if (threadIdx.x == 0) {
+      p.meta[blockIdx.x * kMetaInts] = 0;
+      st_record(st, kStatusBadArgs, kSiteNone);
+    }
+    return;
+  }
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(q_full, 64);
+    mbar_init(q_empty, 1);
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&s_full[x], 1);
+      mbar_init(&p_full[x], 4);
+    }
+    mbar_init(o_final, 1);
+    mbar_init(o_free, 8);
+    mbar_init(joined, 8);
+    mbar_init(drain, 1);
+    for (int i = 0; i < kItems; ++i) {
+      mbar_init(&item_full[i], 1);
+      mbar_init(&item_empty[i], 1 + 2 + 8);  // MMA thread, query warps, softmax warps
+    }
+    s_dirty[0] = s_dirty[1] = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(s_tmem, kCols);
+    tmem_relinquish();
+  }
+  const Range range = find_range<kN, kThreads>(p, kRows, s_sums, s_request, s_sums + 12);
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;
+
+  if (warp < 4) {
+    warpgroup_reg_dec<kRegsLow>();
+    if (warp == 0) {
+      // ------------------------------------------------------ pieces and loads
+      const int lane = lane_id();
+      Walk<kN> walk;
+      if (lane == 0) {
+        tma_prefetch_desc(&tmK);
+        tma_prefetch_desc(&tmV);
+        walk.start(p, range, kRows);
+        p.meta[blockIdx.x * kMetaInts] = 0;
+      }
+      const int rows_box = min(p.page_size, kN);
+      const int boxes = kN / rows_box * (D / 64);
+      int n = 0;  // loads issued (K and V tiles)
+      bool ok = true;
+      for (int w = 0; ok; ++w) {
+        if (w >= kItems)
+          ok = __all_sync(0xffffffffu, mbar_wait(&item_empty[w % kItems], (w / kItems - 1) & 1, st,
+                                                 kSiteItemQueue, tmo));
+        if (!ok) break;
+        Piece* slot = item_slot(w);
+        if (lane == 0) {
+          Piece c;
+          if (walk.next(p, range, kRows, &c)) {
+            if (walk.merges) write_meta(p, c, true, walk.merge_c0);
+          } else {
+            c.request = -1;
+          }
+          *slot = c;
+        }
+        __syncwarp();
+        const Piece c = *slot;
+        if (lane == 0) mbar_arrive(&item_full[w % kItems]);
+        if (c.request < 0) break;
+        const int* table = p.table + static_cast<int64_t>(c.request) * p.table_stride;
+        const int last_entry = (c.keys - 1) / p.page_size;
+        for (int tile = c.tile_begin; tile < c.tile_end && ok; ++tile) {
+          // this lane's box: page, rows within the tile, 64-column half
+          const int half = lane % (D / 64), part = lane / (D / 64);
+          int page = p.num_pages, token = 0;
+          if (lane < boxes) {
+            const int key = tile * kN + part * rows_box;
+            const int entry = key / p.page_size;
+            token = key - entry * p.page_size;
+            // behind the last key: a page coordinate past the pool loads zeros
+            if (entry <= last_entry) {
+              page = table[entry];
+              if (page < 0 || page >= p.num_pages) {
+                if (half == 0) st_record(st, kStatusBadArgs, kBadPage, static_cast<uint32_t>(page));
+                page = p.num_pages;
+              }
+            }
+          }
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv) {
+            const int stage = n % NS;
+            ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], ((n / NS) & 1) ^ 1, st,
+                                                   kv ? kSiteVEmpty : kSiteKEmpty, tmo));
+            if (!ok) break;
+            if (lane == 0) mbar_arrive_expect_tx(&full[stage], C::kTile);
+            __syncwarp();
+            if (lane < boxes)
+              tma_load_4d(sKV + stage * C::kTile + half * (kN * 128) + part * rows_box * 128,
+                          kv ? &tmV : &tmK, &full[stage], half * 64, token, c.head_kv, page);
+            ++n;
+          }
+        }
+      }
+      if (!ok) {  // the loads in flight land before the block gives its memory back
+        for (int i = 0; i < NS && i < n; ++i) {
+          const int k = n - 1 - i;
+          mbar_wait(&full[k % NS], (k / NS) & 1, nullptr, kSiteKFull, 100000000ull);
+        }
+      }
+    } else if (warp == 1) {
+      // ------------------------------------------------------------------ MMA
+      if (elect_one()) {
+        int g0 = 0;  // tiles of the pieces before this one
+        int px[2] = {0, 0};  // P tiles taken from each chain
+        bool ok = true;
+        const uint32_t kvb = smem_u32(sKV), qb0 = smem_u32(sQ);
+        auto wait_tile = [&](int idx, uint32_t site) {
+          return mbar_wait(&full[idx % NS], (idx / NS) & 1, st, site, tmo);
+        };
+        auto qk = [&](int x, int g, int qtile) {
+          const uint32_t kb = kvb + (2 * g % NS) * C::kTile;
+          const uint32_t qb = qb0 + qtile * (kM * D * 2);
+#pragma unroll
+          for (int ks = 0; ks < D / 16; ++ks) {
+            const uint32_t sub = ks >> 2, inner = (ks & 3) * 32;
+            mma_ss<false>(tmem + x * 128, make_sdesc(qb + sub * (kM * 128) + inner, 16, 1024),
+                          make_sdesc(kb + sub * (kN * 128) + inner, 16, 1024), kIdescQK,
+                          ks ? 1u : 0u);
+          }
+          mma_commit(&s_full[x]);
+        };
+        auto pv = [&](int x, int g, bool first) {
+          const uint32_t vb = kvb + ((2 * g + 1) % NS) * C::kTile;
+#pragma unroll
+          for (int ks = 0; ks < kN / 16; ++ks)
+            mma_ts<false>(tmem + 256 + x * 128, tmem + x * 128 + ks * 8,
+                          make_sdesc(vb + ks * 2048, kN * 128, 1024), kIdescPV,
+                          (first && ks == 0) ? 0u : 1u);
+        };
+        auto wait_p = [&](int x) {
+          return mbar_wait(&p_full[x], px[x] & 1, st, kSitePFull, tmo);
+        };
+        for (int w = 0; ok; ++w) {
+          ok = mbar_wait(&item_full[w % kItems], (w / kItems) & 1, st, kSiteItemQueue, tmo);
+          if (!ok) break;
+          const Piece c = *item_slot(w);
+          mbar_arrive(&item_empty[w % kItems]);
+          if (c.request < 0) break;
+          const int n = c.tile_end - c.tile_begin;
+          ok = mbar_wait(q_full, w & 1, st, kSiteQFull, tmo);
+          if (!ok) break;
+          tc_fence_after();
+          // the results of the piece before have left the accumulators
+          auto wait_o = [&]() {
+            return w == 0 || mbar_wait(o_free, (w - 1) & 1, st, kSiteOReady, tmo);
+          };
+          if constexpr (!kTwoRows) {
+            auto next_qk = [&](int j) -> bool {
+              if (!wait_tile(2 * (g0 + j), kSiteKFull)) return false;
+              tc_fence_after();
+              qk(j & 1, g0 + j, 0);
+              mma_commit(&empty[2 * (g0 + j) % NS]);
+              if (j == n - 1) mma_commit(q_empty);
+              return true;
+            };
+            ok = next_qk(0) && (n < 2 || next_qk(1));
+            for (int j = 0; j < n && ok; ++j) {
+              const int x = j & 1;
+              ok = wait_p(x) && wait_tile(2 * (g0 + j) + 1, kSiteVFull) && (j > 0 || wait_o());
+              if (!ok) break;
+              ++px[x];
+              tc_fence_after();
+              pv(x, g0 + j, j < 2);
+              mma_commit(&empty[(2 * (g0 + j) + 1) % NS]);
+              if (j + 2 < n) ok = next_qk(j + 2);
+            }
+          } else {
+            auto do_pv = [&](int x, int j) -> bool {
+              if (!wait_p(x)) return false;
+              // a tile whose V both chains clean: each has done its half
+              if (x == 0 && (c.tile_begin + j + 1) * kN > c.ctx && !wait_p(1)) return false;
+              if (x == 0 && !wait_tile(2 * (g0 + j) + 1, kSiteVFull)) return false;
+              if (x == 0 && j == 0 && !wait_o()) return false;
+              ++px[x];
+              tc_fence_after();
+              pv(x, g0 + j, j == 0);
+              if (x == 1) mma_commit(&empty[(2 * (g0 + j) + 1) % NS]);
+              return true;
+            };
+            for (int j = 0; j < n && ok; ++j) {
+              ok = wait_tile(2 * (g0 + j), kSiteKFull);
+              if (!ok) break;
+              tc_fence_after();
+              qk(0, g0 + j, 0);
+              if (j > 0) {
+                ok = do_pv(1, j - 1);
+                if (!ok) break;
+              }
+              qk(1, g0 + j, 1);
+              mma_commit(&empty[2 * (g0 + j) % NS]);
+              if (j == n - 1) mma_commit(q_empty);
+              ok = do_pv(0, j);
+            }
+            if (ok) ok = do_pv(1, n - 1);
+          }
+          if (!ok) break;
+          mma_commit(o_final);
+          g0 += n;
+        }
+        mma_commit(drain);
+        mbar_wait(drain, 0, nullptr, kSiteOReady, 1000000000ull);
+      }
+    } else {
+      // -------------------------------------------------------------- queries
+      const int tid = threadIdx.x - 64;
+      bool ok = true;
+      for (int w = 0; ok; ++w) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&item_full[w % kItems], (w / kItems) & 1, st,
+                                               kSiteItemQueue, tmo));
+        if (!ok) break;
+        const Piece c = *item_slot(w);
+        __syncwarp();
+        if (lane_id() == 0) mbar_arrive(&item_empty[w % kItems]);
+        if (c.request < 0) break;
+        ok = __all_sync(0xffffffffu, mbar_wait(q_empty, (w & 1) ^ 1, st, kSiteQFull, tmo));
+        if (!ok) break;
+        // rows behind the unit's last keep what they held: an MMA row is its own
+        constexpr int kChunks = D / 8;
+        const uint32_t qb = smem_u32(sQ);
+        const int h0 = c.head_kv * p.group;
+        for (int i = tid; i < c.rows * kChunks; i += 64) {
+          const int r = i / kChunks, x = i % kChunks;
+          const int row = c.row0 + r, t = row / p.group, h = h0 + row - t * p.group;
+          const uint16_t* src = static_cast<const uint16_t*>(p.q) +
+                                static_cast<int64_t>(c.first + t) * p.q_t + h * p.q_h + x * 8;
+          const uint32_t dst = qb + (r / kM) * (kM * D * 2) + (x / 8) * (kM * 128) +
+                               (r % kM) * 128 + (((x % 8) ^ (r & 7)) << 4);
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        fence_proxy_async_smem();
+        mbar_arrive(q_full);
+      }
+    }
+  } else {
+    warpgroup_reg_inc<kRegsHigh>();
+    // -------------------------------------------------------------- softmax
+    const int x = (warp - 4) >> 2;
+    const int row = (threadIdx.x - 128) & 127;
+    const uint32_t lane_base = ((warp & 3) * 32) << 16;
+    const uint32_t s_col = tmem + lane_base + x * 128;
+    // a scale of zero or below is applied before the mask and the maximum
+    const bool flip = !(p.scale_log2 > 0.f);
+    const float sl2 = flip ? 1.f : p.scale_log2;
+    int g0 = 0;
+    int sx = 0;  // tiles this chain has seen
+    bool ok = true;
+    for (int w = 0; ok; ++w) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&item_full[w % kItems], (w / kItems) & 1, st,
+                                             kSiteItemQueue, tmo));
+      if (!ok) break;
+      const Piece c = *item_slot(w);
+      if (c.request < 0) break;
+      const int n = c.tile_end - c.tile_begin;
+      const int r = kTwoRows ? x * kM + row : row;  // row of the unit
+      // a warp without rows only keeps the order of things
+      const bool active = r - static_cast<int>(lane_id()) < c.rows;
+      const int token = min(c.row0 + r, c.row0 + c.rows - 1) / p.group;
+      const uint32_t o_col = tmem + lane_base + 256 + x * 128;
+      float m_run = -INFINITY, l_run = 0.f;
+      bool begun = false;
+      for (int j = kTwoRows ? 0 : x; j < n; j += kTwoRows ? 1 : 2) {
+        const int k0 = (c.tile_begin + j) * kN;
+        const bool tail = k0 + kN > c.ctx;
+        if (tail) {
+          // clean V: 16 bytes a step; with two row tiles each chain takes half the rows
+          const int idx = 2 * (g0 + j) + 1;
+          ok = __all_sync(0xffffffffu,
+                          mbar_wait(&full[idx % NS], (idx / NS) & 1, st, kSiteVFull, tmo));
+          if (!ok) break;
+          uint8_t* vt = sKV + (idx % NS) * C::kTile;
+          constexpr int kPerRow = D / 8;
+          constexpr int kVRows = kTwoRows ? kN / 2 : kN;
+          bool dirty = false;
+          for (int i = row; i < kVRows * kPerRow; i += 128) {
+            const int vr = i / kPerRow + (kTwoRows ? x * kVRows : 0), ch = i % kPerRow;
+            const int rel = k0 + vr - c.ctx;
+            if (rel < 0) continue;
+            uint4* at = reinterpret_cast<uint4*>(vt + (ch / 8) * (kN * 128) + vr * 128 +
+                                                 (ch % 8) * 16);
+            if (k0 + vr >= c.keys) {
+              *at = make_uint4(0u, 0u, 0u, 0u);
+            } else {
+              uint4 v = *at;
+              bool hit = false;
+              uint32_t* e = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+              for (int u = 0; u < 4; ++u) {
+                if (not_finite<kBF16>(e[u])) e[u] &= 0xffff0000u, hit = true;
+                if (not_finite<kBF16>(e[u] >> 16)) e[u] &= 0x0000ffffu, hit = true;
+              }
+              if (hit) *at = v, dirty = true;
+            }
+          }
+          if (dirty) s_dirty[w & 1] = w + 1;
+          fence_proxy_async_smem();
+        }
+        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[x], sx & 1, st, kSiteSFull, tmo));
+        if (!ok) break;
+        ++sx;
+        tc_fence_after();
+        if (active) {
+          uint32_t sr[kN];
+#pragma unroll
+          for (int k = 0; k < kN; k += 32) tmem_ld32(s_col + k, sr + k);
+          tmem_ld_wait();
+          if (flip) {
+#pragma unroll
+            for (int k = 0; k < kN; ++k)
+              sr[k] = __float_as_uint(__uint_as_float(sr[k]) * p.scale_log2);
+          }
+          if (tail) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const uint32_t bits = seen_bits(p, c, token, k0 + 32 * q - c.ctx);
+#pragma unroll
+              for (int k = 0; k < 32; ++k)
+                if (!((bits >> k) & 1u)) sr[32 * q + k] = 0xff800000u;  // -inf
+            }
+          }
+          float pm[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) pm[i] = __uint_as_float(sr[i]);
+#pragma unroll
+          for (int k = 8; k < kN; k += 2)
+            pm[(k >> 1) & 7] =
+                fmax3(pm[(k >> 1) & 7], __uint_as_float(sr[k]), __uint_as_float(sr[k + 1]));
+          const float mx = fmaxf(fmax3(fmax3(pm[0], pm[1], pm[2]), fmax3(pm[3], pm[4], pm[5]),
+                                       pm[6]),
+                                 pm[7]) * sl2;
+          const bool need = mx > m_run + kRescale;
+          float alpha = 1.f;
+          if (need) {
+            alpha = m_run == -INFINITY ? 0.f : ex2_approx(m_run - mx);
+            m_run = mx;
+            l_run *= alpha;
+          }
+          // the scores' commit covers this chain's products before them: O is at rest
+          if (begun && __any_sync(0xffffffffu, need)) {
+#pragma unroll
+            for (int k = 0; k < D; k += 32) {
+              uint32_t o[32];
+              tmem_ld32(o_col + k, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st32(o_col + k, o);
+            }
+          }
+          const float m_use = m_run == -INFINITY ? 0.f : m_run;
+          const float2 scale2 = make_float2(sl2, sl2);
+          const float2 shift2 = make_float2(-m_use, -m_use);
+          float2 ps[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
+                          make_float2(0.f, 0.f)};
+#pragma unroll
+          for (int hlf = 0; hlf < 2; ++hlf) {
+            uint32_t pk[32];
+#pragma unroll
+            for (int q = 0; q < 32; ++q) {
+              const int i = hlf * 32 + q;
+              const float2 y = ffma2(make_float2(__uint_as_float(sr[2 * i]),
+                                                 __uint_as_float(sr[2 * i + 1])),
+                                     scale2, shift2);
+              const float2 e = make_float2(ex2_approx(y.x), ex2_approx(y.y));
+              ps[q & 3] = fadd2(ps[q & 3], e);  // the sum takes the weights unrounded
+              pk[q] = pack2<kBF16>(e.x, e.y);
+            }
+            tmem_st32(s_col + hlf * 32, pk);
+          }
+          const float2 sum = fadd2(fadd2(ps[0], ps[1]), fadd2(ps[2], ps[3]));
+          l_run += sum.x + sum.y;
+          tmem_st_wait();
+        }
+        begun = true;
+        tc_fence_before();
+        __syncwarp();
+        if (lane_id() == 0) mbar_arrive(&p_full[x]);
+      }
+      if (!ok) break;
+      // ------------------------------------------------------------ results
+      ok = __all_sync(0xffffffffu, mbar_wait(o_final, w & 1, st, kSiteOReady, tmo));
+      if (!ok) break;
+      tc_fence_after();
+      s_ml[x * kM + row] = make_float2(m_run, l_run);
+      __syncwarp();
+      if (lane_id() == 0) mbar_arrive(joined);
+      ok = __all_sync(0xffffffffu, mbar_wait(joined, w & 1, st, kSiteOReady, tmo));
+      if (!ok) break;
+      const bool dirty = s_dirty[w & 1] == w + 1;
+      float f0 = 1.f, f1 = 0.f;  // factors of the two chains' outputs
+      if constexpr (!kTwoRows) {
+        const float2 a = s_ml[row], b = s_ml[kM + row];
+        const float top = fmaxf(a.x, b.x);
+        if (top != -INFINITY) {
+          f0 = ex2_approx(a.x - top);
+          f1 = ex2_approx(b.x - top);
+        }
+        m_run = top;
+        l_run = f0 * a.y + f1 * b.y;
+      }
+      const bool mine = r < c.rows;
+      const int out_row = c.row0 + r, t = out_row / p.group;
+      const int h = c.head_kv * p.group + out_row - t * p.group;
+      const bool split = c.record >= 0;
+      const float inv = split ? 1.f : (l_run == 0.f ? 0.f : 1.f / l_run);
+      const int64_t rr = static_cast<int64_t>(c.record) * kRows + r;
+      float* rec = split ? p.rec_acc + rr * D : nullptr;
+      uint16_t* dst = static_cast<uint16_t*>(p.out) +
+                      static_cast<int64_t>(c.first + t) * p.out_t + h * p.out_h;
+      if (active) {
+        // with two key chains each warpgroup writes half the columns
+        constexpr int kSpan = kTwoRows ? D : D / 2;
+        const int k_first = kTwoRows ? 0 : x * kSpan;
+#pragma unroll 2
+        for (int kk = 0; kk < kSpan; kk += 16) {
+          const int k = k_first + kk;
+          uint32_t o[16];
+          float v[16];
+          if constexpr (kTwoRows) {
+            tmem_ld16(o_col + k, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(o[i]);
+          } else {
+            uint32_t o1[16];
+            tmem_ld16(tmem + lane_base + 256 + k, o);
+            if (n > 1) tmem_ld16(tmem + lane_base + 384 + k, o1);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              v[i] = n > 1 ? __uint_as_float(o[i]) * f0 + __uint_as_float(o1[i]) * f1
+                           : __uint_as_float(o[i]);
+          }
+          if (dirty && mine) {
+            // what was taken out of V, for the rows that see it
+            const int lo = max(c.ctx, c.tile_begin * kN), hi = min(c.keys, c.tile_end * kN);
+            const int* table = p.table + static_cast<int64_t>(c.request) * p.table_stride;
+            for (int key = lo; key < hi; ++key) {
+              const int rel = key - c.ctx;
+              if (!(seen_bits(p, c, t, rel & ~31) >> (rel & 31) & 1u)) continue;
+              const int page = table[key / p.page_size];
+              if (page < 0 || page >= p.num_pages) continue;
+              const uint16_t* src =
+                  static_cast<const uint16_t*>(p.v) + page * p.v_page +
+                  (static_cast<int64_t>(c.head_kv) * p.page_size + key % p.page_size) * D + k;
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                if (not_finite<kBF16>(src[i])) v[i] += widen<kBF16>(src[i]);
+            }
+          }
+          if (!mine) {
+            // (the TMEM loads above are warp-collective)
+          } else if (split) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+              *reinterpret_cast<float4*>(rec + k + i) =
+                  make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; i += 8)
+              *reinterpret_cast<uint4*>(dst + k + i) =
+                  make_uint4(pack2<kBF16>(v[i] * inv, v[i + 1] * inv),
+                             pack2<kBF16>(v[i + 2] * inv, v[i + 3] * inv),
+                             pack2<kBF16>(v[i + 4] * inv, v[i + 5] * inv),
+                             pack2<kBF16>(v[i + 6] * inv, v[i + 7] * inv));
+          }
+        }
+        if (mine && (kTwoRows || x == 0)) {
+          if (split) {
+            p.rec_m[rr] = m_run;
+            p.rec_l[rr] = l_run;
+          } else if (p.lse != nullptr) {
+            p.lse[static_cast<int64_t>(c.first + t) * p.heads + h] =
+                l_run == 0.f ? -INFINITY : (m_run + log2f(l_run)) * kLn2;
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane_id() == 0) {
+        mbar_arrive(o_free);
+        mbar_arrive(&item_empty[w % kItems]);
+      }
+      g0 += n;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kCols);
+  }
+}
+
+template <int D, bool kBF16, bool kTwoRows>
+int launch(const TreeParams& p, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t stream) {
+  using C = Cfg<D, kTwoRows>;
+  static bool done[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !done[dev]) {
+    const cudaError_t err =
+        cudaFuncSetAttribute(tree_attn_kernel<D, kBF16, kTwoRows>,
+                             cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (err != cudaSuccess) return static_cast<int>(err);
+    if (dev >= 0 && dev < 64) done[dev] = true;
+  }
+  tree_attn_kernel<D, kBF16, kTwoRows><<<p.grid, kThreads, C::kSmem, stream>>>(p, k, v);
+  return static_cast<int>(cudaGetLastError());
+}
+
+CUtensorMap pool_map(const TreeParams& p, const void* base, int64_t page_stride) {
+  const uint64_t d = p.dim, page = p.page_size;
+  uint64_t dims[4] = {d, page, static_cast<uint64_t>(p.heads_kv),
+                      static_cast<uint64_t>(p.num_pages)};
+  uint64_t strides[3] = {d * 2, page * d * 2, static_cast<uint64_t>(page_stride) * 2};
+  uint32_t box[4] = {64, static_cast<uint32_t>(p.page_size < kN ? p.page_size : kN), 1, 1};
+  // 16-bit elements are copied, not read, so one type serves bf16 and fp16
+  return make_tmap(base, TmapDtype::kBF16, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+}  // namespace
+
+int tree_sm100_launch(Elem elem, const TreeParams& p, int rows_per_unit, cudaStream_t stream) {
+  const CUtensorMap k = pool_map(p, p.k, p.k_page), v = pool_map(p, p.v, p.v_page);
+  const bool two = rows_per_unit == 256;
+  if (elem == Elem::kBF16) {
+    if (p.dim == 64)
+      return two ? launch<64, true, true>(p, k, v, stream) : launch<64, true, false>(p, k, v, stream);
+    return two ? launch<128, true, true>(p, k, v, stream) : launch<128, true, false>(p, k, v, stream);
+  }
+  if (p.dim == 64)
+    return two ? launch<64, false, true>(p, k, v, stream) : launch<64, false, false>(p, k, v, stream);
+  return two ? launch<128, false, true>(p, k, v, stream) : launch<128, false, false>(p, k, v, stream);
+}
+
+}  // namespace rab

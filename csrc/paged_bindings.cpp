@@ -430,6 +430,8 @@ std::tuple<torch::Tensor, OptTensor> tree_attention(torch::Tensor q, torch::Tens
   RAB_CHECK(page >= 16 && page <= 256 && (page & (page - 1)) == 0,
             "page size %lld: attention takes 16, 32, 64, 128 or 256", ll(page));
   const Requests r = check_requests(table, ctx, cu, total);
+  RAB_CHECK(table.size(1) <= (1 << 30) / page, "block_table has room for over 2^30 tokens");
+  RAB_CHECK(total <= (1 << 30), "over 2^30 tokens");
   RAB_CHECK(!max_q || *max_q >= 1, "max_q must be positive");
   if (mask) {
     RAB_CHECK(mask->dim() == 2 && mask->size(0) == total,
