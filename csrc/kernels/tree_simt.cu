@@ -49,6 +49,10 @@ __device__ __forceinline__ float4 ld4(const float* p) {
 template <typename T>
 __device__ __forceinline__ T cast_out(float x);
 template <>
+__device__ __forceinline__ float cast_out<float>(float x) {
+  return x;
+}
+template <>
 __device__ __forceinline__ __nv_bfloat16 cast_out<__nv_bfloat16>(float x) {
   return __float2bfloat16_rn(x);
 }
@@ -80,23 +84,22 @@ __global__ void __launch_bounds__(kSimtThreads)
   float* sQ = reinterpret_cast<float*>(smem + C::kStages);
   float* sP = reinterpret_cast<float*>(smem + C::kStages + C::kQBytes);
   float* sJoin = reinterpret_cast<float*>(smem);
-  __shared__ long long s_sums[kSimtThreads / 32];
-  __shared__ int s_request;
-  __shared__ long long s_at;
+  __shared__ int s_sums[kSimtThreads / 32];
+  __shared__ Start s_start;
   __shared__ Piece s_piece;
   __shared__ int s_have, s_merges, s_c0;
   __shared__ float s_m[4][kSimtRows], s_l[4][kSimtRows], s_alpha[4][kSimtRows];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-  const Range range = find_range<kSimtTile, kSimtThreads>(p, kSimtRows, s_sums, &s_request, &s_at);
-  Walk<kSimtTile> walk;
+  const Range range = find_range<kSimtTile, kSimtRows, kSimtThreads>(p, s_sums, &s_start);
+  Walk<kSimtTile, kSimtRows> walk;
   if (tid == 0) {
-    walk.start(p, range, kSimtRows);
+    walk.start(p, range, s_start);
     p.meta[blockIdx.x * kMetaInts] = 0;
   }
   while (true) {
     if (tid == 0) {
-      s_have = walk.next(p, range, kSimtRows, &s_piece);
+      s_have = walk.next(p, range, &s_piece);
       s_merges = s_have && walk.merges;
       s_c0 = walk.merge_c0;
     }
@@ -280,14 +283,17 @@ __global__ void __launch_bounds__(kSimtThreads)
       }
       if (c.record >= 0) {
         const int64_t rr = static_cast<int64_t>(c.record) * kSimtRows + r;
-        p.rec_acc[rr * D + x] = o;
+        // a record is [dim / 4][rows][4], the rows of the unit side by side
+        p.rec_acc[static_cast<int64_t>(c.record) * (kSimtRows * D) + ((x >> 2) * c.rows + r) * 4 +
+                  (x & 3)] = o;
         if (x == 0) {
           p.rec_m[rr] = top;
           p.rec_l[rr] = sum;
         }
       } else {
         const int row = c.row0 + r, t = row / p.group, h = c.head_kv * p.group + row % p.group;
-        static_cast<float*>(p.out)[(c.first + t) * p.out_t + h * p.out_h + x] =
+        static_cast<float*>(p.out)[static_cast<int64_t>(c.first + t) * p.out_t +
+                                   static_cast<int64_t>(h) * p.out_h + x] =
             sum == 0.f ? 0.f : o / sum;
         if (x == 0 && p.lse != nullptr)
           p.lse[static_cast<int64_t>(c.first + t) * p.heads + h] =
@@ -300,53 +306,98 @@ __global__ void __launch_bounds__(kSimtThreads)
 }
 
 // ---------------------------------------------------------------------------
-// Merge: block (c, y) joins the records of the unit that CTA c ended.
+// Merge: the blocks (c, y) join the records of the unit that CTA c ended.  A
+// thread owns four columns of a row; a record is [dim / 4][rows][4], so the
+// threads of a warp read side by side whatever the number of rows.  Bound by
+// latency: eight records' maxima, sums and outputs are in flight at once, and
+// with more than eight (long contexts, few rows) the block's four warps share the
+// records of the same 32 elements and join theirs through shared memory.  The
+// launch overlaps the attention kernel's end (griddepcontrol.wait holds it until
+// every record is written).
 // ---------------------------------------------------------------------------
 constexpr int kMergeThreads = 128;
+
+struct Joined {
+  float top, sum;
+  float4 o;
+};
+
+__device__ __forceinline__ void join_into(Joined& a, float m, float l, const float4& o) {
+  const float top = fmaxf(a.top, m);
+  const float use = top == -INFINITY ? 0.f : top;
+  const float f = sm100::ex2_approx(a.top - use), g = sm100::ex2_approx(m - use);
+  a.top = top;
+  a.sum = f * a.sum + g * l;
+  a.o.x = f * a.o.x + g * o.x;
+  a.o.y = f * a.o.y + g * o.y;
+  a.o.z = f * a.o.z + g * o.z;
+  a.o.w = f * a.o.w + g * o.w;
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kMergeThreads)
     tree_merge_kernel(const __grid_constant__ TreeParams p, int rows_per_unit) {
-  constexpr int kLanes = D / 4;  // threads of a row
-  constexpr int kRows = kMergeThreads / kLanes;
-  const int* meta = p.meta + blockIdx.x * kMetaInts;
-  if (meta[0] == 0) return;
-  const int c0 = meta[1], head_kv = meta[2], row0 = meta[3], rows = meta[4], first = meta[5];
-  const int c1 = blockIdx.x;
-  const int x = (threadIdx.x % kLanes) * 4;
-  for (int r = blockIdx.y * kRows + threadIdx.x / kLanes; r < rows; r += gridDim.y * kRows) {
-    // the first record is the last piece of CTA c0, the others the first of each
-    auto record = [&](int c) {
-      return (static_cast<int64_t>(2 * c + (c == c0 ? 1 : 0))) * rows_per_unit + r;
-    };
-    float top = -INFINITY;
-    for (int c = c0; c <= c1; ++c) top = fmaxf(top, p.rec_m[record(c)]);
-    float sum = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int c = c0; c <= c1; ++c) {
-      const int64_t k = record(c);
-      const float f = top == -INFINITY ? 1.f : sm100::ex2_approx(p.rec_m[k] - top);
-      const float4 a = *reinterpret_cast<const float4*>(p.rec_acc + k * D + x);
-      sum += f * p.rec_l[k];
-      o.x += f * a.x;
-      o.y += f * a.y;
-      o.z += f * a.z;
-      o.w += f * a.w;
+  __shared__ Joined s_join[3][32];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 m0 = *reinterpret_cast<const int4*>(p.meta + blockIdx.x * kMetaInts);
+  const int2 m1 = *reinterpret_cast<const int2*>(p.meta + blockIdx.x * kMetaInts + 4);
+  if (m0.x == 0) return;
+  const int c0 = m0.y, head_kv = m0.z, row0 = m0.w, rows = m1.x, first = m1.y;
+  const int n = blockIdx.x - c0 + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool share = n > 8;
+  const int i_first = share ? warp : 0, i_step = share ? 4 : 1;
+  const int elems = rows * (D / 4), per_block = share ? 32 : kMergeThreads;
+  for (int e0 = blockIdx.y * per_block; e0 < elems; e0 += gridDim.y * per_block) {
+    const int e = min(e0 + (share ? lane : static_cast<int>(threadIdx.x)), elems - 1);
+    const bool mine = e0 + (share ? lane : static_cast<int>(threadIdx.x)) < elems;
+    const int x4 = e / rows, r = e - x4 * rows;
+    Joined a{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+    for (int i0 = i_first; i0 < n; i0 += 8 * i_step) {
+      float m[8], l[8];
+      float4 o[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        // past the last: the same record again, left out below
+        const int i = min(i0 + u * i_step, n - 1);
+        // the first record is the last piece of CTA c0, the others the first of each
+        const int k = 2 * (c0 + i) + (i == 0 ? 1 : 0);
+        m[u] = p.rec_m[k * rows_per_unit + r];
+        l[u] = p.rec_l[k * rows_per_unit + r];
+        o[u] = *reinterpret_cast<const float4*>(
+            p.rec_acc + static_cast<int64_t>(k) * rows_per_unit * D + e * 4);
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (i0 + u * i_step < n) join_into(a, m[u], l[u], o[u]);
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int row = row0 + r, t = row / p.group, h = head_kv * p.group + row % p.group;
-    T* dst = static_cast<T*>(p.out) + (first + t) * p.out_t + h * p.out_h + x;
-    if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<float4*>(dst) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-    } else {
-      T v[4] = {cast_out<T>(o.x * inv), cast_out<T>(o.y * inv), cast_out<T>(o.z * inv),
-                cast_out<T>(o.w * inv)};
-      *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(v);
+    if (share) {
+      if (warp > 0) s_join[warp - 1][lane] = a;
+      __syncthreads();
+      if (warp == 0) {
+#pragma unroll
+        for (int w = 0; w < 3; ++w) {
+          const Joined b = s_join[w][lane];
+          join_into(a, b.top, b.sum, b.o);
+        }
+      }
+      __syncthreads();
+      if (warp > 0) continue;
     }
-    if (x == 0 && p.lse != nullptr)
+    if (!mine) continue;
+    const float inv = a.sum == 0.f ? 0.f : 1.f / a.sum;
+    const int row = row0 + r, t = row / p.group, h = head_kv * p.group + row - t * p.group;
+    T* dst = static_cast<T*>(p.out) + static_cast<int64_t>(first + t) * p.out_t +
+             static_cast<int64_t>(h) * p.out_h + x4 * 4;
+    alignas(16) T v[4] = {cast_out<T>(a.o.x * inv), cast_out<T>(a.o.y * inv),
+                          cast_out<T>(a.o.z * inv), cast_out<T>(a.o.w * inv)};
+    if constexpr (sizeof(T) == 4)
+      *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(v);
+    else
+      *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(v);
+    if (x4 == 0 && p.lse != nullptr)
       p.lse[static_cast<int64_t>(first + t) * p.heads + h] =
-          sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2f;
+          a.sum == 0.f ? -INFINITY : (a.top + log2f(a.sum)) * kLn2f;
   }
 }
 
@@ -368,11 +419,18 @@ int run_simt(const TreeParams& p, cudaStream_t stream) {
 
 template <typename T, int D>
 int run_merge(const TreeParams& p, int rows_per_unit, cudaStream_t stream) {
-  constexpr int kRows = kMergeThreads / (D / 4);
-  const int gy = (rows_per_unit + kRows - 1) / kRows;
-  tree_merge_kernel<T, D>
-      <<<dim3(p.grid, gy < 8 ? gy : 8), kMergeThreads, 0, stream>>>(p, rows_per_unit);
-  return static_cast<int>(cudaGetLastError());
+  cudaLaunchAttribute overlap;
+  overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  overlap.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  // a block per 128 elements up to 32 of them; blocks without a unit leave at once
+  const int blocks = rows_per_unit * (D / 4) / kMergeThreads;
+  cfg.gridDim = dim3(p.grid, blocks < 1 ? 1 : (blocks < 32 ? blocks : 32));
+  cfg.blockDim = dim3(kMergeThreads);
+  cfg.stream = stream;
+  cfg.attrs = &overlap;
+  cfg.numAttrs = 1;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, tree_merge_kernel<T, D>, p, rows_per_unit));
 }
 
 // ---------------------------------------------------------------------------

@@ -71,11 +71,12 @@ struct Cfg {
   static constexpr int kBarOff = kQBytes + kStages * kTile;
   static constexpr int kMlOff = kBarOff + kBars * 8;       // float2 [2][128]
   static constexpr int kItemOff = kMlOff + 2 * kM * 8;     // Piece [kItems]
-  static constexpr int kSumOff = kItemOff + kItems * 48;   // long long [12 + 1]
-  static constexpr int kMiscOff = kSumOff + 13 * 8;        // int [8]
-  static constexpr int kSmem = kMiscOff + 32;
+  static constexpr int kSumOff = kItemOff + kItems * 48;   // int [12]
+  static constexpr int kStartOff = kSumOff + 12 * 4;       // Start
+  static constexpr int kMiscOff = kStartOff + 32;          // int [4]
+  static constexpr int kSmem = kMiscOff + 16;
   static_assert(kMlOff % 8 == 0 && kSumOff % 8 == 0 && kSmem <= 232448, "shared memory");
-  static_assert(sizeof(Piece) <= 48, "piece");
+  static_assert(sizeof(Piece) <= 48 && sizeof(Start) <= 32, "piece");
 };
 
 template <bool kBF16>
@@ -102,15 +103,15 @@ __device__ __forceinline__ float widen(uint32_t h) {
 
 // The 32 columns of new tokens rel0 .. rel0 + 31 that token t of the request
 // sees, as bits; places before the new tokens (rel < 0) are cached and seen.
-__device__ __forceinline__ uint32_t seen_bits(const TreeParams& p, const Piece& c, int t,
+__device__ __forceinline__ uint32_t seen_bits(const TreeParams& p, const Piece* c, int t,
                                               int rel0) {
-  int n = min(c.tokens, c.keys - c.ctx) - rel0;  // columns that hold a key
+  int n = min(c->tokens, c->keys - c->ctx) - rel0;  // columns that hold a key
   uint32_t bits;
   if (p.mask == nullptr) {
     n = min(n, t - rel0 + 1);
     bits = 0xffffffffu;
   } else {
-    const uint32_t* row = p.mask + static_cast<int64_t>(c.first + t) * p.mask_stride;
+    const uint32_t* row = p.mask + static_cast<int64_t>(c->first + t) * p.mask_stride;
     const int w = rel0 >> 5, sh = rel0 & 31;
     auto word = [&](int i) { return i < 0 ? 0xffffffffu : (i < p.mask_w ? row[i] : 0u); };
     const uint32_t lo = word(w);
@@ -119,6 +120,65 @@ __device__ __forceinline__ uint32_t seen_bits(const TreeParams& p, const Piece& 
   }
   if (n <= 0) return 0u;
   return n < 32 ? bits & ((1u << n) - 1u) : bits;
+}
+
+// V rows [vr0, vr0 + n_rows) of a tile whose first key is k0, by 128 threads:
+// rows at or past `keys` become zeros, and among the new tokens (from ctx on)
+// what is not finite does; true when this thread took something out.
+template <int D, bool kBF16>
+__device__ __noinline__ bool clean_v(uint8_t* tile, int k0, int ctx, int keys, int vr0, int n_rows,
+                                     int tid) {
+  constexpr int kPerRow = D / 8;
+  bool dirty = false;
+  for (int i = tid; i < n_rows * kPerRow; i += 128) {
+    const int vr = vr0 + i / kPerRow, ch = i % kPerRow;
+    if (k0 + vr < ctx) continue;
+    uint4* at = reinterpret_cast<uint4*>(tile + (ch / 8) * (kN * 128) + vr * 128 + (ch % 8) * 16);
+    if (k0 + vr >= keys) {
+      *at = make_uint4(0u, 0u, 0u, 0u);
+      continue;
+    }
+    const uint4 v = *at;
+    uint32_t e[4] = {v.x, v.y, v.z, v.w};
+    bool hit = false;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (not_finite<kBF16>(e[u])) e[u] &= 0xffff0000u, hit = true;
+      if (not_finite<kBF16>(e[u] >> 16)) e[u] &= 0x0000ffffu, hit = true;
+    }
+    if (hit) {
+      *at = make_uint4(e[0], e[1], e[2], e[3]);
+      dirty = true;
+    }
+  }
+  return dirty;
+}
+
+// Adds what clean_v took out to columns [k0, k1) of a result this thread has
+// just written (a record's row, or the output row), for the keys its token sees.
+template <bool kBF16>
+__device__ __noinline__ void add_taken_out(const TreeParams& p, const Piece* c, int t, int k0,
+                                           int k1, int dim, float* rec, uint16_t* dst) {
+  const int lo = max(c->ctx, c->tile_begin * kN), hi = min(c->keys, c->tile_end * kN);
+  const int* table = p.table + static_cast<int64_t>(c->request) * p.table_stride;
+  for (int key = lo; key < hi; ++key) {
+    const int rel = key - c->ctx;
+    if (!((seen_bits(p, c, t, rel & ~31) >> (rel & 31)) & 1u)) continue;
+    const int page = table[key / p.page_size];
+    if (page < 0 || page >= p.num_pages) continue;
+    const uint16_t* src =
+        static_cast<const uint16_t*>(p.v) + page * p.v_page +
+        (static_cast<int64_t>(c->head_kv) * p.page_size + key % p.page_size) * dim;
+    for (int k = k0; k < k1; ++k) {
+      if (!not_finite<kBF16>(src[k])) continue;
+      const float v = widen<kBF16>(src[k]);
+      if (rec != nullptr) {
+        rec[(k & ~3) * c->rows + (k & 3)] += v;
+      } else {
+        dst[k] = static_cast<uint16_t>(pack2<kBF16>(widen<kBF16>(dst[k]) + v, 0.f));
+      }
+    }
+  }
 }
 
 template <int D, bool kBF16, bool kTwoRows>
@@ -147,10 +207,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* item_full = q_full + 10;           // [kItems]
   uint64_t* item_empty = item_full + kItems;   // [kItems]
   float2* s_ml = reinterpret_cast<float2*>(smem + C::kMlOff);
-  long long* s_sums = reinterpret_cast<long long*>(smem + C::kSumOff);
+  int* s_sums = reinterpret_cast<int*>(smem + C::kSumOff);
   int* s_misc = reinterpret_cast<int*>(smem + C::kMiscOff);
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_misc);
-  int* s_request = s_misc + 1;
+  Start* s_start = reinterpret_cast<Start*>(smem + C::kStartOff);
   volatile int* s_dirty = s_misc + 2;  // [2], by the piece's parity
   auto item_slot = [&](int w) {
     return reinterpret_cast<Piece*>(smem + C::kItemOff + (w % kItems) * 48);
@@ -169,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     return;
   }
 
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == 64) {
     for (int i = 0; i < NS; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
@@ -195,8 +255,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_alloc(s_tmem, kCols);
     tmem_relinquish();
   }
-  const Range range = find_range<kN, kThreads>(p, kRows, s_sums, s_request, s_sums + 12);
-  __syncthreads();
+  const Range range = find_range<kN, kRows, kThreads>(p, s_sums, s_start);
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
 
@@ -205,11 +264,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 0) {
       // ------------------------------------------------------ pieces and loads
       const int lane = lane_id();
-      Walk<kN> walk;
+      Walk<kN, kRows> walk;
       if (lane == 0) {
         tma_prefetch_desc(&tmK);
         tma_prefetch_desc(&tmV);
-        walk.start(p, range, kRows);
+        walk.start(p, range, *s_start);
         p.meta[blockIdx.x * kMetaInts] = 0;
       }
       const int rows_box = min(p.page_size, kN);
@@ -224,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         Piece* slot = item_slot(w);
         if (lane == 0) {
           Piece c;
-          if (walk.next(p, range, kRows, &c)) {
+          if (walk.next(p, range, &c)) {
             if (walk.merges) write_meta(p, c, true, walk.merge_c0);
           } else {
             c.request = -1;
@@ -427,50 +486,29 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = __all_sync(0xffffffffu, mbar_wait(&item_full[w % kItems], (w / kItems) & 1, st,
                                              kSiteItemQueue, tmo));
       if (!ok) break;
-      const Piece c = *item_slot(w);
-      if (c.request < 0) break;
-      const int n = c.tile_end - c.tile_begin;
+      // the piece stays in its slot: its fields are read again where they are
+      // used rather than kept beside a row of 128 scores
+      const Piece* c = item_slot(w);
+      if (c->request < 0) break;
+      const int n = c->tile_end - c->tile_begin;
+      const int old_keys = c->ctx - c->tile_begin * kN;  // of the piece, before the new tokens
       const int r = kTwoRows ? x * kM + row : row;  // row of the unit
       // a warp without rows only keeps the order of things
-      const bool active = r - static_cast<int>(lane_id()) < c.rows;
-      const int token = min(c.row0 + r, c.row0 + c.rows - 1) / p.group;
+      const bool active = r - static_cast<int>(lane_id()) < c->rows;
       const uint32_t o_col = tmem + lane_base + 256 + x * 128;
       float m_run = -INFINITY, l_run = 0.f;
-      bool begun = false;
       for (int j = kTwoRows ? 0 : x; j < n; j += kTwoRows ? 1 : 2) {
-        const int k0 = (c.tile_begin + j) * kN;
-        const bool tail = k0 + kN > c.ctx;
+        const bool tail = (j + 1) * kN > old_keys;
         if (tail) {
           // clean V: 16 bytes a step; with two row tiles each chain takes half the rows
           const int idx = 2 * (g0 + j) + 1;
           ok = __all_sync(0xffffffffu,
                           mbar_wait(&full[idx % NS], (idx / NS) & 1, st, kSiteVFull, tmo));
           if (!ok) break;
-          uint8_t* vt = sKV + (idx % NS) * C::kTile;
-          constexpr int kPerRow = D / 8;
           constexpr int kVRows = kTwoRows ? kN / 2 : kN;
-          bool dirty = false;
-          for (int i = row; i < kVRows * kPerRow; i += 128) {
-            const int vr = i / kPerRow + (kTwoRows ? x * kVRows : 0), ch = i % kPerRow;
-            const int rel = k0 + vr - c.ctx;
-            if (rel < 0) continue;
-            uint4* at = reinterpret_cast<uint4*>(vt + (ch / 8) * (kN * 128) + vr * 128 +
-                                                 (ch % 8) * 16);
-            if (k0 + vr >= c.keys) {
-              *at = make_uint4(0u, 0u, 0u, 0u);
-            } else {
-              uint4 v = *at;
-              bool hit = false;
-              uint32_t* e = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-              for (int u = 0; u < 4; ++u) {
-                if (not_finite<kBF16>(e[u])) e[u] &= 0xffff0000u, hit = true;
-                if (not_finite<kBF16>(e[u] >> 16)) e[u] &= 0x0000ffffu, hit = true;
-              }
-              if (hit) *at = v, dirty = true;
-            }
-          }
-          if (dirty) s_dirty[w & 1] = w + 1;
+          if (clean_v<D, kBF16>(sKV + (idx % NS) * C::kTile, (c->tile_begin + j) * kN, c->ctx,
+                                c->keys, kTwoRows ? x * kVRows : 0, kVRows, row))
+            s_dirty[w & 1] = w + 1;
           fence_proxy_async_smem();
         }
         ok = __all_sync(0xffffffffu, mbar_wait(&s_full[x], sx & 1, st, kSiteSFull, tmo));
@@ -488,9 +526,10 @@ __global__ void __launch_bounds__(kThreads, 1)
               sr[k] = __float_as_uint(__uint_as_float(sr[k]) * p.scale_log2);
           }
           if (tail) {
+            const int token = min(c->row0 + r, c->row0 + c->rows - 1) / p.group;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-              const uint32_t bits = seen_bits(p, c, token, k0 + 32 * q - c.ctx);
+              const uint32_t bits = seen_bits(p, c, token, j * kN + 32 * q - old_keys);
 #pragma unroll
               for (int k = 0; k < 32; ++k)
                 if (!((bits >> k) & 1u)) sr[32 * q + k] = 0xff800000u;  // -inf
@@ -514,7 +553,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             l_run *= alpha;
           }
           // the scores' commit covers this chain's products before them: O is at rest
-          if (begun && __any_sync(0xffffffffu, need)) {
+          if (j > (kTwoRows ? 0 : 1) && __any_sync(0xffffffffu, need)) {
 #pragma unroll
             for (int k = 0; k < D; k += 32) {
               uint32_t o[32];
@@ -550,109 +589,101 @@ __global__ void __launch_bounds__(kThreads, 1)
           l_run += sum.x + sum.y;
           tmem_st_wait();
         }
-        begun = true;
         tc_fence_before();
         __syncwarp();
         if (lane_id() == 0) mbar_arrive(&p_full[x]);
       }
       if (!ok) break;
       // ------------------------------------------------------------ results
+      s_ml[x * kM + row] = make_float2(m_run, l_run);
       ok = __all_sync(0xffffffffu, mbar_wait(o_final, w & 1, st, kSiteOReady, tmo));
       if (!ok) break;
       tc_fence_after();
-      s_ml[x * kM + row] = make_float2(m_run, l_run);
       __syncwarp();
       if (lane_id() == 0) mbar_arrive(joined);
       ok = __all_sync(0xffffffffu, mbar_wait(joined, w & 1, st, kSiteOReady, tmo));
       if (!ok) break;
-      const bool dirty = s_dirty[w & 1] == w + 1;
-      float f0 = 1.f, f1 = 0.f;  // factors of the two chains' outputs
-      if constexpr (!kTwoRows) {
-        const float2 a = s_ml[row], b = s_ml[kM + row];
-        const float top = fmaxf(a.x, b.x);
-        if (top != -INFINITY) {
-          f0 = ex2_approx(a.x - top);
-          f1 = ex2_approx(b.x - top);
-        }
-        m_run = top;
-        l_run = f0 * a.y + f1 * b.y;
-      }
-      const bool mine = r < c.rows;
-      const int out_row = c.row0 + r, t = out_row / p.group;
-      const int h = c.head_kv * p.group + out_row - t * p.group;
-      const bool split = c.record >= 0;
-      const float inv = split ? 1.f : (l_run == 0.f ? 0.f : 1.f / l_run);
-      const int64_t rr = static_cast<int64_t>(c.record) * kRows + r;
-      float* rec = split ? p.rec_acc + rr * D : nullptr;
-      uint16_t* dst = static_cast<uint16_t*>(p.out) +
-                      static_cast<int64_t>(c.first + t) * p.out_t + h * p.out_h;
       if (active) {
+        float f0 = 1.f, f1 = 0.f;  // factors of the two chains' outputs
+        if constexpr (!kTwoRows) {
+          const float2 a = s_ml[row], b = s_ml[kM + row];
+          const float top = fmaxf(a.x, b.x);
+          if (top != -INFINITY) {
+            f0 = ex2_approx(a.x - top);
+            f1 = ex2_approx(b.x - top);
+          }
+          m_run = top;
+          l_run = f0 * a.y + f1 * b.y;
+        }
+        const bool mine = r < c->rows;
+        const int record = c->record, rows = c->rows;
+        const int out_row = c->row0 + r;
+        const int t = static_cast<int>(static_cast<uint32_t>(out_row) /
+                                       static_cast<uint32_t>(p.group));
+        const int h = c->head_kv * p.group + out_row - t * p.group;
+        if (record < 0) {
+          const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+          f0 *= inv;
+          f1 *= inv;
+        }
+        // a record is [dim / 4][rows][4]: the rows of a warp lie side by side
+        float* rec = p.rec_acc + static_cast<int64_t>(record) * (kRows * D) + r * 4;
+        uint16_t* dst = static_cast<uint16_t*>(p.out) +
+                        static_cast<int64_t>(c->first + t) * p.out_t +
+                        static_cast<int64_t>(h) * p.out_h;
         // with two key chains each warpgroup writes half the columns
         constexpr int kSpan = kTwoRows ? D : D / 2;
         const int k_first = kTwoRows ? 0 : x * kSpan;
-#pragma unroll 2
-        for (int kk = 0; kk < kSpan; kk += 16) {
-          const int k = k_first + kk;
-          uint32_t o[16];
-          float v[16];
+#pragma unroll 1
+        for (int k = k_first; k < k_first + kSpan; k += 32) {
+          uint32_t o[32];
+          float* v = reinterpret_cast<float*>(o);
           if constexpr (kTwoRows) {
-            tmem_ld16(o_col + k, o);
+            tmem_ld32(o_col + k, o);
             tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(o[i]);
+            for (int i = 0; i < 32; ++i) v[i] *= f0;
           } else {
-            uint32_t o1[16];
-            tmem_ld16(tmem + lane_base + 256 + k, o);
-            if (n > 1) tmem_ld16(tmem + lane_base + 384 + k, o1);
-            tmem_ld_wait();
+            uint32_t o1[32];
+            tmem_ld32(tmem + lane_base + 256 + k, o);
+            if (n > 1) {
+              tmem_ld32(tmem + lane_base + 384 + k, o1);
+              tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              v[i] = n > 1 ? __uint_as_float(o[i]) * f0 + __uint_as_float(o1[i]) * f1
-                           : __uint_as_float(o[i]);
-          }
-          if (dirty && mine) {
-            // what was taken out of V, for the rows that see it
-            const int lo = max(c.ctx, c.tile_begin * kN), hi = min(c.keys, c.tile_end * kN);
-            const int* table = p.table + static_cast<int64_t>(c.request) * p.table_stride;
-            for (int key = lo; key < hi; ++key) {
-              const int rel = key - c.ctx;
-              if (!(seen_bits(p, c, t, rel & ~31) >> (rel & 31) & 1u)) continue;
-              const int page = table[key / p.page_size];
-              if (page < 0 || page >= p.num_pages) continue;
-              const uint16_t* src =
-                  static_cast<const uint16_t*>(p.v) + page * p.v_page +
-                  (static_cast<int64_t>(c.head_kv) * p.page_size + key % p.page_size) * D + k;
+              for (int i = 0; i < 32; ++i) v[i] = v[i] * f0 + __uint_as_float(o1[i]) * f1;
+            } else {
+              tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 16; ++i)
-                if (not_finite<kBF16>(src[i])) v[i] += widen<kBF16>(src[i]);
+              for (int i = 0; i < 32; ++i) v[i] *= f0;
             }
           }
           if (!mine) {
             // (the TMEM loads above are warp-collective)
-          } else if (split) {
+          } else if (record >= 0) {
 #pragma unroll
-            for (int i = 0; i < 16; i += 4)
-              *reinterpret_cast<float4*>(rec + k + i) =
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<float4*>(rec + (k + i) * rows) =
                   make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
           } else {
 #pragma unroll
-            for (int i = 0; i < 16; i += 8)
+            for (int i = 0; i < 32; i += 8)
               *reinterpret_cast<uint4*>(dst + k + i) =
-                  make_uint4(pack2<kBF16>(v[i] * inv, v[i + 1] * inv),
-                             pack2<kBF16>(v[i + 2] * inv, v[i + 3] * inv),
-                             pack2<kBF16>(v[i + 4] * inv, v[i + 5] * inv),
-                             pack2<kBF16>(v[i + 6] * inv, v[i + 7] * inv));
+                  make_uint4(pack2<kBF16>(v[i], v[i + 1]), pack2<kBF16>(v[i + 2], v[i + 3]),
+                             pack2<kBF16>(v[i + 4], v[i + 5]), pack2<kBF16>(v[i + 6], v[i + 7]));
           }
         }
         if (mine && (kTwoRows || x == 0)) {
-          if (split) {
-            p.rec_m[rr] = m_run;
-            p.rec_l[rr] = l_run;
+          if (record >= 0) {
+            p.rec_m[record * kRows + r] = m_run;
+            p.rec_l[record * kRows + r] = l_run;
           } else if (p.lse != nullptr) {
-            p.lse[static_cast<int64_t>(c.first + t) * p.heads + h] =
+            p.lse[static_cast<int64_t>(c->first + t) * p.heads + h] =
                 l_run == 0.f ? -INFINITY : (m_run + log2f(l_run)) * kLn2;
           }
         }
+        if (mine && s_dirty[w & 1] == w + 1)
+          add_taken_out<kBF16>(p, c, t, k_first, k_first + kSpan, D,
+                               record >= 0 ? rec : nullptr, dst);
       }
       tc_fence_before();
       __syncwarp();

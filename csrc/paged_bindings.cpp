@@ -431,7 +431,11 @@ std::tuple<torch::Tensor, OptTensor> tree_attention(torch::Tensor q, torch::Tens
             "page size %lld: attention takes 16, 32, 64, 128 or 256", ll(page));
   const Requests r = check_requests(table, ctx, cu, total);
   RAB_CHECK(table.size(1) <= (1 << 30) / page, "block_table has room for over 2^30 tokens");
-  RAB_CHECK(total <= (1 << 30), "over 2^30 tokens");
+  // the kernels count rows and the places of their line of units in 32 bits
+  const int64_t rows = total * (heads / hk);
+  RAB_CHECK(rows <= (1 << 30), "over 2^30 rows of a kv head");
+  RAB_CHECK((rows / 8 + r.batch) * hk <= (int64_t{1} << 31) / (table.size(1) * page / 64 + 4),
+            "too many units of work for one call: split the batch");
   RAB_CHECK(!max_q || *max_q >= 1, "max_q must be positive");
   if (mask) {
     RAB_CHECK(mask->dim() == 2 && mask->size(0) == total,
