@@ -55,17 +55,23 @@ struct RopeParams {
 int rope_launch(Elem elem, const RopeParams& p, bool vectors, cudaStream_t stream);
 
 // ---- page copies ----
-constexpr int kMaxPagePairs = 1000;  // pairs of one launch (kernel parameters)
+// The pairs of one launch travel in its parameters; few of them take a small
+// block of parameters, which a launch hands over faster.
+constexpr int kFewPairs = 32, kManyPairs = 1000;
+template <int kPairs>
 struct PageCopyParams {
+  static constexpr int kMax = kPairs;
   uint8_t* k;
   uint8_t* v;
   int64_t k_layer, k_page, v_layer, v_page;  // byte strides
   int64_t page_bytes;
-  int layers, n;
-  int src[kMaxPagePairs];
-  int dst[kMaxPagePairs];
+  int layers, n_src;
+  int src[kPairs];        // distinct source pages
+  int first[kPairs + 1];  // source s goes to dst[first[s]] .. dst[first[s + 1] - 1]
+  int dst[kPairs];
 };
-int page_copy_launch(const PageCopyParams& p, cudaStream_t stream);
+int page_copy_launch(const PageCopyParams<kFewPairs>& p, cudaStream_t stream);
+int page_copy_launch(const PageCopyParams<kManyPairs>& p, cudaStream_t stream);
 
 // ---- accepted path ----
 struct PathParams {
@@ -122,6 +128,7 @@ struct TreeParams {
 struct TreePlan {
   int rows_per_unit;
   int grid;
+  int merge_rows;  // rows the merge launch is sized for
   size_t acc_floats, ml_floats, meta_ints;
 };
 

@@ -10,10 +10,13 @@
 // only the rounding of step (2^-53 relative) grows with it.  sin and cos of
 // the top 32 bits follow in fp32 (sincospif).
 //
-// Bound by memory: every element is read and written once.  A thread owns two
-// 16-byte vectors of a row (8 pairs of 2-byte types, 4 of fp32), forms their
-// sines and cosines once and then walks a group of heads with all loads of four
-// heads in flight; the head group shrinks until the grid fills the GPU.
+// Bound by memory: every element is read and written once.  A block takes a few
+// tokens and a group of heads: its threads first form the sines and cosines of
+// the tokens' pairs once, into shared memory, together with each token's place in
+// the cache, and then stream rows past them.  A thread keeps one place in the row
+// (two 16-byte vectors: 8 pairs of a 2-byte type, 4 of fp32), so its sines stay in
+// the same shared-memory words, and has the loads of two rows in flight before
+// the first is used.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -88,108 +91,156 @@ __device__ __forceinline__ void rotate(Pack<T, VEC>& a, Pack<T, VEC>& b, const f
   }
 }
 
-// grid.x: token groups; grid.y: head groups of `hc` heads, operand after operand
+// Where a pair's sine lies among its token's: a thread reads the VEC pairs of its
+// task two at a time, and the tasks of a row side by side, so that a warp's
+// 16-byte reads meet no bank twice.
+template <int VEC>
+__device__ __forceinline__ int cs_slot(int pair, int pairs) {
+  if constexpr (VEC == 1) return pair;
+  const int task = pair / VEC, i = pair % VEC;
+  return (i / 2) * 2 * (pairs / VEC) + 2 * task + (i & 1);
+}
+
+constexpr int kRopeTokens = 8;  // tokens of a block, at most
+constexpr int kRopeRows = 2;    // rows a thread has in flight
+
+// grid.x: groups of `tb` tokens; grid.y: groups of `hc` heads, operand after operand
 template <typename T, int VEC, bool kInter>
 __global__ void __launch_bounds__(kRopeThreads)
-    rope_kernel(const __grid_constant__ RopeParams p, int tasks, int tokens_per_block, int hc) {
+    rope_kernel(const __grid_constant__ RopeParams p, int tasks, int tb, int hc) {
   using P = Pack<T, VEC>;
-  const int local = threadIdx.x / tasks;
-  const int task = threadIdx.x - local * tasks;
-  const int token = blockIdx.x * tokens_per_block + local;
-  if (local >= tokens_per_block || token >= p.tokens) return;
+  extern __shared__ __align__(16) float2 s_cs[];  // [tb][rotary_dim / 2]
+  __shared__ int64_t s_dst[kRopeTokens], s_pos[kRopeTokens];
+  __shared__ int s_ok[kRopeTokens];
   int o = 0, g = blockIdx.y;
   while (o + 1 < p.n_op && g >= (p.op[o].heads + hc - 1) / hc) {
     g -= (p.op[o].heads + hc - 1) / hc;
     ++o;
   }
   const RopeOperand& op = p.op[o];
-  const int h_end = min(op.heads, (g + 1) * hc);
+  const int h0 = g * hc, heads = min(op.heads - h0, hc);
+  const int token0 = blockIdx.x * tb, tokens = min(tb, p.tokens - token0);
 
-  // where the token lies in the cache
-  int64_t at = 0, dst = static_cast<int64_t>(token) * op.out_t;
-  if (p.ctx != nullptr) {
-    int b;
-    int first;
-    if (p.cu == nullptr) {
-      b = token / p.uniform;
-      first = b * p.uniform;
-    } else {
-      int lo = 0, hi = p.batch;  // the last request that starts at or before the token
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (p.cu[mid] <= token) lo = mid;
-        else hi = mid;
+  if (threadIdx.x < tokens) {  // where the token lies in the cache, and its position
+    const int token = token0 + threadIdx.x;
+    int64_t at = 0, dst = static_cast<int64_t>(token) * op.out_t;
+    bool ok = true;
+    if (p.ctx != nullptr) {
+      int b, first;
+      if (p.cu == nullptr) {
+        b = token / p.uniform;
+        first = b * p.uniform;
+      } else {
+        int lo = 0, hi = p.batch;  // the last request that starts at or before the token
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (p.cu[mid] <= token) lo = mid;
+          else hi = mid;
+        }
+        b = lo;
+        first = p.cu[b];
+        ok = token >= first && token < p.cu[b + 1];  // else: behind the last request
       }
-      b = lo;
-      first = p.cu[b];
-      if (token < first || token >= p.cu[b + 1]) return;  // behind the last request
+      if (ok) at = static_cast<int64_t>(p.ctx[b]) + (token - first);
+      if (ok && op.paged) {
+        ok = at >= 0 && at < static_cast<int64_t>(p.table_w) * p.page_size;
+        if (!ok) {
+          if (g == 0) st_record(p.status, kStatusBadArgs, kBadPosition, token);
+        } else {
+          const uint32_t entry = static_cast<uint32_t>(at) / static_cast<uint32_t>(p.page_size);
+          const int page = p.table[static_cast<int64_t>(b) * p.table_stride + entry];
+          ok = page >= 0 && page < p.num_pages;
+          if (!ok && g == 0) st_record(p.status, kStatusBadArgs, kBadPage, page);
+          dst = static_cast<int64_t>(page) * op.out_t +
+                (at - static_cast<int64_t>(entry) * p.page_size) * p.dim;
+        }
+      }
     }
-    at = static_cast<int64_t>(p.ctx[b]) + (token - first);
-    if (op.paged) {
-      const int64_t entry = at / p.page_size;
-      if (at < 0 || entry >= p.table_w) {
-        if (task == 0 && g == 0) st_record(p.status, kStatusBadArgs, kBadPosition, token);
-        return;
-      }
-      const int page = p.table[static_cast<int64_t>(b) * p.table_stride + entry];
-      if (page < 0 || page >= p.num_pages) {
-        if (task == 0 && g == 0) st_record(p.status, kStatusBadArgs, kBadPage, page);
-        return;
-      }
-      dst = static_cast<int64_t>(page) * op.out_t + (at - entry * p.page_size) * p.dim;
-    }
+    s_dst[threadIdx.x] = dst;
+    s_ok[threadIdx.x] = ok;
+    if (p.positions != nullptr)
+      at = p.positions64 ? static_cast<const int64_t*>(p.positions)[token]
+                         : static_cast<int64_t>(static_cast<const int*>(p.positions)[token]);
+    s_pos[threadIdx.x] = at;
   }
+  const int pairs = op.rotate ? p.rotary_dim / 2 : 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < tokens * pairs; i += kRopeThreads) {
+    const int t = i / pairs, pair = i - t * pairs;
+    const uint64_t phase = static_cast<uint64_t>(s_pos[t]) * phase_step(p.inv_freq[pair]);
+    const int top = static_cast<int>((phase + 0x80000000ull) >> 32);
+    float sn, cs;
+    sincospif(static_cast<float>(top) * 0x1p-31f, &sn, &cs);
+    s_cs[t * pairs + cs_slot<VEC>(pair, pairs)] = make_float2(cs * p.scale, sn * p.scale * p.sign);
+  }
+  __syncthreads();
 
-  const int rot_tasks = op.rotate ? p.rotary_dim / (2 * VEC) : 0;
+  const int rows_step = kRopeThreads / tasks;
+  const int task = threadIdx.x % tasks, sub = threadIdx.x / tasks;
+  if (sub >= rows_step) return;
+  const int rot_tasks = pairs / VEC;
   const bool rot = task < rot_tasks;
-  const int rest = rot_tasks * 2 * VEC;  // first element that passes through
   int ea, eb;
   if (rot && !kInter) {
     ea = task * VEC;
-    eb = p.rotary_dim / 2 + task * VEC;
-  } else {
-    ea = rot ? task * 2 * VEC : rest + (task - rot_tasks) * 2 * VEC;
+    eb = pairs + task * VEC;
+  } else {  // pairs side by side, or elements behind the rotated ones
+    ea = task * 2 * VEC;
     eb = ea + VEC;
   }
-  if (ea >= p.dim) return;
   const bool two = eb < p.dim;
-
-  float cs[VEC], sn[VEC];
-  if (rot) {
-    int64_t pos = at;
-    if (p.positions != nullptr)
-      pos = p.positions64 ? static_cast<const int64_t*>(p.positions)[token]
-                          : static_cast<int64_t>(static_cast<const int*>(p.positions)[token]);
+  const T* in = static_cast<const T*>(op.in) + static_cast<int64_t>(token0) * op.in_t +
+                static_cast<int64_t>(h0) * op.in_h;
+  T* out = static_cast<T*>(op.out) + static_cast<int64_t>(h0) * op.out_h;
+  const int rows = tokens * heads;
+  int t = sub / heads, h = sub - t * heads;
+  const int step_t = rows_step / heads, step_h = rows_step - step_t * heads;
+  for (int row = sub; row < rows; row += kRopeRows * rows_step) {
+    P a[kRopeRows], b[kRopeRows];
+    T* w[kRopeRows];
+    int tt[kRopeRows];
+    bool have[kRopeRows];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const uint64_t phase = static_cast<uint64_t>(pos) * phase_step(p.inv_freq[task * VEC + i]);
-      const int top = static_cast<int>((phase + 0x80000000ull) >> 32);
-      sincospif(static_cast<float>(top) * 0x1p-31f, &sn[i], &cs[i]);
-      cs[i] *= p.scale;
-      sn[i] *= p.scale * p.sign;
-    }
-  }
-
-  const T* in = static_cast<const T*>(op.in) + static_cast<int64_t>(token) * op.in_t;
-  T* out = static_cast<T*>(op.out) + dst;
-  constexpr int kU = 4;
-  for (int h = g * hc; h < h_end; h += kU) {
-    P a[kU], b[kU];
-#pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      if (h + u < h_end) {
-        const T* r = in + static_cast<int64_t>(h + u) * op.in_h;
+    for (int u = 0; u < kRopeRows; ++u) {
+      have[u] = row + u * rows_step < rows && s_ok[t];
+      tt[u] = t;
+      if (have[u]) {
+        const T* r = in + static_cast<int64_t>(t) * op.in_t + static_cast<int64_t>(h) * op.in_h;
         a[u] = *reinterpret_cast<const P*>(r + ea);
         if (two) b[u] = *reinterpret_cast<const P*>(r + eb);
+        w[u] = out + s_dst[t] + static_cast<int64_t>(h) * op.out_h;
       }
+      t += step_t;
+      h += step_h;
+      if (h >= heads) {
+        h -= heads;
+        ++t;
+      }
+      t = min(t, kRopeTokens - 1);  // past the last row: any slot
     }
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      if (h + u < h_end) {
-        if (rot) rotate<T, VEC, kInter>(a[u], b[u], cs, sn);
-        T* w = out + static_cast<int64_t>(h + u) * op.out_h;
-        *reinterpret_cast<P*>(w + ea) = a[u];
-        if (two) *reinterpret_cast<P*>(w + eb) = b[u];
+    for (int u = 0; u < kRopeRows; ++u) {
+      if (have[u]) {
+        if (rot) {
+          float cs[VEC], sn[VEC];
+          const float2* c = s_cs + tt[u] * pairs;
+          if constexpr (VEC == 1) {
+            cs[0] = c[task].x;
+            sn[0] = c[task].y;
+          } else {
+#pragma unroll
+            for (int i = 0; i < VEC; i += 2) {
+              const float4 v = *reinterpret_cast<const float4*>(c + i * rot_tasks + 2 * task);
+              cs[i] = v.x;
+              sn[i] = v.y;
+              cs[i + 1] = v.z;
+              sn[i + 1] = v.w;
+            }
+          }
+          rotate<T, VEC, kInter>(a[u], b[u], cs, sn);
+        }
+        *reinterpret_cast<P*>(w[u] + ea) = a[u];
+        if (two) *reinterpret_cast<P*>(w[u] + eb) = b[u];
       }
     }
   }
@@ -199,18 +250,22 @@ template <typename T, int VEC, bool kInter>
 int rope_run(const RopeParams& p, cudaStream_t stream) {
   // a row's tasks: two vectors each; one more when the dims leave a single vector over
   const int tasks = (p.dim + 2 * VEC - 1) / (2 * VEC);
-  // rows wider than a block are not offered (the bindings bound dim)
-  const int tpb = kRopeThreads / tasks;
-  const int gx = (p.tokens + tpb - 1) / tpb;
-  int hc = 16, gy = 0;
-  // shrink the head group until there are eight blocks per SM: each block
-  // repeats its tokens' sines, which is cheap beside idle SMs
-  for (; hc >= 1; hc >>= 1) {
+  // Tokens of a block and heads of a group: as many as leave eight blocks per SM;
+  // few tokens are cut into single ones and the heads into small groups, so that
+  // a decoding step spreads over the GPU (each block forms its sines itself,
+  // which is cheap beside idle SMs).
+  const int want = 148 * 8;
+  int tb = kRopeTokens, hc = 64, gy = 0;
+  auto blocks = [&] {
     gy = 0;
     for (int i = 0; i < p.n_op; ++i) gy += (p.op[i].heads + hc - 1) / hc;
-    if (hc == 1 || static_cast<int64_t>(gx) * gy >= 148 * 8) break;
-  }
-  rope_kernel<T, VEC, kInter><<<dim3(gx, gy), kRopeThreads, 0, stream>>>(p, tasks, tpb, hc);
+    return static_cast<int64_t>((p.tokens + tb - 1) / tb) * gy;
+  };
+  while (blocks() < want && tb > 1) tb >>= 1;
+  while (blocks() < want && hc > 4) hc >>= 1;
+  const size_t smem = static_cast<size_t>(tb) * (p.rotary_dim / 2) * sizeof(float2);
+  rope_kernel<T, VEC, kInter>
+      <<<dim3((p.tokens + tb - 1) / tb, gy), kRopeThreads, smem, stream>>>(p, tasks, tb, hc);
   return static_cast<int>(cudaGetLastError());
 }
 

@@ -358,14 +358,14 @@ __global__ void __launch_bounds__(kMergeThreads)
       float4 o[8];
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        // past the last: the same record again, left out below
-        const int i = min(i0 + u * i_step, n - 1);
         // the first record is the last piece of CTA c0, the others the first of each
-        const int k = 2 * (c0 + i) + (i == 0 ? 1 : 0);
-        m[u] = p.rec_m[k * rows_per_unit + r];
-        l[u] = p.rec_l[k * rows_per_unit + r];
-        o[u] = *reinterpret_cast<const float4*>(
-            p.rec_acc + static_cast<int64_t>(k) * rows_per_unit * D + e * 4);
+        const int i = i0 + u * i_step, k = 2 * (c0 + i) + (i == 0 ? 1 : 0);
+        if (i < n) {
+          m[u] = p.rec_m[k * rows_per_unit + r];
+          l[u] = p.rec_l[k * rows_per_unit + r];
+          o[u] = *reinterpret_cast<const float4*>(
+              p.rec_acc + static_cast<int64_t>(k) * rows_per_unit * D + e * 4);
+        }
       }
 #pragma unroll
       for (int u = 0; u < 8; ++u)
@@ -418,14 +418,14 @@ int run_simt(const TreeParams& p, cudaStream_t stream) {
 }
 
 template <typename T, int D>
-int run_merge(const TreeParams& p, int rows_per_unit, cudaStream_t stream) {
+int run_merge(const TreeParams& p, int rows_per_unit, int merge_rows, cudaStream_t stream) {
   cudaLaunchAttribute overlap;
   overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   overlap.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  // a block per 128 elements up to 32 of them; blocks without a unit leave at once
-  const int blocks = rows_per_unit * (D / 4) / kMergeThreads;
-  cfg.gridDim = dim3(p.grid, blocks < 1 ? 1 : (blocks < 32 ? blocks : 32));
+  // a block per 128 elements of the largest unit, up to 64; blocks without a unit leave at once
+  const int blocks = (merge_rows * (D / 4) + kMergeThreads - 1) / kMergeThreads;
+  cfg.gridDim = dim3(p.grid, blocks < 64 ? blocks : 64);
   cfg.blockDim = dim3(kMergeThreads);
   cfg.stream = stream;
   cfg.attrs = &overlap;
@@ -498,6 +498,9 @@ TreePlan tree_plan(Elem elem, const TreeParams& p, int max_q, int sms) {
     plan.rows_per_unit = static_cast<int64_t>(max_q) * p.group > 128 ? 256 : 128;
     plan.grid = sms;
   }
+  // rows of the largest unit that can occur (max_q is a hint: the merge loops)
+  const int64_t most = static_cast<int64_t>(max_q) * p.group;
+  plan.merge_rows = static_cast<int>(most < plan.rows_per_unit ? most : plan.rows_per_unit);
   const size_t rows = static_cast<size_t>(2) * plan.grid * plan.rows_per_unit;
   plan.acc_floats = rows * p.dim;
   plan.ml_floats = 2 * rows;
@@ -515,14 +518,14 @@ int tree_launch(Elem elem, const TreeParams& p, const TreePlan& plan, cudaStream
   if (err != 0) return err;
   switch (elem) {
     case Elem::kBF16:
-      return p.dim == 64 ? run_merge<__nv_bfloat16, 64>(p, rows, stream)
-                         : run_merge<__nv_bfloat16, 128>(p, rows, stream);
+      return p.dim == 64 ? run_merge<__nv_bfloat16, 64>(p, rows, plan.merge_rows, stream)
+                         : run_merge<__nv_bfloat16, 128>(p, rows, plan.merge_rows, stream);
     case Elem::kF16:
-      return p.dim == 64 ? run_merge<__half, 64>(p, rows, stream)
-                         : run_merge<__half, 128>(p, rows, stream);
+      return p.dim == 64 ? run_merge<__half, 64>(p, rows, plan.merge_rows, stream)
+                         : run_merge<__half, 128>(p, rows, plan.merge_rows, stream);
     default:
-      return p.dim == 64 ? run_merge<float, 64>(p, rows, stream)
-                         : run_merge<float, 128>(p, rows, stream);
+      return p.dim == 64 ? run_merge<float, 64>(p, rows, plan.merge_rows, stream)
+                         : run_merge<float, 128>(p, rows, plan.merge_rows, stream);
   }
 }
 

@@ -322,43 +322,75 @@ void copy_pages(torch::Tensor k_pages, torch::Tensor v_pages, torch::Tensor src,
                                             : static_cast<const int64_t*>(t.data_ptr())[i];
   };
   // every page is written once at most, and none that is also read: the copies
-  // of a launch run at the same time
-  std::vector<uint8_t> written(static_cast<size_t>(pages), 0);
+  // of a launch run at the same time.  `mark`: a page that is written, or the
+  // number of the group of pairs that read it.
+  constexpr int kFree = -1, kWritten = -2;
+  std::vector<int> mark(static_cast<size_t>(pages), kFree);
   for (int64_t i = 0; i < n; ++i) {
     const int64_t x = at(dst, i);
     RAB_CHECK(x >= 0 && x < pages, "dst[%lld] = %lld is no page of a pool of %lld", ll(i), ll(x),
               ll(pages));
-    RAB_CHECK(!written[static_cast<size_t>(x)], "page %lld is twice in dst", ll(x));
-    written[static_cast<size_t>(x)] = 1;
+    RAB_CHECK(mark[static_cast<size_t>(x)] == kFree, "page %lld is twice in dst", ll(x));
+    mark[static_cast<size_t>(x)] = kWritten;
   }
+  std::vector<int> group(static_cast<size_t>(n)), sources, count;
   for (int64_t i = 0; i < n; ++i) {
     const int64_t x = at(src, i);
     RAB_CHECK(x >= 0 && x < pages, "src[%lld] = %lld is no page of a pool of %lld", ll(i), ll(x),
               ll(pages));
-    RAB_CHECK(!written[static_cast<size_t>(x)], "page %lld is both in src and in dst", ll(x));
+    int& m = mark[static_cast<size_t>(x)];
+    RAB_CHECK(m != kWritten, "page %lld is both in src and in dst", ll(x));
+    if (m == kFree) {
+      m = static_cast<int>(sources.size());
+      sources.push_back(static_cast<int>(x));
+      count.push_back(0);
+    }
+    group[static_cast<size_t>(i)] = m;
+    ++count[static_cast<size_t>(m)];
   }
+  // the pairs in the order of their groups
+  std::vector<int> place(sources.size() + 1, 0), sorted(static_cast<size_t>(n));
+  for (size_t s = 0; s < sources.size(); ++s) place[s + 1] = place[s] + count[s];
+  const std::vector<int> begin = place;
+  for (int64_t i = 0; i < n; ++i)
+    sorted[static_cast<size_t>(place[static_cast<size_t>(group[static_cast<size_t>(i)])]++)] =
+        static_cast<int>(at(dst, i));
   RAB_CHECK(k_pages.is_cuda(), "k_pages must be a CUDA tensor");
   check_same(v_pages, "v_pages", k_pages);
   const c10::cuda::CUDAGuard guard(k_pages.device());
   const int64_t es = k_pages.element_size();
-  PageCopyParams p;
-  p.k = static_cast<uint8_t*>(k_pages.data_ptr());
-  p.v = static_cast<uint8_t*>(v_pages.data_ptr());
-  p.k_page = k_pages.stride(d - 4) * es;
-  p.v_page = v_pages.stride(d - 4) * es;
-  p.layers = d == 5 ? static_cast<int>(k_pages.size(0)) : 1;
-  p.k_layer = d == 5 ? k_pages.stride(0) * es : 0;
-  p.v_layer = d == 5 ? v_pages.stride(0) * es : 0;
-  p.page_bytes = k_pages.size(d - 3) * k_pages.size(d - 2) * k_pages.size(d - 1) * es;
-  for (int64_t i = 0; i < n; i += kMaxPagePairs) {
-    p.n = static_cast<int>(std::min<int64_t>(kMaxPagePairs, n - i));
-    for (int j = 0; j < p.n; ++j) {
-      p.src[j] = static_cast<int>(at(src, i + j));
-      p.dst[j] = static_cast<int>(at(dst, i + j));
+  auto launch = [&](auto& p) {
+    constexpr int kMax = std::remove_reference_t<decltype(p)>::kMax;
+    p.k = static_cast<uint8_t*>(k_pages.data_ptr());
+    p.v = static_cast<uint8_t*>(v_pages.data_ptr());
+    p.k_page = k_pages.stride(d - 4) * es;
+    p.v_page = v_pages.stride(d - 4) * es;
+    p.layers = d == 5 ? static_cast<int>(k_pages.size(0)) : 1;
+    p.k_layer = d == 5 ? k_pages.stride(0) * es : 0;
+    p.v_layer = d == 5 ? v_pages.stride(0) * es : 0;
+    p.page_bytes = k_pages.size(d - 3) * k_pages.size(d - 2) * k_pages.size(d - 1) * es;
+    size_t s = 0;
+    for (int i = 0; i < n; i += kMax) {  // a group cut here reads its page again
+      const int end = static_cast<int>(std::min<int64_t>(n, i + kMax));
+      p.n_src = 0;
+      p.first[0] = 0;
+      std::copy(sorted.begin() + i, sorted.begin() + end, p.dst);
+      for (; s < sources.size() && begin[s] < end; ++s) {
+        p.src[p.n_src] = sources[s];
+        p.first[++p.n_src] = std::min(begin[s + 1], end) - i;
+        if (begin[s + 1] > end) break;
+      }
+      const int err = page_copy_launch(p, cur_stream());
+      RAB_CHECK(err == 0, "copy_pages launch failed: %s",
+                cudaGetErrorString(static_cast<cudaError_t>(err)));
     }
-    const int err = page_copy_launch(p, cur_stream());
-    RAB_CHECK(err == 0, "copy_pages launch failed: %s",
-              cudaGetErrorString(static_cast<cudaError_t>(err)));
+  };
+  if (n <= kFewPairs) {
+    PageCopyParams<kFewPairs> p;
+    launch(p);
+  } else {
+    PageCopyParams<kManyPairs> p;
+    launch(p);
   }
 }
 
