@@ -49,7 +49,11 @@ constexpr int kPathSteps = 64;  // steps whose places a block holds at a time
 // [heads, dim] row and walks the path in order.  Places increase, so what step
 // i writes (place i) lies before every place a later step reads (path[j] >= j
 // > i): the walk is safe in place without a second buffer.  The steps' byte
-// offsets are formed once per block, eight loads are in flight per thread.
+// offsets are formed once per block, eight loads are in flight per thread.  Bound
+// by DRAM at its grain: a token's row of one head is 128 to 512 bytes alone in its
+// page.  128 paths of 9 in 64 tokens, 16 layers of 8 heads x 128 fp16: 24.7 us, 117
+// MB at 4.8 TB/s; two to nine loads in flight, 64 to 256 threads and twice the
+// blocks per SM all measured 25 to 29 us.
 __global__ void __launch_bounds__(kPathThreads) path_kernel(const __grid_constant__ PathParams p) {
   __shared__ int64_t s_from[kPathSteps], s_to[kPathSteps];
   __shared__ int s_bad;
