@@ -5,6 +5,7 @@
 
 #include <cstdint>
 
+#include "launch.h"
 #include "paged.h"
 
 namespace rab {
@@ -30,6 +31,8 @@ __global__ void __launch_bounds__(kCopyThreads)
   const int64_t i0 = static_cast<int64_t>(blockIdx.x) * (kCopyThreads * kCopyUnroll) + threadIdx.x;
   const uint4* src = reinterpret_cast<const uint4*>(base + p.src[s] * page) + i0;
   uint4 x[kCopyUnroll];
+  let_successor_start();
+  wait_for_predecessor();
 #pragma unroll
   for (int u = 0; u < kCopyUnroll; ++u)
     if (i0 + u * kCopyThreads < n) x[u] = __ldcs(src + u * kCopyThreads);
@@ -60,6 +63,8 @@ __global__ void __launch_bounds__(kPathThreads) path_kernel(const __grid_constan
   const int b = blockIdx.x;
   const int layer = blockIdx.y >> 1;
   const bool is_v = blockIdx.y & 1;
+  let_successor_start();
+  wait_for_predecessor();
   const int n = p.path_lens[b];
   if (n <= 0) return;
   const int ctx = p.ctx[b];
@@ -126,8 +131,7 @@ int copy_run(const PageCopyParams<kPairs>& p, cudaStream_t stream) {
   if (p.n_src == 0 || p.layers == 0 || p.page_bytes == 0) return 0;
   const dim3 grid(static_cast<unsigned>((p.page_bytes + kCopyChunk - 1) / kCopyChunk), p.n_src,
                   2 * p.layers);
-  page_copy_kernel<kPairs><<<grid, kCopyThreads, 0, stream>>>(p);
-  return static_cast<int>(cudaGetLastError());
+  return launch_overlapped(page_copy_kernel<kPairs>, grid, kCopyThreads, 0, stream, &p);
 }
 
 }  // namespace
@@ -141,8 +145,7 @@ int page_copy_launch(const PageCopyParams<kManyPairs>& p, cudaStream_t stream) {
 
 int path_compact_launch(const PathParams& p, cudaStream_t stream) {
   if (p.batch == 0 || p.layers == 0 || p.path_w == 0) return 0;
-  path_kernel<<<dim3(p.batch, 2 * p.layers), kPathThreads, 0, stream>>>(p);
-  return static_cast<int>(cudaGetLastError());
+  return launch_overlapped(path_kernel, dim3(p.batch, 2 * p.layers), kPathThreads, 0, stream, &p);
 }
 
 }  // namespace rab

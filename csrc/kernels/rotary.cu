@@ -25,6 +25,7 @@
 
 #include <cstdint>
 
+#include "launch.h"
 #include "paged.h"
 
 namespace rab {
@@ -127,6 +128,7 @@ __global__ void __launch_bounds__(kRopeThreads, 8)
   extern __shared__ __align__(16) float2 s_cs[];  // [tb][rotary_dim / 2]
   __shared__ int64_t s_dst[kRopeTokens], s_pos[kRopeTokens];
   __shared__ int s_ok[kRopeTokens];
+  let_successor_start();
   int o = 0, g = blockIdx.y;
   while (o + 1 < p.n_op && g >= (p.op[o].heads + hc - 1) / hc) {
     g -= (p.op[o].heads + hc - 1) / hc;
@@ -155,6 +157,7 @@ __global__ void __launch_bounds__(kRopeThreads, 8)
                 static_cast<int64_t>(h0) * op.in_h;
   int row = sub < rows_step ? sub : tokens * heads;
   int t = sub / heads, h = sub - t * heads;
+  wait_for_predecessor();
   const int step_t = rows_step / heads, step_h = rows_step - step_t * heads;
   if (row < tokens * heads) {  // holds no registers until it is used
     const T* r = in + static_cast<int64_t>(t) * op.in_t + static_cast<int64_t>(h) * op.in_h;
@@ -268,9 +271,8 @@ int rope_run(const RopeParams& p, cudaStream_t stream) {
     if (tb == 1) hc = kRopeThreads / tasks;
   }
   const size_t smem = static_cast<size_t>(tb) * (p.rotary_dim / 2) * sizeof(float2);
-  rope_kernel<T, VEC, kInter>
-      <<<dim3((p.tokens + tb - 1) / tb, gy), kRopeThreads, smem, stream>>>(p, tasks, tb, hc);
-  return static_cast<int>(cudaGetLastError());
+  return launch_overlapped(rope_kernel<T, VEC, kInter>, dim3((p.tokens + tb - 1) / tb, gy),
+                           kRopeThreads, smem, stream, &p, &tasks, &tb, &hc);
 }
 
 template <typename T, int VEC>

@@ -36,6 +36,7 @@
 
 #include <cstdint>
 
+#include "launch.h"
 #include "paged.h"
 #include "sm100.cuh"
 #include "tmap.h"
@@ -222,6 +223,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // the swizzle of the tiles counts from 1024-byte boundaries; the block has no
   // other shared memory, so its dynamic part starts on one
   if ((smem_u32(smem) & 1023u) != 0) {
+    wait_for_predecessor();
     if (threadIdx.x == 0) {
       p.meta[blockIdx.x * kMetaInts] = 0;
       st_record(st, kStatusBadArgs, kSiteNone);
@@ -255,6 +257,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_alloc(s_tmem, kCols);
     tmem_relinquish();
   }
+  let_successor_start();
+  wait_for_predecessor();
   const Range range = find_range<kN, kRows, kThreads>(p, s_sums, s_start);
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
@@ -328,11 +332,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      if (!ok) {  // the loads in flight land before the block gives its memory back
-        for (int i = 0; i < NS && i < n; ++i) {
-          const int k = n - 1 - i;
-          mbar_wait(&full[k % NS], (k / NS) & 1, nullptr, kSiteKFull, 100000000ull);
-        }
+      // the loads in flight land before the block gives its memory back
+      for (int i = 0; i < NS && i < n; ++i) {
+        const int k = n - 1 - i;
+        mbar_wait(&full[k % NS], (k / NS) & 1, nullptr, kSiteKFull, 100000000ull);
       }
     } else if (warp == 1) {
       // ------------------------------------------------------------------ MMA
@@ -716,8 +719,8 @@ int launch(const TreeParams& p, const CUtensorMap& k, const CUtensorMap& v, cuda
     if (err != cudaSuccess) return static_cast<int>(err);
     if (dev >= 0 && dev < 64) done[dev] = true;
   }
-  tree_attn_kernel<D, kBF16, kTwoRows><<<p.grid, kThreads, C::kSmem, stream>>>(p, k, v);
-  return static_cast<int>(cudaGetLastError());
+  return launch_overlapped(tree_attn_kernel<D, kBF16, kTwoRows>, dim3(p.grid), kThreads, C::kSmem,
+                           stream, &p, &k, &v);
 }
 
 CUtensorMap pool_map(const TreeParams& p, const void* base, int64_t page_stride) {
