@@ -19,6 +19,14 @@ def __getattr__(name):
         from .models.ring_attention import RingAttention
 
         return RingAttention
+    if name == "PagedKVCache":
+        from .models.kv_cache import PagedKVCache
+
+        return PagedKVCache
+    if name == "Rotary":
+        from .ops.rotary import Rotary
+
+        return Rotary
     if name == "RingRuntime":
         from .parallel.dist import RingRuntime
 
