@@ -68,7 +68,10 @@ struct Cfg {
   static constexpr int kQBytes = (kTwoRows ? 2 : 1) * kM * D * 2;
   // K and V tiles take turns in one ring: what is left of 227 KB beside the queries
   static constexpr int kStages = D == 64 ? (kTwoRows ? 10 : 12) : (kTwoRows ? 5 : 6);
-  static constexpr int kBars = 2 * kStages + 2 + 2 + 2 + 4 + 2 * kItems;
+  // softmax hands P over in this many parts: with two, the PV products of the first
+  // 64 keys start while the second half's exponentials form
+  static constexpr int kParts = kTwoRows ? 2 : 1;
+  static constexpr int kBars = 2 * kStages + 2 + 2 + 2 + 4 + 2 * kItems + 2;
   static constexpr int kBarOff = kQBytes + kStages * kTile;
   static constexpr int kMlOff = kBarOff + kBars * 8;       // float2 [2][128]
   static constexpr int kItemOff = kMlOff + 2 * kM * 8;     // Piece [kItems]
@@ -207,6 +210,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* drain = q_full + 9;
   uint64_t* item_full = q_full + 10;           // [kItems]
   uint64_t* item_empty = item_full + kItems;   // [kItems]
+  uint64_t* p_hi = item_empty + kItems;        // [2], with two parts
   float2* s_ml = reinterpret_cast<float2*>(smem + C::kMlOff);
   int* s_sums = reinterpret_cast<int*>(smem + C::kSumOff);
   int* s_misc = reinterpret_cast<int*>(smem + C::kMiscOff);
@@ -241,6 +245,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int x = 0; x < 2; ++x) {
       mbar_init(&s_full[x], 1);
       mbar_init(&p_full[x], 4);
+      mbar_init(&p_hi[x], 4);
     }
     mbar_init(o_final, 1);
     mbar_init(o_free, 8);
@@ -359,13 +364,20 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           mma_commit(&s_full[x]);
         };
-        auto pv = [&](int x, int g, bool first) {
+        auto pv = [&](int x, int g, bool first) -> bool {
           const uint32_t vb = kvb + ((2 * g + 1) % NS) * C::kTile;
 #pragma unroll
-          for (int ks = 0; ks < kN / 16; ++ks)
+          for (int ks = 0; ks < kN / 16; ++ks) {
+            if (C::kParts == 2 && ks == kN / 32) {
+              if (!mbar_wait(&p_hi[x], px[x] & 1, st, kSitePFull, tmo)) return false;
+              tc_fence_after();
+            }
             mma_ts<false>(tmem + 256 + x * 128, tmem + x * 128 + ks * 8,
                           make_sdesc(vb + ks * 2048, kN * 128, 1024), kIdescPV,
                           (first && ks == 0) ? 0u : 1u);
+          }
+          ++px[x];
+          return true;
         };
         auto wait_p = [&](int x) {
           return mbar_wait(&p_full[x], px[x] & 1, st, kSitePFull, tmo);
@@ -398,9 +410,9 @@ __global__ void __launch_bounds__(kThreads, 1)
               const int x = j & 1;
               ok = wait_p(x) && wait_tile(2 * (g0 + j) + 1, kSiteVFull) && (j > 0 || wait_o());
               if (!ok) break;
-              ++px[x];
               tc_fence_after();
-              pv(x, g0 + j, j < 2);
+              ok = pv(x, g0 + j, j < 2);
+              if (!ok) break;
               mma_commit(&empty[(2 * (g0 + j) + 1) % NS]);
               if (j + 2 < n) ok = next_qk(j + 2);
             }
@@ -411,9 +423,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (x == 0 && (c.tile_begin + j + 1) * kN > c.ctx && !wait_p(1)) return false;
               if (x == 0 && !wait_tile(2 * (g0 + j) + 1, kSiteVFull)) return false;
               if (x == 0 && j == 0 && !wait_o()) return false;
-              ++px[x];
               tc_fence_after();
-              pv(x, g0 + j, j == 0);
+              if (!pv(x, g0 + j, j == 0)) return false;
               if (x == 1) mma_commit(&empty[(2 * (g0 + j) + 1) % NS]);
               return true;
             };
@@ -454,18 +465,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (c.request < 0) break;
         ok = __all_sync(0xffffffffu, mbar_wait(q_empty, (w & 1) ^ 1, st, kSiteQFull, tmo));
         if (!ok) break;
-        // rows behind the unit's last keep what they held: an MMA row is its own
+        // Rows behind the unit's last are zeros: an MMA row is its own, but products of
+        // zeros draw less power, which is what bounds the clock here (32 trees,
+        // 128-row tiles 58 % full: POWER_NOTE).
         constexpr int kChunks = D / 8;
         const uint32_t qb = smem_u32(sQ);
         const int h0 = c.head_kv * p.group;
-        for (int i = tid; i < c.rows * kChunks; i += 64) {
+        for (int i = tid; i < kRows * kChunks; i += 64) {
           const int r = i / kChunks, x = i % kChunks;
+          const uint32_t at = qb + (r / kM) * (kM * D * 2) + (x / 8) * (kM * 128) +
+                              (r % kM) * 128 + (((x % 8) ^ (r & 7)) << 4);
+          if (r >= c.rows) {
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+            continue;
+          }
           const int row = c.row0 + r, t = row / p.group, h = h0 + row - t * p.group;
           const uint16_t* src = static_cast<const uint16_t*>(p.q) +
                                 static_cast<int64_t>(c.first + t) * p.q_t + h * p.q_h + x * 8;
-          const uint32_t dst = qb + (r / kM) * (kM * D * 2) + (x / 8) * (kM * 128) +
-                               (r % kM) * 128 + (((x % 8) ^ (r & 7)) << 4);
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(src) : "memory");
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         fence_proxy_async_smem();
@@ -497,7 +514,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int old_keys = c->ctx - c->tile_begin * kN;  // of the piece, before the new tokens
       const int r = kTwoRows ? x * kM + row : row;  // row of the unit
       // a warp without rows only keeps the order of things
-      const bool active = r - static_cast<int>(lane_id()) < c->rows;
+      const int rows = c->rows;
+      const bool active = r - static_cast<int>(lane_id()) < rows;
       const uint32_t o_col = tmem + lane_base + 256 + x * 128;
       float m_run = -INFINITY, l_run = 0.f;
       for (int j = kTwoRows ? 0 : x; j < n; j += kTwoRows ? 1 : 2) {
@@ -568,7 +586,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               tmem_st32(o_col + k, o);
             }
           }
-          const float m_use = m_run == -INFINITY ? 0.f : m_run;
+          // a row of the tile that is none of the unit's gets weights of zero
+          const float m_use = r >= rows ? INFINITY : (m_run == -INFINITY ? 0.f : m_run);
           const float2 scale2 = make_float2(sl2, sl2);
           const float2 shift2 = make_float2(-m_use, -m_use);
           float2 ps[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
@@ -587,14 +606,23 @@ __global__ void __launch_bounds__(kThreads, 1)
               pk[q] = pack2<kBF16>(e.x, e.y);
             }
             tmem_st32(s_col + hlf * 32, pk);
+            if (C::kParts == 2 && hlf == 0) {
+              tmem_st_wait();
+              tc_fence_before();
+              __syncwarp();
+              if (lane_id() == 0) mbar_arrive(&p_full[x]);
+            }
           }
           const float2 sum = fadd2(fadd2(ps[0], ps[1]), fadd2(ps[2], ps[3]));
           l_run += sum.x + sum.y;
           tmem_st_wait();
+        } else if (C::kParts == 2) {
+          __syncwarp();
+          if (lane_id() == 0) mbar_arrive(&p_full[x]);
         }
         tc_fence_before();
         __syncwarp();
-        if (lane_id() == 0) mbar_arrive(&p_full[x]);
+        if (lane_id() == 0) mbar_arrive(C::kParts == 2 ? &p_hi[x] : &p_full[x]);
       }
       if (!ok) break;
       // ------------------------------------------------------------ results
@@ -618,8 +646,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           m_run = top;
           l_run = f0 * a.y + f1 * b.y;
         }
-        const bool mine = r < c->rows;
-        const int record = c->record, rows = c->rows;
+        const bool mine = r < rows;
+        const int record = c->record;
         const int out_row = c->row0 + r;
         const int t = static_cast<int>(static_cast<uint32_t>(out_row) /
                                        static_cast<uint32_t>(p.group));

@@ -3,6 +3,7 @@
 // shapes, types and strides first, then the devices, so a refused call raises a
 // RuntimeError before anything is launched.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <pybind11/stl.h>
 #include <torch/extension.h>
@@ -49,6 +50,12 @@ void check_rows(const torch::Tensor& t, const char* name) {
   RAB_CHECK(t.dim() == 3, "%s must be [tokens, heads, dim]", name);
   RAB_CHECK(t.size(2) == 1 || t.stride(2) == 1, "%s must be contiguous in its last dimension", name);
   RAB_CHECK(t.size(0) <= INT32_MAX && t.size(1) <= 65535, "%s is too large", name);
+}
+
+// A new contiguous tensor, straight from the caching allocator: torch::empty goes
+// through the dispatcher, which costs a short call about a microsecond a tensor.
+torch::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const torch::Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
 }
 
 bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
@@ -154,9 +161,9 @@ std::tuple<torch::Tensor, OptTensor> rotary(torch::Tensor q, OptTensor k, torch:
   if (q_out) check_same(*q_out, "q_out", q);
   if (k_out) check_same(*k_out, "k_out", q);
   const c10::cuda::CUDAGuard guard(q.device());
-  torch::Tensor qo = q_out ? *q_out : torch::empty(q.sizes(), q.options());
+  torch::Tensor qo = q_out ? *q_out : fresh(q.sizes(), q.scalar_type(), q);
   OptTensor ko = k_out;
-  if (k && !ko) ko = torch::empty(k->sizes(), k->options());
+  if (k && !ko) ko = fresh(k->sizes(), k->scalar_type(), q);
   p.interleaved = interleaved;
   p.scale = static_cast<float>(scale);
   p.sign = inverse ? -1.f : 1.f;
@@ -273,7 +280,7 @@ OptTensor append_kv(torch::Tensor k, torch::Tensor v, torch::Tensor k_pages, tor
   bool vec = rope_vectors(e, dim, p.rotary_dim, interleaved) && rows_aligned(k) && rows_aligned(v);
   OptTensor qo = q_out;
   if (q) {
-    if (!qo) qo = torch::empty(q->sizes(), q->options());
+    if (!qo) qo = fresh(q->sizes(), q->scalar_type(), k);
     if (q->size(1) > 0) {
       p.op[p.n_op++] = dense_operand(*q, *qo);
       vec = vec && rows_aligned(*q) && rows_aligned(*qo);
@@ -495,15 +502,15 @@ std::tuple<torch::Tensor, OptTensor> tree_attention(torch::Tensor q, torch::Tens
   p.status = status_of(status, q);
   const c10::cuda::CUDAGuard guard(q.device());
   if (!rows_aligned(q)) q = q.contiguous();
-  torch::Tensor o = out ? *out : torch::empty({total, heads, dim}, q.options());
+  torch::Tensor o = out ? *out : fresh({total, heads, dim}, q.scalar_type(), q);
   OptTensor lse;
-  if (return_lse) lse = torch::empty({total, heads}, q.options().dtype(torch::kFloat32));
+  if (return_lse) lse = fresh({total, heads}, torch::kFloat32, q);
   if (total == 0) return {o, lse};
   const cudaStream_t stream = cur_stream();
   torch::Tensor bits;
   if (mask && mask->scalar_type() == torch::kBool) {
     const int64_t words = (mask->size(1) + 31) / 32;
-    bits = torch::empty({total, words}, q.options().dtype(torch::kInt32));
+    bits = fresh({total, words}, torch::kInt32, q);
     const int err = pack_mask_launch(static_cast<const uint8_t*>(mask->data_ptr()), mask->stride(0),
                                      static_cast<int>(total), static_cast<int>(mask->size(1)),
                                      static_cast<uint32_t*>(bits.data_ptr()),
@@ -547,7 +554,7 @@ std::tuple<torch::Tensor, OptTensor> tree_attention(torch::Tensor q, torch::Tens
   const int64_t most = max_q ? std::min<int64_t>(*max_q, total) : (cu ? total : r.uniform);
   const TreePlan plan = tree_plan(e, p, static_cast<int>(most), flash_sm_count());
   const size_t floats = plan.acc_floats + plan.ml_floats + plan.meta_ints;
-  torch::Tensor ws = torch::empty({static_cast<int64_t>(floats)}, q.options().dtype(torch::kFloat32));
+  torch::Tensor ws = fresh({static_cast<int64_t>(floats)}, torch::kFloat32, q);
   p.rec_acc = static_cast<float*>(ws.data_ptr());
   p.rec_m = p.rec_acc + plan.acc_floats;
   p.rec_l = p.rec_m + plan.ml_floats / 2;
@@ -578,8 +585,8 @@ std::tuple<torch::Tensor, torch::Tensor> tree_mask(torch::Tensor parents, OptTen
   DeviceStatus* st = status_of(status, parents);
   const c10::cuda::CUDAGuard guard(parents.device());
   const int64_t words = (max_q + 31) / 32;
-  torch::Tensor mask = torch::empty({total, words}, parents.options());
-  torch::Tensor depth = torch::empty({total}, parents.options());
+  torch::Tensor mask = fresh({total, words}, torch::kInt32, parents);
+  torch::Tensor depth = fresh({total}, torch::kInt32, parents);
   const int err = tree_mask_launch(
       static_cast<const int*>(parents.data_ptr()), cu ? static_cast<const int*>(cu->data_ptr()) : nullptr,
       static_cast<int>(batch), cu ? 0 : static_cast<int>(total / batch), static_cast<int>(total),
@@ -598,7 +605,7 @@ torch::Tensor pack_mask(torch::Tensor mask) {
   RAB_CHECK(mask.is_cuda(), "mask must be a CUDA tensor");
   const c10::cuda::CUDAGuard guard(mask.device());
   const int64_t words = (mask.size(1) + 31) / 32;
-  torch::Tensor bits = torch::empty({mask.size(0), words}, mask.options().dtype(torch::kInt32));
+  torch::Tensor bits = fresh({mask.size(0), words}, torch::kInt32, mask);
   const int err = pack_mask_launch(static_cast<const uint8_t*>(mask.data_ptr()), mask.stride(0),
                                    static_cast<int>(mask.size(0)), static_cast<int>(mask.size(1)),
                                    static_cast<uint32_t*>(bits.data_ptr()), static_cast<int>(words),
