@@ -102,7 +102,7 @@ struct TreeParams {
   const void* k;
   const void* v;
   int64_t k_page, v_page;  // element strides of a page
-  int num_pages, page_size;
+  int num_pages, page_size, page_shift;  // a power of two
   const int* table;
   int64_t table_stride;
   int table_w;

@@ -104,77 +104,73 @@ struct Range {
   }
 };
 
-// Where a range begins: the request that holds its first place, and that
-// request's own first place.  One thread finds it and leaves it in shared memory.
+// Where a range begins: the request that holds its first place, that request's
+// own first place, and the places of one of its kv heads.
 struct Start {
-  int at;
-  int request;
+  int at, request, per_head;
   Request r;
 };
 
-// Whole block executes; `sums` holds an int per warp.  Every CTA reaches the same
-// totals.  Up to kThreads requests are read once and kept in registers.
-template <int kTile, int kRows, int kThreads>
-__device__ __forceinline__ Range find_range(const TreeParams& p, int* sums, Start* start) {
-  constexpr int kWarps = kThreads / 32;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// One warp executes, on its own: nothing but the piece queue ties the block's other
+// warps to it.  Every CTA reaches the same totals.  Returns the lane that holds the
+// range's first request (its `start` is the one filled in) and goes on to walk the
+// range.  A decoding step waits for this before its first load, so up to 32
+// requests take one read and one scan; more are read again to find the first.
+template <int kTile, int kRows>
+__device__ __forceinline__ int find_range(const TreeParams& p, Range* range, Start* start) {
+  const int lane = threadIdx.x & 31;
   Range g;
-  g.total = 0;
-  Request r;
-  int mine = 0, lo = 0;
-  // one block of kThreads requests: adds up, leaves this thread's in r / mine / lo
-  auto block_of = [&](int b0, int before) {
-    const int b = b0 + threadIdx.x;
-    mine = 0;
-    if (b < p.batch) {
-      r = load_request(p, b);
-      mine = head_places<kTile, kRows>(p, r) * p.heads_kv;
-    }
-    int inc = mine;  // inclusive sum over the warp
+  auto places = [&](int b) {
+    if (b >= p.batch) return 0;
+    start->request = b;
+    start->r = load_request(p, b);
+    start->per_head = head_places<kTile, kRows>(p, start->r);
+    if (blockIdx.x == 0 && start->r.tokens > 0 &&
+        (p.ctx[b] < 0 || start->r.keys - start->r.tokens != p.ctx[b]))
+      st_record(p.status, kStatusBadArgs, kBadPosition, b);  // longer than its table
+    return start->per_head * p.heads_kv;
+  };
+  auto scan = [&](int v) {  // inclusive sum over the warp
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int o = __shfl_up_sync(0xffffffffu, inc, d);
-      if (lane >= d) inc += o;
+      const int o = __shfl_up_sync(0xffffffffu, v, d);
+      if (lane >= d) v += o;
     }
-    if (lane == 31) sums[warp] = inc;
-    __syncthreads();
-    int base = before, all = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const int v = sums[w];
-      if (w < warp) base += v;
-      all += v;
-    }
-    lo = base + inc - mine;
-    if (p.batch > kThreads) __syncthreads();  // `sums` is used again
-    return before + all;
+    return v;
   };
-  for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
-    g.total = block_of(b0, g.total);
-    const int b = b0 + threadIdx.x;
-    if (blockIdx.x == 0 && mine > 0 && (p.ctx[b] < 0 || r.keys - r.tokens != p.ctx[b]))
-      st_record(p.status, kStatusBadArgs, kBadPosition, b);  // longer than its table
+  int mine = 0, inc;
+  if (p.batch <= 32) {
+    mine = places(lane);
+    inc = scan(mine);
+  } else {
+    int sum = 0;
+#pragma unroll 4
+    for (int b = lane; b < p.batch; b += 32) sum += places(b);
+    inc = scan(sum);
   }
+  g.total = __shfl_sync(0xffffffffu, inc, 31);
   const int c = blockIdx.x;
   g.grid = min(max(g.total / kMinShare, 1), p.grid);
   g.share = static_cast<int>(static_cast<uint32_t>(g.total) / static_cast<uint32_t>(g.grid));
   g.more = g.total - g.share * g.grid;
   g.begin = c < g.grid ? g.start(c) : g.total;
   g.end = c < g.grid ? g.start(c + 1) : g.total;
+  *range = g;
+  if (g.begin >= g.end) return 0;
   int before = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
-    if (p.batch > kThreads) before = block_of(b0, before);
-    if (mine > 0 && g.begin >= lo && g.begin < lo + mine) {
-      start->at = lo;
-      start->request = b0 + threadIdx.x;
-      start->r = r;
-    }
+  for (int b0 = 0; p.batch > 32; b0 += 32) {  // ends: the range begins below the total
+    mine = places(b0 + lane);
+    inc = scan(mine);
+    const int all = __shfl_sync(0xffffffffu, inc, 31);
+    if (g.begin < before + all) break;
+    before += all;
   }
-  __syncthreads();
-  return g;
+  start->at = before + inc - mine;
+  return __ffs(__ballot_sync(0xffffffffu, g.begin < before + inc)) - 1;
 }
 
-// Walks the pieces of a CTA's range; one thread uses it.
+// Walks the pieces of a CTA's range; one thread uses it, and the block waits for
+// its first piece, so `next` moves on from a unit only when it is called again.
 template <int kTile, int kRows>
 struct Walk {
   int pos, end;        // place reached, end of the range
@@ -189,66 +185,64 @@ struct Walk {
   __device__ __forceinline__ void start(const TreeParams& p, const Range& g, const Start& s) {
     pos = g.begin;
     end = g.end;
-    head = 0;
     tile = 0;
     if (pos >= end) return;
     request = s.request;
-    unit_at = s.at;
     r = s.r;
     n_tiles = row_tiles<kRows>(p, r);
-    const uint32_t per_head = head_places<kTile, kRows>(p, r);
-    head = static_cast<int>(static_cast<uint32_t>(pos - unit_at) / per_head);
-    unit_at += head * static_cast<int>(per_head);
-    while (true) {
-      tiles = unit_tiles<kTile, kRows>(p, r, tile);
-      if (pos < unit_at + kUnitCost + tiles) break;
-      unit_at += kUnitCost + tiles;
-      ++tile;
+    head = static_cast<int>(static_cast<uint32_t>(pos - s.at) / static_cast<uint32_t>(s.per_head));
+    unit_at = s.at + head * s.per_head;
+    if (n_tiles == 1) {
+      tiles = s.per_head - kUnitCost;
+    } else {
+      while (true) {
+        tiles = unit_tiles<kTile, kRows>(p, r, tile);
+        if (pos < unit_at + kUnitCost + tiles) break;
+        unit_at += kUnitCost + tiles;
+        ++tile;
+      }
     }
   }
 
+  __device__ __forceinline__ void next_unit(const TreeParams& p) {
+    unit_at = pos;
+    if (++tile == n_tiles) {
+      tile = 0;
+      if (++head == p.heads_kv) {
+        head = 0;
+        do {
+          r = load_request(p, ++request);
+          n_tiles = row_tiles<kRows>(p, r);
+        } while (n_tiles == 0);
+      }
+    }
+    tiles = unit_tiles<kTile, kRows>(p, r, tile);
+  }
+
   // the next piece with tiles in it, or false at the range's end
-  __device__ __forceinline__ bool next(const TreeParams& p, const Range& g, Piece* out) {
+  __device__ __forceinline__ bool next(const TreeParams& p, const Range& g, Piece* c) {
     while (pos < end) {
-      const int unit_end = unit_at + kUnitCost + tiles;
-      const int stop = min(unit_end, end);
-      Piece c;
-      c.tile_begin = max(pos - unit_at - kUnitCost, 0);
-      c.tile_end = max(stop - unit_at - kUnitCost, 0);
-      c.request = request;
-      c.head_kv = head;
-      c.row0 = tile * kRows;
-      c.rows = min(kRows, r.tokens * p.group - c.row0);
-      c.first = r.first;
-      c.ctx = r.ctx;
-      c.tokens = r.tokens;
-      c.keys = r.keys;
-      const int cta = 2 * static_cast<int>(blockIdx.x);
-      const bool from_start = c.tile_begin == 0, to_end = c.tile_end == tiles;
-      c.record = from_start ? (to_end ? -1 : cta + 1) : cta;
+      if (pos == unit_at + kUnitCost + tiles) next_unit(p);
+      const int stop = min(unit_at + kUnitCost + tiles, end);
+      const int tb = max(pos - unit_at - kUnitCost, 0), te = max(stop - unit_at - kUnitCost, 0);
+      pos = stop;
+      if (te <= tb) continue;
+      const bool from_start = tb == 0, to_end = te == tiles;
       merges = to_end && !from_start;
       if (merges) merge_c0 = g.owner(unit_at + kUnitCost);
-      pos = stop;
-      if (pos == unit_end) {  // the next unit
-        unit_at = unit_end;
-        if (++tile == n_tiles) {
-          tile = 0;
-          if (++head == p.heads_kv) {
-            head = 0;
-            if (pos < end) {
-              do {
-                r = load_request(p, ++request);
-                n_tiles = row_tiles<kRows>(p, r);
-              } while (n_tiles == 0);
-            }
-          }
-        }
-        if (pos < end) tiles = unit_tiles<kTile, kRows>(p, r, tile);
-      }
-      if (c.tile_end > c.tile_begin) {
-        *out = c;
-        return true;
-      }
+      const int cta = 2 * static_cast<int>(blockIdx.x);
+      c->request = request;
+      c->head_kv = head;
+      c->row0 = tile * kRows;
+      c->rows = min(kRows, r.tokens * p.group - tile * kRows);
+      c->first = r.first;
+      c->ctx = r.ctx;
+      c->tokens = r.tokens;
+      c->keys = r.keys;
+      c->tile_begin = tb;
+      c->tile_end = te;
+      c->record = from_start ? (to_end ? -1 : cta + 1) : cta;
+      return true;
     }
     return false;
   }

@@ -74,9 +74,7 @@ struct SimtCfg {
   static constexpr int kItemOff = kAlphaOff + kSimtWarps * kSimtRows * 4;
   static constexpr int kBarOff = kItemOff + kSimtItems * 48;
   static constexpr int kBars = 2 * kSimtStages + 2 * kSimtItems + 2;
-  static constexpr int kStartOff = kBarOff + kBars * 8;
-  static constexpr int kSumOff = kStartOff + 32;
-  static constexpr int kSmem = kSumOff + 48;
+  static constexpr int kSmem = kBarOff + kBars * 8;
   static_assert(kSmem <= 232448 && kBarOff % 8 == 0, "shared memory");
 };
 
@@ -103,7 +101,6 @@ __global__ void __launch_bounds__(kSimtThreads, 1)
   uint64_t* item_empty = item_full + kSimtItems;
   uint64_t* joined = item_empty + kSimtItems;
   uint64_t* released = joined + 1;
-  Start* s_start = reinterpret_cast<Start*>(smem + C::kStartOff);
   auto item_slot = [&](int w) {
     return reinterpret_cast<Piece*>(smem + C::kItemOff + (w % kSimtItems) * 48);
   };
@@ -132,19 +129,21 @@ __global__ void __launch_bounds__(kSimtThreads, 1)
     fence_barrier_init();
   }
   let_successor_start();
+  __syncthreads();
   wait_for_predecessor();
-  const Range range = find_range<kTile, kSimtRows, kSimtThreads>(
-      p, reinterpret_cast<int*>(smem + C::kSumOff), s_start);
 
   if (warp == kSimtWarps) {
     // -------------------------------------------------------- pieces and loads
-    Walk<kTile, kSimtRows> walk;
     if (lane == 0) {
       tma_prefetch_desc(&tmK);
       tma_prefetch_desc(&tmV);
-      walk.start(p, range, *s_start);
       p.meta[blockIdx.x * kMetaInts] = 0;
     }
+    Range range;
+    Start first;
+    const int walker = find_range<kTile, kSimtRows>(p, &range, &first);
+    Walk<kTile, kSimtRows> walk;
+    if (lane == walker) walk.start(p, range, first);
     const int rows_box = min(p.page_size, kTile);
     const int boxes = kTile / rows_box * (D / 32);
     int n = 0;  // tiles loaded
@@ -155,7 +154,7 @@ __global__ void __launch_bounds__(kSimtThreads, 1)
                                                (w / kSimtItems - 1) & 1, st, kSiteItemQueue, tmo));
       if (!ok) break;
       Piece* slot = item_slot(w);
-      if (lane == 0) {
+      if (lane == walker) {
         Piece c;
         if (walk.next(p, range, &c)) {
           if (walk.merges) write_meta(p, c, true, walk.merge_c0);
@@ -169,15 +168,15 @@ __global__ void __launch_bounds__(kSimtThreads, 1)
       if (lane == 0) mbar_arrive(&item_full[w % kSimtItems]);
       if (c.request < 0) break;
       const int* table = p.table + static_cast<int64_t>(c.request) * p.table_stride;
-      const int last_entry = (c.keys - 1) / p.page_size;
+      const int last_entry = (c.keys - 1) >> p.page_shift;
       for (int tile = c.tile_begin; tile < c.tile_end; ++tile) {
         // this lane's box: page, rows within the tile, 32-column segment
         const int seg = lane % (D / 32), part = lane / (D / 32);
         int page = p.num_pages, token = 0;
         if (lane < boxes) {
           const int key = tile * kTile + part * rows_box;
-          const int entry = key / p.page_size;
-          token = key - entry * p.page_size;
+          const int entry = key >> p.page_shift;
+          token = key & (p.page_size - 1);
           if (entry <= last_entry) {  // behind it: a coordinate past the pool loads zeros
             page = table[entry];
             if (page < 0 || page >= p.num_pages) {

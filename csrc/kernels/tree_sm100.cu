@@ -75,12 +75,10 @@ struct Cfg {
   static constexpr int kBarOff = kQBytes + kStages * kTile;
   static constexpr int kMlOff = kBarOff + kBars * 8;       // float2 [2][128]
   static constexpr int kItemOff = kMlOff + 2 * kM * 8;     // Piece [kItems]
-  static constexpr int kSumOff = kItemOff + kItems * 48;   // int [12]
-  static constexpr int kStartOff = kSumOff + 12 * 4;       // Start
-  static constexpr int kMiscOff = kStartOff + 32;          // int [4]
+  static constexpr int kMiscOff = kItemOff + kItems * 48;  // int [4]
   static constexpr int kSmem = kMiscOff + 16;
-  static_assert(kMlOff % 8 == 0 && kSumOff % 8 == 0 && kSmem <= 232448, "shared memory");
-  static_assert(sizeof(Piece) <= 48 && sizeof(Start) <= 32, "piece");
+  static_assert(kMlOff % 8 == 0 && kMiscOff % 8 == 0 && kSmem <= 232448, "shared memory");
+  static_assert(sizeof(Piece) <= 48, "piece");
 };
 
 template <bool kBF16>
@@ -126,17 +124,19 @@ __device__ __forceinline__ uint32_t seen_bits(const TreeParams& p, const Piece* 
   return n < 32 ? bits & ((1u << n) - 1u) : bits;
 }
 
-// V rows [vr0, vr0 + n_rows) of a tile whose first key is k0, by 128 threads:
-// rows at or past `keys` become zeros, and among the new tokens (from ctx on)
-// what is not finite does; true when this thread took something out.
+// V rows [vr0, vr1) of a tile whose first key is k0, by 128 threads: rows at or
+// past `keys` become zeros (up to the end of the last page: behind it TMA wrote
+// zeros), and among the new tokens (from ctx on) what is not finite does; true when
+// this thread took something out.
 template <int D, bool kBF16>
-__device__ __noinline__ bool clean_v(uint8_t* tile, int k0, int ctx, int keys, int vr0, int n_rows,
-                                     int tid) {
+__device__ __noinline__ bool clean_v(uint8_t* tile, int k0, int ctx, int keys, int page_size,
+                                     int vr0, int vr1, int tid) {
   constexpr int kPerRow = D / 8;
   bool dirty = false;
-  for (int i = tid; i < n_rows * kPerRow; i += 128) {
-    const int vr = vr0 + i / kPerRow, ch = i % kPerRow;
-    if (k0 + vr < ctx) continue;
+  vr0 = max(vr0, ctx - k0);
+  vr1 = min(vr1, ((keys + page_size - 1) & ~(page_size - 1)) - k0);
+  for (int i = vr0 * kPerRow + tid; i < vr1 * kPerRow; i += 128) {
+    const int vr = i / kPerRow, ch = i % kPerRow;
     uint4* at = reinterpret_cast<uint4*>(tile + (ch / 8) * (kN * 128) + vr * 128 + (ch % 8) * 16);
     if (k0 + vr >= keys) {
       *at = make_uint4(0u, 0u, 0u, 0u);
@@ -168,11 +168,11 @@ __device__ __noinline__ void add_taken_out(const TreeParams& p, const Piece* c, 
   for (int key = lo; key < hi; ++key) {
     const int rel = key - c->ctx;
     if (!((seen_bits(p, c, t, rel & ~31) >> (rel & 31)) & 1u)) continue;
-    const int page = table[key / p.page_size];
+    const int page = table[key >> p.page_shift];
     if (page < 0 || page >= p.num_pages) continue;
     const uint16_t* src =
         static_cast<const uint16_t*>(p.v) + page * p.v_page +
-        (static_cast<int64_t>(c->head_kv) * p.page_size + key % p.page_size) * dim;
+        (static_cast<int64_t>(c->head_kv) * p.page_size + (key & (p.page_size - 1))) * dim;
     for (int k = k0; k < k1; ++k) {
       if (!not_finite<kBF16>(src[k])) continue;
       const float v = widen<kBF16>(src[k]);
@@ -212,10 +212,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* item_empty = item_full + kItems;   // [kItems]
   uint64_t* p_hi = item_empty + kItems;        // [2], with two parts
   float2* s_ml = reinterpret_cast<float2*>(smem + C::kMlOff);
-  int* s_sums = reinterpret_cast<int*>(smem + C::kSumOff);
   int* s_misc = reinterpret_cast<int*>(smem + C::kMiscOff);
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_misc);
-  Start* s_start = reinterpret_cast<Start*>(smem + C::kStartOff);
   volatile int* s_dirty = s_misc + 2;  // [2], by the piece's parity
   auto item_slot = [&](int w) {
     return reinterpret_cast<Piece*>(smem + C::kItemOff + (w % kItems) * 48);
@@ -261,11 +259,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 1) {
     tmem_alloc(s_tmem, kCols);
     tmem_relinquish();
+  } else if (warp >= 4) {  // the rows that no query will fill (below, among the queries)
+    for (int i = threadIdx.x - 128; i < C::kQBytes / 16; i += kThreads - 128)
+      reinterpret_cast<uint4*>(sQ)[i] = make_uint4(0u, 0u, 0u, 0u);
+    fence_proxy_async_smem();
   }
   let_successor_start();
-  wait_for_predecessor();
-  const Range range = find_range<kN, kRows, kThreads>(p, s_sums, s_start);
+  __syncthreads();
   tc_fence_after();
+  wait_for_predecessor();
   const uint32_t tmem = *s_tmem;
 
   if (warp < 4) {
@@ -273,13 +275,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 0) {
       // ------------------------------------------------------ pieces and loads
       const int lane = lane_id();
-      Walk<kN, kRows> walk;
       if (lane == 0) {
         tma_prefetch_desc(&tmK);
         tma_prefetch_desc(&tmV);
-        walk.start(p, range, *s_start);
         p.meta[blockIdx.x * kMetaInts] = 0;
       }
+      Range range;
+      Start first;
+      const int walker = find_range<kN, kRows>(p, &range, &first);
+      Walk<kN, kRows> walk;
+      if (lane == walker) walk.start(p, range, first);
       const int rows_box = min(p.page_size, kN);
       const int boxes = kN / rows_box * (D / 64);
       int n = 0;  // loads issued (K and V tiles)
@@ -290,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                                  kSiteItemQueue, tmo));
         if (!ok) break;
         Piece* slot = item_slot(w);
-        if (lane == 0) {
+        if (lane == walker) {
           Piece c;
           if (walk.next(p, range, &c)) {
             if (walk.merges) write_meta(p, c, true, walk.merge_c0);
@@ -304,15 +309,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&item_full[w % kItems]);
         if (c.request < 0) break;
         const int* table = p.table + static_cast<int64_t>(c.request) * p.table_stride;
-        const int last_entry = (c.keys - 1) / p.page_size;
+        const int last_entry = (c.keys - 1) >> p.page_shift;
         for (int tile = c.tile_begin; tile < c.tile_end && ok; ++tile) {
           // this lane's box: page, rows within the tile, 64-column half
           const int half = lane % (D / 64), part = lane / (D / 64);
           int page = p.num_pages, token = 0;
           if (lane < boxes) {
             const int key = tile * kN + part * rows_box;
-            const int entry = key / p.page_size;
-            token = key - entry * p.page_size;
+            const int entry = key >> p.page_shift;
+            token = key & (p.page_size - 1);
             // behind the last key: a page coordinate past the pool loads zeros
             if (entry <= last_entry) {
               page = table[entry];
@@ -454,6 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else {
       // -------------------------------------------------------------- queries
       const int tid = threadIdx.x - 64;
+      int filled = 0;  // rows that hold queries of a piece before
       bool ok = true;
       for (int w = 0; ok; ++w) {
         ok = __all_sync(0xffffffffu, mbar_wait(&item_full[w % kItems], (w / kItems) & 1, st,
@@ -471,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr int kChunks = D / 8;
         const uint32_t qb = smem_u32(sQ);
         const int h0 = c.head_kv * p.group;
-        for (int i = tid; i < kRows * kChunks; i += 64) {
+        for (int i = tid; i < max(c.rows, filled) * kChunks; i += 64) {
           const int r = i / kChunks, x = i % kChunks;
           const uint32_t at = qb + (r / kM) * (kM * D * 2) + (x / 8) * (kM * 128) +
                               (r % kM) * 128 + (((x % 8) ^ (r & 7)) << 4);
@@ -484,6 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 static_cast<int64_t>(c.first + t) * p.q_t + h * p.q_h + x * 8;
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(src) : "memory");
         }
+        filled = c.rows;
         asm volatile("cp.async.wait_all;" ::: "memory");
         fence_proxy_async_smem();
         mbar_arrive(q_full);
@@ -520,18 +527,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m_run = -INFINITY, l_run = 0.f;
       for (int j = kTwoRows ? 0 : x; j < n; j += kTwoRows ? 1 : 2) {
         const bool tail = (j + 1) * kN > old_keys;
-        if (tail) {
-          // clean V: 16 bytes a step; with two row tiles each chain takes half the rows
-          const int idx = 2 * (g0 + j) + 1;
-          ok = __all_sync(0xffffffffu,
-                          mbar_wait(&full[idx % NS], (idx / NS) & 1, st, kSiteVFull, tmo));
-          if (!ok) break;
-          constexpr int kVRows = kTwoRows ? kN / 2 : kN;
-          if (clean_v<D, kBF16>(sKV + (idx % NS) * C::kTile, (c->tile_begin + j) * kN, c->ctx,
-                                c->keys, kTwoRows ? x * kVRows : 0, kVRows, row))
-            s_dirty[w & 1] = w + 1;
-          fence_proxy_async_smem();
-        }
         ok = __all_sync(0xffffffffu, mbar_wait(&s_full[x], sx & 1, st, kSiteSFull, tmo));
         if (!ok) break;
         ++sx;
@@ -606,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               pk[q] = pack2<kBF16>(e.x, e.y);
             }
             tmem_st32(s_col + hlf * 32, pk);
-            if (C::kParts == 2 && hlf == 0) {
+            if (C::kParts == 2 && hlf == 0 && !tail) {
               tmem_st_wait();
               tc_fence_before();
               __syncwarp();
@@ -616,13 +611,27 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float2 sum = fadd2(fadd2(ps[0], ps[1]), fadd2(ps[2], ps[3]));
           l_run += sum.x + sum.y;
           tmem_st_wait();
-        } else if (C::kParts == 2) {
-          __syncwarp();
-          if (lane_id() == 0) mbar_arrive(&p_full[x]);
+        }
+        if (tail) {
+          // Clean V before the weights are handed over, whole: by now it has arrived.
+          // With two row tiles each chain takes half the rows.
+          const int idx = 2 * (g0 + j) + 1;
+          ok = __all_sync(0xffffffffu,
+                          mbar_wait(&full[idx % NS], (idx / NS) & 1, st, kSiteVFull, tmo));
+          if (!ok) break;
+          constexpr int kVRows = kTwoRows ? kN / 2 : kN;
+          if (clean_v<D, kBF16>(sKV + (idx % NS) * C::kTile, (c->tile_begin + j) * kN, c->ctx,
+                                c->keys, p.page_size, kTwoRows ? x * kVRows : 0,
+                                kTwoRows ? (x + 1) * kVRows : kVRows, row))
+            s_dirty[w & 1] = w + 1;
+          fence_proxy_async_smem();
         }
         tc_fence_before();
         __syncwarp();
-        if (lane_id() == 0) mbar_arrive(C::kParts == 2 ? &p_hi[x] : &p_full[x]);
+        if (lane_id() == 0) {
+          if (C::kParts == 1 || tail || !active) mbar_arrive(&p_full[x]);
+          if (C::kParts == 2) mbar_arrive(&p_hi[x]);
+        }
       }
       if (!ok) break;
       // ------------------------------------------------------------ results

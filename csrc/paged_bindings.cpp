@@ -532,6 +532,7 @@ std::tuple<torch::Tensor, OptTensor> tree_attention(torch::Tensor q, torch::Tens
   p.v_page = v_pages.stride(0);
   p.num_pages = static_cast<int>(k_pages.size(0));
   p.page_size = static_cast<int>(page);
+  while ((1 << p.page_shift) < p.page_size) ++p.page_shift;
   p.table = static_cast<const int*>(table.data_ptr());
   p.table_stride = table.stride(0);
   p.table_w = static_cast<int>(table.size(1));
