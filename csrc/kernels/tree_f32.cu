@@ -1,6 +1,5 @@
-// tree_simt.cu - attention of new tokens over a paged cache on the CUDA cores
-// (fp32), the merge of split units for every element type, and the masks of
-// drafted trees.
+// tree_f32.cu - attention of new tokens over a paged cache in fp32, the merge of
+// split units for every element type, and the masks of drafted trees.
 //
 // Row (token t, head h) of a request with ctx cached tokens sees key j when
 // j < ctx, or when j is new token j - ctx and the mask has that bit (without a
@@ -10,15 +9,22 @@
 // gives 0 and lse = -inf.
 //
 // One CTA per SM takes its even share of the work (tree_sched.cuh), 8 rows of a kv
-// head at a time: at 8 rows the 2 x 8 x dim products of a key take the CUDA cores
-// about half the time its 8 x dim bytes take from memory, so a decoding step stays
-// bound by reading the cache (more rows read it again, from L2 where it fits).
+// head at a time: the width of a small tensor-core product, whose other side is
+// keys (scores) or columns of V (outputs), so a decoding step reads the cache once
+// at fp32-level accuracy and stays bound by that (more rows read it again, from L2
+// where it fits).  Products are 3xTF32: x = hi + lo, hi rounded to 11 bits, and
+// hi*hi + lo*hi + hi*lo; what is left out is 2^-22 of a product.
+//
 // Warp 8 walks the pieces and brings tiles of 64 KB (K and V of 128 keys at dim 64,
 // 64 keys at dim 128) by TMA into a ring of three.  Warps 0-7 take an eighth of a
-// tile's keys each: lanes are keys while scores form (the 128-byte swizzle spreads
-// eight keys' words over all banks), then columns for the product with V.  Every
-// warp keeps its own running maximum, sum and 8 x dim outputs in registers; they
-// are joined once per piece.
+// tile's keys each, with their own running maximum, sum and outputs in registers,
+// joined once per piece.  Inside a product the order of the summed index is free:
+// it is chosen so that every read of K, V and the weights is 8 or 16 bytes wide and
+// the lanes of one pass meet different banks.
+//
+// 3 trees over 4096 to 16384 keys, 8 heads x 64 (126 MB, 19 us at the copy rate): 32
+// us with the merge, against 39 us with the products on the CUDA cores, which issue
+// three times the instructions.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -37,11 +43,11 @@ using namespace tree_detail;
 
 namespace {
 
-constexpr int kSimtThreads = 288;
-constexpr int kSimtRows = 8;
-constexpr int kSimtWarps = 8;   // that compute
-constexpr int kSimtStages = 3;
-constexpr int kSimtItems = 4;   // queue of pieces
+constexpr int kF32Threads = 288;
+constexpr int kF32Rows = 8;
+constexpr int kF32Warps = 8;   // that compute
+constexpr int kF32Stages = 3;
+constexpr int kF32Items = 4;   // queue of pieces
 constexpr float kLn2f = 0.69314718055994530942f;
 
 template <typename T>
@@ -60,21 +66,20 @@ __device__ __forceinline__ __half cast_out<__half>(float x) {
 }
 
 template <int D>
-struct SimtCfg {
-  static constexpr int kTile = 8192 / D;       // keys: 32 KB of K
-  static constexpr int kKeys = kTile / kSimtWarps;  // of a warp: 16 or 8
-  static constexpr int kGroups = 32 / kKeys;   // groups of lanes, each with its rows
-  static constexpr int kGroupRows = kSimtRows / kGroups;
+struct F32Cfg {
+  static constexpr int kTile = 8192 / D;           // keys: 32 KB of K
+  static constexpr int kKeys = kTile / kF32Warps;  // of a warp: 16, or 8 (half a product's height)
   static constexpr int kHalf = kTile * D * 4;  // bytes of K (or V) of a tile
   static constexpr int kStage = 2 * kHalf;
-  static constexpr int kOwn = kSimtRows * D;   // floats of a warp: its queries, then its outputs
-  static constexpr int kPOff = kSimtStages * kStage + kSimtWarps * kOwn * 4;
-  static constexpr int kPBytes = kSimtRows * kKeys * 4;  // of a warp: weights; at a piece's end float2 [rows]
-  static constexpr int kAlphaOff = kPOff + kSimtWarps * kPBytes;
-  static constexpr int kItemOff = kAlphaOff + kSimtWarps * kSimtRows * 4;
-  static constexpr int kBarOff = kItemOff + kSimtItems * 48;
-  static constexpr int kBars = 2 * kSimtStages + 2 * kSimtItems + 2;
-  static constexpr int kSmem = kBarOff + kBars * 8;
+  // floats of a warp: weights [row][key] in the tiles, [row][dim] outputs at a piece's end
+  static constexpr int kOwn = kF32Rows * D;
+  static constexpr int kPRow = kKeys + 4;  // between the weights of two rows
+  static constexpr int kMlOff = kF32Stages * kStage + kF32Warps * kOwn * 4;  // float2 [warps][rows]
+  static constexpr int kItemOff = kMlOff + kF32Warps * kF32Rows * 8;
+  static constexpr int kBarOff = kItemOff + kF32Items * 48;
+  static constexpr int kBars = 2 * kF32Stages + 2 * kF32Items + 2;
+  static constexpr int kDirtyOff = kBarOff + kBars * 8;  // int [2]
+  static constexpr int kSmem = kDirtyOff + 8;
   static_assert(kSmem <= 232448 && kBarOff % 8 == 0, "shared memory");
 };
 
@@ -82,27 +87,83 @@ struct SimtCfg {
 // 16-byte chunks swizzled by the row within 128 bytes
 template <int D>
 __device__ __forceinline__ int tile_at(int key, int col) {
-  return (col >> 5) * (SimtCfg<D>::kTile * 128) + key * 128 + ((((col >> 2) & 7) ^ (key & 7)) << 4) +
+  return (col >> 5) * (F32Cfg<D>::kTile * 128) + key * 128 + ((((col >> 2) & 7) ^ (key & 7)) << 4) +
          (col & 3) * 4;
 }
 
+// x = hi + lo for a 3xTF32 product, hi the nearest of 11 bits: rounded, lo has either
+// sign, and the product lo * lo that is left out does not add up (cut off, it is
+// always positive: the results here were off by 2.3e-6 instead of 2.8e-7).  lo of an
+// infinity is kept finite, so that it stays an infinity.
+__device__ __forceinline__ void split3x(float x, float& hi, float& lo) {
+  const float top = __uint_as_float(sm100::f32_to_tf32(x));
+  lo = fmaxf(x - top, -3.0e38f);
+  hi = top;
+}
+
+// c += a * b, one 16 x 8 x 8 product of 11-bit operands
+__device__ __forceinline__ void mma_tf32(float* c, const float* a, const float* b) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(__float_as_uint(a[0])), "r"(__float_as_uint(a[1])), "r"(__float_as_uint(a[2])),
+        "r"(__float_as_uint(a[3])), "r"(__float_as_uint(b[0])), "r"(__float_as_uint(b[1])));
+}
+
+// c + c_lo += a * b at fp32 level.  The tensor core cuts its sums off instead of
+// rounding them, so c is a short sum (a tile's), added up in fp32 outside.
+__device__ __forceinline__ void mma_3x(float* c, float* c_lo, const float* a, const float* a_lo,
+                                       const float* b, const float* b_lo) {
+  mma_tf32(c_lo, a_lo, b);
+  mma_tf32(c_lo, a, b_lo);
+  mma_tf32(c, a, b);
+}
+
+// Columns [k0, k1) of a result that this thread has just written take what was left
+// out of V among the new tokens of the piece, for the keys that token t sees.
+__device__ __noinline__ void add_left_out(const TreeParams& p, const Piece& c, int t, int tile, int k0,
+                                          int k1, int dim, float* rec, float* dst) {
+  const int* table = p.table + static_cast<int64_t>(c.request) * p.table_stride;
+  const int lo = max(c.ctx, c.tile_begin * tile), hi = min(c.keys, c.tile_end * tile);
+  for (int key = lo; key < hi; ++key) {
+    const int rel = key - c.ctx;
+    const bool sees =
+        p.mask == nullptr
+            ? rel <= t
+            : (rel >> 5) < p.mask_w &&
+                  ((p.mask[static_cast<int64_t>(c.first + t) * p.mask_stride + (rel >> 5)] >>
+                    (rel & 31)) &
+                   1u);
+    const int page = table[key >> p.page_shift];
+    if (!sees || page < 0 || page >= p.num_pages) continue;
+    const float* src = static_cast<const float*>(p.v) + page * p.v_page +
+                       (static_cast<int64_t>(c.head_kv) * p.page_size + (key & (p.page_size - 1))) * dim;
+    for (int k = k0; k < k1; ++k) {
+      if (isfinite(src[k])) continue;
+      if (rec != nullptr) rec[(k & ~3) * c.rows + (k & 3)] += src[k];
+      else dst[k] += src[k];
+    }
+  }
+}
+
 template <int D>
-__global__ void __launch_bounds__(kSimtThreads, 1)
-    tree_simt_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap tmK,
+__global__ void __launch_bounds__(kF32Threads, 1)
+    tree_f32_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap tmK,
                      const __grid_constant__ CUtensorMap tmV) {
-  using C = SimtCfg<D>;
+  using C = F32Cfg<D>;
   using namespace sm100;
-  constexpr int kTile = C::kTile, kKeys = C::kKeys, kGR = C::kGroupRows;
-  constexpr int kCols = D / 32;
+  constexpr int kTile = C::kTile, kKeys = C::kKeys;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
-  uint64_t* empty = full + kSimtStages;
-  uint64_t* item_full = empty + kSimtStages;
-  uint64_t* item_empty = item_full + kSimtItems;
-  uint64_t* joined = item_empty + kSimtItems;
+  uint64_t* empty = full + kF32Stages;
+  uint64_t* item_full = empty + kF32Stages;
+  uint64_t* item_empty = item_full + kF32Items;
+  uint64_t* joined = item_empty + kF32Items;
   uint64_t* released = joined + 1;
+  volatile int* s_dirty = reinterpret_cast<int*>(smem + C::kDirtyOff);  // [2], by the piece's parity
   auto item_slot = [&](int w) {
-    return reinterpret_cast<Piece*>(smem + C::kItemOff + (w % kSimtItems) * 48);
+    return reinterpret_cast<Piece*>(smem + C::kItemOff + (w % kF32Items) * 48);
   };
   const int warp = warp_id(), lane = lane_id();
   DeviceStatus* st = p.status;
@@ -116,23 +177,24 @@ __global__ void __launch_bounds__(kSimtThreads, 1)
     return;
   }
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kSimtStages; ++i) {
+    for (int i = 0; i < kF32Stages; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], kSimtWarps);
+      mbar_init(&empty[i], kF32Warps);
     }
-    for (int i = 0; i < kSimtItems; ++i) {
+    for (int i = 0; i < kF32Items; ++i) {
       mbar_init(&item_full[i], 1);
-      mbar_init(&item_empty[i], kSimtWarps);
+      mbar_init(&item_empty[i], kF32Warps);
     }
-    mbar_init(joined, kSimtWarps);
-    mbar_init(released, kSimtWarps);
+    mbar_init(joined, kF32Warps);
+    mbar_init(released, kF32Warps);
+    s_dirty[0] = s_dirty[1] = 0;
     fence_barrier_init();
   }
   let_successor_start();
   __syncthreads();
   wait_for_predecessor();
 
-  if (warp == kSimtWarps) {
+  if (warp == kF32Warps) {
     // -------------------------------------------------------- pieces and loads
     if (lane == 0) {
       tma_prefetch_desc(&tmK);
@@ -141,17 +203,17 @@ __global__ void __launch_bounds__(kSimtThreads, 1)
     }
     Range range;
     Start first;
-    const int walker = find_range<kTile, kSimtRows>(p, &range, &first);
-    Walk<kTile, kSimtRows> walk;
+    const int walker = find_range<kTile, kF32Rows>(p, &range, &first);
+    Walk<kTile, kF32Rows> walk;
     if (lane == walker) walk.start(p, range, first);
     const int rows_box = min(p.page_size, kTile);
     const int boxes = kTile / rows_box * (D / 32);
     int n = 0;  // tiles loaded
     bool ok = true;
     for (int w = 0; ok; ++w) {
-      if (w >= kSimtItems)
-        ok = __all_sync(0xffffffffu, mbar_wait(&item_empty[w % kSimtItems],
-                                               (w / kSimtItems - 1) & 1, st, kSiteItemQueue, tmo));
+      if (w >= kF32Items)
+        ok = __all_sync(0xffffffffu, mbar_wait(&item_empty[w % kF32Items],
+                                               (w / kF32Items - 1) & 1, st, kSiteItemQueue, tmo));
       if (!ok) break;
       Piece* slot = item_slot(w);
       if (lane == walker) {
@@ -165,7 +227,7 @@ __global__ void __launch_bounds__(kSimtThreads, 1)
       }
       __syncwarp();
       const Piece c = *slot;
-      if (lane == 0) mbar_arrive(&item_full[w % kSimtItems]);
+      if (lane == 0) mbar_arrive(&item_full[w % kF32Items]);
       if (c.request < 0) break;
       const int* table = p.table + static_cast<int64_t>(c.request) * p.table_stride;
       const int last_entry = (c.keys - 1) >> p.page_shift;
@@ -185,8 +247,8 @@ __global__ void __launch_bounds__(kSimtThreads, 1)
             }
           }
         }
-        const int stage = n % kSimtStages;
-        ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], ((n / kSimtStages) & 1) ^ 1, st,
+        const int stage = n % kF32Stages;
+        ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], ((n / kF32Stages) & 1) ^ 1, st,
                                                kSiteKEmpty, tmo));
         if (!ok) break;
         if (lane == 0) mbar_arrive_expect_tx(&full[stage], C::kStage);
@@ -200,190 +262,259 @@ __global__ void __launch_bounds__(kSimtThreads, 1)
       }
     }
     // the loads in flight land before the block gives its memory back
-    for (int i = 0; i < kSimtStages && i < n; ++i) {
+    for (int i = 0; i < kF32Stages && i < n; ++i) {
       const int k = n - 1 - i;
-      mbar_wait(&full[k % kSimtStages], (k / kSimtStages) & 1, nullptr, kSiteKFull, 100000000ull);
+      mbar_wait(&full[k % kF32Stages], (k / kF32Stages) & 1, nullptr, kSiteKFull, 100000000ull);
     }
     return;
   }
 
   // ------------------------------------------------------------------ arithmetic
-  float* own = reinterpret_cast<float*>(smem + kSimtStages * C::kStage) + warp * C::kOwn;
-  float* s_p = reinterpret_cast<float*>(smem + C::kPOff) + warp * kSimtRows * kKeys;
+  // Fragments of a 16 x 8 x 8 product: lane = 4 g + t.  Scores: rows are keys, columns
+  // query rows, the summed index is dim; this lane's sums are keys g and g + 8 (of the
+  // warp's, in the order key_of) of query rows 2t and 2t + 1.  Outputs: rows are columns
+  // of V, the summed index is keys; this lane's are dims 32 h + 4 g + 0..3 of query rows
+  // 2t and 2t + 1.
+  float* own = reinterpret_cast<float*>(smem + kF32Stages * C::kStage) + warp * C::kOwn;
+  float* s_p = own;
   auto s_ml = [&](int u, int r) -> float2& {  // maximum and sum of warp u's row r
-    return reinterpret_cast<float2*>(smem + C::kPOff + u * C::kPBytes)[r];
+    return reinterpret_cast<float2*>(smem + C::kMlOff)[u * kF32Rows + r];
   };
-  float* s_alpha = reinterpret_cast<float*>(smem + C::kAlphaOff) + warp * kSimtRows;
-  const int key = lane % kKeys, row0 = lane / kKeys * kGR;  // this lane's key and first row
-  const int turn = lane / kKeys * 4;
+  const int g = lane >> 2, t = lane & 3;
+  // rows g and g + 1 of one pass lie four keys apart: their swizzled words meet no bank twice
+  const int key_g = (g >> 1) + 4 * (g & 1);
   int n = 0;  // tiles taken
   bool ok = true;
   for (int w = 0; ok; ++w) {
-    ok = __all_sync(0xffffffffu, mbar_wait(&item_full[w % kSimtItems], (w / kSimtItems) & 1, st,
+    ok = __all_sync(0xffffffffu, mbar_wait(&item_full[w % kF32Items], (w / kF32Items) & 1, st,
                                            kSiteItemQueue, tmo));
     if (!ok) break;
     const Piece c = *item_slot(w);
     if (c.request < 0) break;
-    // the piece before has been read out of every warp's outputs
-    if (w > 0)
-      ok = __all_sync(0xffffffffu, mbar_wait(released, (w - 1) & 1, st, kSiteOReady, tmo));
-    if (!ok) break;
-    // queries, scaled to base-2 exponents; a copy for each warp
-    for (int i = lane; i < kSimtRows * (D / 4); i += 32) {
-      const int r = i / (D / 4), x = (i % (D / 4)) * 4;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (r < c.rows) {
-        const int row = c.row0 + r, t = row / p.group, h = c.head_kv * p.group + row - t * p.group;
-        v = *reinterpret_cast<const float4*>(static_cast<const float*>(p.q) +
-                                             static_cast<int64_t>(c.first + t) * p.q_t +
-                                             static_cast<int64_t>(h) * p.q_h + x);
-        v.x *= p.scale_log2;
-        v.y *= p.scale_log2;
-        v.z *= p.scale_log2;
-        v.w *= p.scale_log2;
+    // queries of row g, scaled to base-2 exponents; dim 16 b + 4 t + 0..3 is summed at
+    // places t, t + 4 of step 2 b and t, t + 4 of step 2 b + 1
+    float q_hi[D / 8][2], q_lo[D / 8][2];
+    {
+      const int row = c.row0 + min(g, c.rows - 1), tok = row / p.group;
+      const int h = c.head_kv * p.group + row - tok * p.group;
+      const float* src = static_cast<const float*>(p.q) +
+                         static_cast<int64_t>(c.first + tok) * p.q_t +
+                         static_cast<int64_t>(h) * p.q_h + 4 * t;
+#pragma unroll
+      for (int b = 0; b < D / 16; ++b) {
+        const float4 v = *reinterpret_cast<const float4*>(src + 16 * b);
+        q_hi[2 * b][0] = v.x * p.scale_log2;
+        q_hi[2 * b][1] = v.y * p.scale_log2;
+        q_hi[2 * b + 1][0] = v.z * p.scale_log2;
+        q_hi[2 * b + 1][1] = v.w * p.scale_log2;
       }
-      // the groups of lanes read different rows at once: from different banks
-      *reinterpret_cast<float4*>(own + r * D + (x ^ (r / kGR * 4))) = v;
+#pragma unroll
+      for (int b = 0; b < D / 8; ++b)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) split3x(q_hi[b][i], q_hi[b][i], q_lo[b][i]);
     }
-    __syncwarp();
-    float acc[kSimtRows][kCols];
+    if (w > 0) {  // the piece before has been read out of every warp's outputs
+      ok = __all_sync(0xffffffffu, mbar_wait(released, (w - 1) & 1, st, kSiteOReady, tmo));
+      if (!ok) break;
+    }
+    float acc[D / 16][4];  // [4 h + i]: dims 64 h + 32 e + 4 g + i of rows 2t + r at 2 e + r
 #pragma unroll
-    for (int r = 0; r < kSimtRows; ++r)
+    for (int b = 0; b < D / 16; ++b)
 #pragma unroll
-      for (int x = 0; x < kCols; ++x) acc[r][x] = 0.f;
-    float m[kGR], l[kGR];  // rows row0 + i; l is this lane's share
-#pragma unroll
-    for (int i = 0; i < kGR; ++i) m[i] = -INFINITY, l[i] = 0.f;
+      for (int i = 0; i < 4; ++i) acc[b][i] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // rows 2t + i; l is this lane's share
+    bool dirty = false;
 
     for (int tile = c.tile_begin; tile < c.tile_end; ++tile, ++n) {
-      const int stage = n % kSimtStages;
-      ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], (n / kSimtStages) & 1, st, kSiteKFull,
+      const int stage = n % kF32Stages;
+      ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], (n / kF32Stages) & 1, st, kSiteKFull,
                                              tmo));
       if (!ok) break;
       const uint8_t* sk = smem + stage * C::kStage;
       const uint8_t* sv = sk + C::kHalf;
-      const int k_in = warp * kKeys + key;  // within the tile
-      float s[kGR];
+      // even and odd steps are summed apart, so that products do not wait for one
+      // another, and so are the small products (below)
+      float s2[2][4] = {}, s_lo[4] = {};
 #pragma unroll
-      for (int i = 0; i < kGR; ++i) s[i] = 0.f;
-#pragma unroll 8
-      for (int x = 0; x < D; x += 4) {
-        const float4 kv = *reinterpret_cast<const float4*>(sk + tile_at<D>(k_in, x));
+      for (int b = 0; b < D / 16; ++b) {
+        float k_hi[2][4], k_lo[2][4];  // of the steps 2 b and 2 b + 1
 #pragma unroll
-        for (int i = 0; i < kGR; ++i) {
-          const float4 qv = *reinterpret_cast<const float4*>(own + (row0 + i) * D + (x ^ turn));
-          s[i] = fmaf(qv.x, kv.x, s[i]);
-          s[i] = fmaf(qv.y, kv.y, s[i]);
-          s[i] = fmaf(qv.z, kv.z, s[i]);
-          s[i] = fmaf(qv.w, kv.w, s[i]);
+        for (int hlf = 0; hlf < 2; ++hlf) {
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (hlf == 0 || kKeys == 16)  // with eight keys the lower rows stay empty
+            v = *reinterpret_cast<const float4*>(
+                sk + tile_at<D>(warp * kKeys + key_g + 8 * hlf, 16 * b + 4 * t));
+          k_hi[0][hlf] = v.x;
+          k_hi[0][2 + hlf] = v.y;
+          k_hi[1][hlf] = v.z;
+          k_hi[1][2 + hlf] = v.w;
         }
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) split3x(k_hi[e][i], k_hi[e][i], k_lo[e][i]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          mma_3x(s2[e], s_lo, k_hi[e], k_lo[e], q_hi[2 * b + e], q_lo[2 * b + e]);
       }
-      const int j = tile * kTile + k_in;
+      constexpr int kMine = kKeys / 8;  // keys of this lane
+      float s[kMine][2];
+#pragma unroll
+      for (int u = 0; u < kMine; ++u)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          s[u][i] = s2[0][2 * u + i] + s2[1][2 * u + i] + s_lo[2 * u + i];
+      const int j0 = tile * kTile + warp * kKeys;
       const bool tail = (tile + 1) * kTile > c.ctx;  // new tokens, or past the end
-      if (tail && j >= c.ctx) {
-        const int rel = j - c.ctx;
+      if (tail) {
 #pragma unroll
-        for (int i = 0; i < kGR; ++i) {
-          bool sees = j < c.keys && row0 + i < c.rows;
-          if (sees) {
-            const int t = (c.row0 + row0 + i) / p.group;
-            sees = p.mask == nullptr
-                       ? rel <= t
-                       : (rel >> 5) < p.mask_w &&
-                             ((p.mask[static_cast<int64_t>(c.first + t) * p.mask_stride +
-                                      (rel >> 5)] >>
-                               (rel & 31)) &
-                              1u);
+        for (int u = 0; u < kMine; ++u) {
+          const int j = j0 + key_g + 8 * u, rel = j - c.ctx;
+          if (rel < 0) continue;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int r = 2 * t + i;
+            bool sees = j < c.keys && r < c.rows;
+            if (sees) {
+              const int tok = (c.row0 + r) / p.group;
+              sees = p.mask == nullptr
+                         ? rel <= tok
+                         : (rel >> 5) < p.mask_w &&
+                               ((p.mask[static_cast<int64_t>(c.first + tok) * p.mask_stride +
+                                        (rel >> 5)] >>
+                                 (rel & 31)) &
+                                1u);
+            }
+            if (!sees) s[u][i] = -INFINITY;
           }
-          if (!sees) s[i] = -INFINITY;
         }
       }
+      float alpha[2];
 #pragma unroll
-      for (int i = 0; i < kGR; ++i) {
-        float mx = s[i];
+      for (int i = 0; i < 2; ++i) {
+        float mx = s[0][i];
+        if constexpr (kMine == 2) mx = fmaxf(mx, s[1][i]);
 #pragma unroll
-        for (int d = kKeys / 2; d >= 1; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+        for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
         const float mn = fmaxf(m[i], mx);
         const float use = mn == -INFINITY ? 0.f : mn;
-        const float alpha = ex2_approx(m[i] - use);  // m = -inf: 0
+        alpha[i] = ex2_approx(m[i] - use);  // m = -inf: 0
         m[i] = mn;
-        const float e = ex2_approx(s[i] - use);
-        l[i] = l[i] * alpha + e;
-        s_p[(row0 + i) * kKeys + key] = e;
-        if (key == 0) s_alpha[row0 + i] = alpha;
+        l[i] *= alpha[i];
+#pragma unroll
+        for (int u = 0; u < kMine; ++u) {
+          const float e = ex2_approx(s[u][i] - use);
+          l[i] += e;
+          s_p[(2 * t + i) * C::kPRow + key_g + 8 * u] = e;
+        }
       }
       __syncwarp();
+      float part[D / 16][4];  // this tile's, laid out as acc
 #pragma unroll
-      for (int r = 0; r < kSimtRows; ++r) {
-        const float a = s_alpha[r];
+      for (int b = 0; b < D / 16; ++b)
 #pragma unroll
-        for (int x = 0; x < kCols; ++x) acc[r][x] *= a;
-      }
+        for (int i = 0; i < 4; ++i) part[b][i] = 0.f;
 #pragma unroll
-      for (int k4 = 0; k4 < kKeys; k4 += 4) {
-        float v[4][kCols];
+      for (int step = 0; step < kKeys / 8; ++step) {
+        // keys 8 step + 2t and + 1 are summed at places t and t + 4
+        const float2 w2 =
+            *reinterpret_cast<const float2*>(s_p + g * C::kPRow + 8 * step + 2 * t);
+        float w_hi[2], w_lo[2];
+        split3x(w2.x, w_hi[0], w_lo[0]);
+        split3x(w2.y, w_hi[1], w_lo[1]);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const uint8_t* at = sv + tile_at<D>(warp * kKeys + k4 + u, lane * kCols);
-          if constexpr (kCols == 4)
-            *reinterpret_cast<float4*>(v[u]) = *reinterpret_cast<const float4*>(at);
-          else
-            *reinterpret_cast<float2*>(v[u]) = *reinterpret_cast<const float2*>(at);
-        }
+        for (int h = 0; h < D / 64; ++h) {
+          float v[2][2][4];  // [key][columns 64 h + 32 e + 4 g ..]
 #pragma unroll
-        for (int r = 0; r < kSimtRows; ++r) {
-          const float4 pr = *reinterpret_cast<const float4*>(s_p + r * kKeys + k4);
-          const float pv[4] = {pr.x, pr.y, pr.z, pr.w};
+          for (int u = 0; u < 2; ++u) {
+            const int k = warp * kKeys + 8 * step + 2 * t + u;
 #pragma unroll
-          for (int u = 0; u < 4; ++u)
+            for (int e = 0; e < 2; ++e)
+              *reinterpret_cast<float4*>(v[u][e]) =
+                  *reinterpret_cast<const float4*>(sv + tile_at<D>(k, 64 * h + 32 * e + 4 * g));
+            if (tail) {
+              // rows past the end count for nothing, whatever they hold; what is not
+              // finite among the new tokens is left out here and added at the end
+              const int rel = tile * kTile + k - c.ctx;
+              if (rel >= 0) {
+                const bool past = tile * kTile + k >= c.keys;
 #pragma unroll
-            for (int x = 0; x < kCols; ++x) {
-              // among the new tokens a row does not take what it does not see: not even a NaN
-              if (!tail || pv[u] != 0.f) acc[r][x] = fmaf(pv[u], v[u][x], acc[r][x]);
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) {
+                    dirty |= !past && !isfinite(v[u][e][i]);
+                    if (past || !isfinite(v[u][e][i])) v[u][e][i] = 0.f;
+                  }
+              }
             }
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float a[4], a_lo[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) split3x(v[x >> 1][x & 1][i], a[x], a_lo[x]);
+            mma_3x(part[4 * h + i], part[4 * h + i], a, a_lo, w_hi, w_lo);
+          }
         }
       }
       __syncwarp();  // s_p and the stage have been read
       if (lane == 0) mbar_arrive(&empty[stage]);
+#pragma unroll
+      for (int b = 0; b < D / 16; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[b][i] = fmaf(acc[b][i], alpha[i & 1], part[b][i]);
     }
     if (!ok) break;
 
-    // join the warps: outputs over the queries, which are no longer needed
+    // join the warps
+    if (dirty) s_dirty[w & 1] = w + 1;
 #pragma unroll
-    for (int i = 0; i < kGR; ++i) {
+    for (int i = 0; i < 2; ++i) {
 #pragma unroll
-      for (int d = kKeys / 2; d >= 1; d >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], d);
-      if (key == 0) s_ml(warp, row0 + i) = make_float2(m[i], l[i]);
+      for (int d = 4; d < 32; d <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], d);
+      if (g == 0) s_ml(warp, 2 * t + i) = make_float2(m[i], l[i]);
     }
 #pragma unroll
-    for (int r = 0; r < kSimtRows; ++r)
+    for (int h = 0; h < D / 64; ++h)
 #pragma unroll
-      for (int x = 0; x < kCols; ++x) own[r * D + lane * kCols + x] = acc[r][x];
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          *reinterpret_cast<float4*>(own + (2 * t + i) * D + 64 * h + 32 * e + 4 * g) =
+              make_float4(acc[4 * h][2 * e + i], acc[4 * h + 1][2 * e + i],
+                          acc[4 * h + 2][2 * e + i], acc[4 * h + 3][2 * e + i]);
     __syncwarp();
     if (lane == 0) mbar_arrive(joined);
     ok = __all_sync(0xffffffffu, mbar_wait(joined, w & 1, st, kSiteOReady, tmo));
     if (!ok) break;
-    const float* all = reinterpret_cast<const float*>(smem + kSimtStages * C::kStage);
+    const float* all = reinterpret_cast<const float*>(smem + kF32Stages * C::kStage);
     // row `warp` of the eight, four columns at a time
     if (warp < c.rows) {
       const int r = warp;
       float top = -INFINITY;
 #pragma unroll
-      for (int u = 0; u < kSimtWarps; ++u) top = fmaxf(top, s_ml(u, r).x);
+      for (int u = 0; u < kF32Warps; ++u) top = fmaxf(top, s_ml(u, r).x);
       const float use = top == -INFINITY ? 0.f : top;
-      float sum = 0.f, f[kSimtWarps];
+      float sum = 0.f, f[kF32Warps];
 #pragma unroll
-      for (int u = 0; u < kSimtWarps; ++u) {
+      for (int u = 0; u < kF32Warps; ++u) {
         const float2 ml = s_ml(u, r);
         f[u] = ex2_approx(ml.x - use);
         sum += f[u] * ml.y;
       }
-      const int row = c.row0 + r, t = row / p.group, h = c.head_kv * p.group + row - t * p.group;
+      const int row = c.row0 + r, tok = row / p.group;
+      const int h = c.head_kv * p.group + row - tok * p.group;
       const float inv = c.record >= 0 ? 1.f : (sum == 0.f ? 0.f : 1.f / sum);
+      // a record is [dim / 4][rows][4], the rows of the unit side by side
+      float* rec = c.record >= 0
+                       ? p.rec_acc + static_cast<int64_t>(c.record) * (kF32Rows * D) + r * 4
+                       : nullptr;
+      float* out = static_cast<float*>(p.out) + static_cast<int64_t>(c.first + tok) * p.out_t +
+                   static_cast<int64_t>(h) * p.out_h;
       if (lane < D / 4) {
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int u = 0; u < kSimtWarps; ++u) {
+        for (int u = 0; u < kF32Warps; ++u) {
           const float4 a = *reinterpret_cast<const float4*>(all + u * C::kOwn + r * D + lane * 4);
           o.x += f[u] * a.x;
           o.y += f[u] * a.y;
@@ -391,20 +522,16 @@ __global__ void __launch_bounds__(kSimtThreads, 1)
           o.w += f[u] * a.w;
         }
         o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-        // a record is [dim / 4][rows][4], the rows of the unit side by side
-        float* dst = c.record >= 0
-                         ? p.rec_acc + static_cast<int64_t>(c.record) * (kSimtRows * D) +
-                               (lane * c.rows + r) * 4
-                         : static_cast<float*>(p.out) + static_cast<int64_t>(c.first + t) * p.out_t +
-                               static_cast<int64_t>(h) * p.out_h + lane * 4;
-        *reinterpret_cast<float4*>(dst) = o;
+        *reinterpret_cast<float4*>(rec != nullptr ? rec + lane * 4 * c.rows : out + lane * 4) = o;
+        if (s_dirty[w & 1] == w + 1)
+          add_left_out(p, c, tok, kTile, lane * 4, lane * 4 + 4, D, rec, out);
       }
       if (lane == 0) {
         if (c.record >= 0) {
-          p.rec_m[c.record * kSimtRows + r] = top;
-          p.rec_l[c.record * kSimtRows + r] = sum;
+          p.rec_m[c.record * kF32Rows + r] = top;
+          p.rec_l[c.record * kF32Rows + r] = sum;
         } else if (p.lse != nullptr) {
-          p.lse[static_cast<int64_t>(c.first + t) * p.heads + h] =
+          p.lse[static_cast<int64_t>(c.first + tok) * p.heads + h] =
               sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2f;
         }
       }
@@ -412,7 +539,7 @@ __global__ void __launch_bounds__(kSimtThreads, 1)
     __syncwarp();
     if (lane == 0) {
       mbar_arrive(released);
-      mbar_arrive(&item_empty[w % kSimtItems]);
+      mbar_arrive(&item_empty[w % kF32Items]);
     }
   }
 }
@@ -515,14 +642,14 @@ __global__ void __launch_bounds__(kMergeThreads, 4)
 }
 
 template <int D>
-int run_simt(const TreeParams& p, cudaStream_t stream) {
-  using C = SimtCfg<D>;
+int run_f32(const TreeParams& p, cudaStream_t stream) {
+  using C = F32Cfg<D>;
   static bool done[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !done[dev]) {
     const cudaError_t err = cudaFuncSetAttribute(
-        tree_simt_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+        tree_f32_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
     if (err != cudaSuccess) return static_cast<int>(err);
     if (dev >= 0 && dev < 64) done[dev] = true;
   }
@@ -536,7 +663,7 @@ int run_simt(const TreeParams& p, cudaStream_t stream) {
     return make_tmap(base, TmapDtype::kF32, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
   };
   const CUtensorMap k = pool_map(p.k, p.k_page), v = pool_map(p.v, p.v_page);
-  return launch_overlapped(tree_simt_kernel<D>, dim3(p.grid), kSimtThreads, C::kSmem, stream, &p,
+  return launch_overlapped(tree_f32_kernel<D>, dim3(p.grid), kF32Threads, C::kSmem, stream, &p,
                            &k, &v);
 }
 
@@ -605,7 +732,7 @@ __global__ void pack_mask_kernel(const uint8_t* in, int64_t in_t, int total, int
 TreePlan tree_plan(Elem elem, const TreeParams& p, int max_q, int sms) {
   TreePlan plan;
   if (elem == Elem::kF32) {
-    plan.rows_per_unit = kSimtRows;
+    plan.rows_per_unit = kF32Rows;
   } else {
     // one row tile keeps two key tiles in the air per CTA and suits what reading
     // the cache bounds; from the second row tile on, both share every key tile
@@ -626,7 +753,7 @@ int tree_launch(Elem elem, const TreeParams& p, const TreePlan& plan, cudaStream
   const int rows = plan.rows_per_unit;
   int err;
   if (elem == Elem::kF32)
-    err = p.dim == 64 ? run_simt<64>(p, stream) : run_simt<128>(p, stream);
+    err = p.dim == 64 ? run_f32<64>(p, stream) : run_f32<128>(p, stream);
   else
     err = tree_sm100_launch(elem, p, rows, stream);
   if (err != 0) return err;

@@ -472,8 +472,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = __all_sync(0xffffffffu, mbar_wait(q_empty, (w & 1) ^ 1, st, kSiteQFull, tmo));
         if (!ok) break;
         // Rows behind the unit's last are zeros: an MMA row is its own, but products of
-        // zeros draw less power, which is what bounds the clock here (32 trees,
-        // 128-row tiles 58 % full: POWER_NOTE).
+        // zeros draw less power, which bounds the clock (32 trees, row tiles 58 % full:
+        // 1455 instead of 1402 MHz and 318 instead of 323 us at the 1000 W cap).
         constexpr int kChunks = D / 8;
         const uint32_t qb = smem_u32(sQ);
         const int h0 = c.head_kv * p.group;
