@@ -129,6 +129,7 @@ struct TreePlan {
   int rows_per_unit;
   int grid;
   int merge_rows;  // rows the merge launch is sized for
+  int tile_keys;
   size_t acc_floats, ml_floats, meta_ints;
 };
 

@@ -82,8 +82,8 @@ __global__ void __launch_bounds__(kPathThreads) path_kernel(const __grid_constan
         s_bad = kBadPath;
       } else {
         const uint32_t page = p.page_size;
-        const int s = table[static_cast<uint32_t>(ctx + at) / page];
-        const int d = table[static_cast<uint32_t>(ctx + i) / page];
+        const int s = table[(static_cast<uint32_t>(ctx) + at) / page];
+        const int d = table[(static_cast<uint32_t>(ctx) + i) / page];
         if (s < 0 || s >= p.num_pages || d < 0 || d >= p.num_pages) s_bad = kBadPage;
       }
     }
@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(kPathThreads) path_kernel(const __grid_constan
     if (i0 > 0) __syncthreads();
     for (int i = threadIdx.x; i < 2 * steps; i += kPathThreads) {
       const int step = i0 + (i >> 1);
-      const uint32_t at = ctx + ((i & 1) ? step : path[step]);
+      const uint32_t at = static_cast<uint32_t>(ctx) + ((i & 1) ? step : path[step]);
       const uint32_t e = at / static_cast<uint32_t>(p.page_size);
       const int64_t off = table[e] * page_stride +
                           static_cast<int64_t>(at - e * p.page_size) * p.row_bytes;

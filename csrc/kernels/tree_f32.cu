@@ -733,10 +733,12 @@ TreePlan tree_plan(Elem elem, const TreeParams& p, int max_q, int sms) {
   TreePlan plan;
   if (elem == Elem::kF32) {
     plan.rows_per_unit = kF32Rows;
+    plan.tile_keys = p.dim == 64 ? F32Cfg<64>::kTile : F32Cfg<128>::kTile;
   } else {
     // one row tile keeps two key tiles in the air per CTA and suits what reading
     // the cache bounds; from the second row tile on, both share every key tile
     plan.rows_per_unit = static_cast<int64_t>(max_q) * p.group > 128 ? 256 : 128;
+    plan.tile_keys = 128;
   }
   plan.grid = sms;
   // rows of the largest unit that can occur (max_q is a hint: the merge loops)

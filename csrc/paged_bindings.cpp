@@ -179,6 +179,62 @@ std::tuple<torch::Tensor, OptTensor> rotary(torch::Tensor q, OptTensor k, torch:
   return {qo, ko};
 }
 
+// The rotation as an autograd function.  Its gradient is the transposed rotation, the
+// same pass by the negative angle; it goes through the function again, so it has a
+// gradient of its own.  In C++, since short training steps are bound by host time: a
+// forward call takes 9 us of it, and a backward pass little beside torch's own engine.
+class RotaryFunction : public torch::autograd::Function<RotaryFunction> {
+ public:
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx,
+                                                const torch::Tensor& q, const OptTensor& k,
+                                                const torch::Tensor& positions,
+                                                const torch::Tensor& inv_freq, bool interleaved,
+                                                double scale, bool inverse) {
+    ctx->save_for_backward({positions, inv_freq});
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["inverse"] = inverse;
+    ctx->saved_data["has_k"] = k.has_value();
+    auto out = rotary(q, k, positions, inv_freq, interleaved, scale, inverse, c10::nullopt,
+                      c10::nullopt);
+    if (!k) return {std::get<0>(out)};
+    return {std::get<0>(out), *std::get<1>(out)};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const bool interleaved = ctx->saved_data["interleaved"].toBool();
+    const double scale = ctx->saved_data["scale"].toDouble();
+    const bool inverse = !ctx->saved_data["inverse"].toBool();
+    const bool has_k = ctx->saved_data["has_k"].toBool();
+    // a gradient may be expanded or transposed; the kernel needs adjacent elements
+    auto rows = [](const torch::Tensor& t) {
+      return t.stride(2) == 1 || t.size(2) == 1 ? t : t.contiguous();
+    };
+    const bool need_q = ctx->needs_input_grad(0), need_k = has_k && ctx->needs_input_grad(1);
+    torch::autograd::variable_list result(7);
+    if (need_q && need_k) {
+      auto g = apply(rows(grads[0]), OptTensor(rows(grads[1])), saved[0], saved[1], interleaved,
+                     scale, inverse);
+      result[0] = g[0];
+      result[1] = g[1];
+    } else if (need_q || need_k) {
+      result[need_q ? 0 : 1] = apply(rows(grads[need_q ? 0 : 1]), OptTensor(), saved[0], saved[1],
+                                     interleaved, scale, inverse)[0];
+    }
+    return result;
+  }
+};
+
+std::tuple<torch::Tensor, OptTensor> rotary_autograd(torch::Tensor q, OptTensor k,
+                                                     torch::Tensor positions,
+                                                     torch::Tensor inv_freq, bool interleaved,
+                                                     double scale, bool inverse) {
+  auto out = RotaryFunction::apply(q, k, positions, inv_freq, interleaved, scale, inverse);
+  return {out[0], k ? OptTensor(out[1]) : OptTensor()};
+}
+
 // ---- pools and tables ----
 // k and v pools [.., pages, heads_kv, page_size, dim]; `layers` allows a leading layer dimension
 void check_pools(const torch::Tensor& k, const torch::Tensor& v, bool layers) {
@@ -189,7 +245,7 @@ void check_pools(const torch::Tensor& k, const torch::Tensor& v, bool layers) {
   RAB_CHECK(v.scalar_type() == k.scalar_type(), "v_pages must have k_pages' dtype");
   const int64_t d = k.dim();
   const int64_t hk = k.size(d - 3), page = k.size(d - 2), dim = k.size(d - 1);
-  RAB_CHECK(k.size(d - 4) <= INT32_MAX && hk >= 1 && hk <= 65535 && page >= 1 && page <= 65536 &&
+  RAB_CHECK(k.size(d - 4) >= 1 && k.size(d - 4) <= INT32_MAX && hk >= 1 && hk <= 65535 && page >= 1 && page <= 65536 &&
                 dim >= 1 && dim <= 4096,
             "the cache pool has a dimension of zero or too large");
   for (const torch::Tensor* t : {&k, &v}) {
@@ -470,11 +526,8 @@ std::tuple<torch::Tensor, OptTensor> tree_attention(torch::Tensor q, torch::Tens
             "page size %lld: attention takes 16, 32, 64, 128 or 256", ll(page));
   const Requests r = check_requests(table, ctx, cu, total);
   RAB_CHECK(table.size(1) <= (1 << 30) / page, "block_table has room for over 2^30 tokens");
-  // the kernels count rows and the places of their line of units in 32 bits
   const int64_t rows = total * (heads / hk);
   RAB_CHECK(rows <= (1 << 30), "over 2^30 rows of a kv head");
-  RAB_CHECK((rows / 8 + r.batch) * hk <= (int64_t{1} << 31) / (table.size(1) * page / 64 + 4),
-            "too many units of work for one call: split the batch");
   RAB_CHECK(!max_q || *max_q >= 1, "max_q must be positive");
   if (mask) {
     RAB_CHECK(mask->dim() == 2 && mask->size(0) == total,
@@ -554,6 +607,10 @@ std::tuple<torch::Tensor, OptTensor> tree_attention(torch::Tensor q, torch::Tens
   p.timeout_ns = static_cast<uint64_t>(timeout_s * 1e9);
   const int64_t most = max_q ? std::min<int64_t>(*max_q, total) : (cu ? total : r.uniform);
   const TreePlan plan = tree_plan(e, p, static_cast<int>(most), flash_sm_count());
+  // the kernels count the places of their line of units in 32 bits
+  RAB_CHECK((rows / plan.rows_per_unit + r.batch) * hk <=
+                (int64_t{1} << 31) / (table.size(1) * page / plan.tile_keys + 4),
+            "too many units of work for one call: split the batch");
   const size_t floats = plan.acc_floats + plan.ml_floats + plan.meta_ints;
   torch::Tensor ws = fresh({static_cast<int64_t>(floats)}, torch::kFloat32, q);
   p.rec_acc = static_cast<float*>(ws.data_ptr());
@@ -623,6 +680,9 @@ void register_paged(pybind11::module_& m) {
         py::arg("positions"), py::arg("inv_freq"), py::arg("interleaved") = false,
         py::arg("scale") = 1.0, py::arg("inverse") = false, py::arg("q_out") = c10::nullopt,
         py::arg("k_out") = c10::nullopt);
+  m.def("rotary_autograd", &rab::rotary_autograd, "rotary positions with their gradient",
+        py::arg("q"), py::arg("k"), py::arg("positions"), py::arg("inv_freq"),
+        py::arg("interleaved") = false, py::arg("scale") = 1.0, py::arg("inverse") = false);
   m.def("append_kv", &rab::append_kv, "write new tokens' K and V into a paged cache", py::arg("k"),
         py::arg("v"), py::arg("k_pages"), py::arg("v_pages"), py::arg("block_table"),
         py::arg("context_lens"), py::arg("cu_q") = c10::nullopt,

@@ -29,6 +29,7 @@ belong on one stream (or on streams that the caller orders).
 from __future__ import annotations
 
 import heapq
+import weakref
 from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
@@ -201,6 +202,13 @@ class CacheStep:
         table = cache.table
         if not self.seqs:
             raise ValueError("a step needs a sequence")
+        if cache.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("make the step outside a capture: its table is uploaded once")
+        for s in self.seqs:
+            other = cache._open.get(s, lambda: None)()
+            if other is not None and other._open:
+                raise RuntimeError(f"sequence {s} has a step that is neither committed, accepted "
+                                   "nor cancelled")
         src, dst = table.reserve(self.seqs, self.counts)
         if src:
             paged.copy_pages(cache.k, cache.v, src, dst)
@@ -222,10 +230,15 @@ class CacheStep:
         self.cu_q = dev[b:2 * b + 1]
         self.block_table = dev[2 * b + 1:].view(b, width)
         self._open = True
+        self._moves = cache._moves
+        for s in self.seqs:
+            cache._open[s] = weakref.ref(self)
 
     def _layer(self, layer: int) -> Tuple[torch.Tensor, torch.Tensor]:
         if not self._open:
             raise RuntimeError("the step is committed")
+        if self._moves != self.cache._moves:
+            raise RuntimeError("the cache was defragmented: the step's table is out of date")
         return self.cache.k[layer], self.cache.v[layer]
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, rotary: Optional[Rotary] = None,
@@ -277,6 +290,11 @@ class CacheStep:
         self._layer(0)
         self._close(self.counts)
 
+    def cancel(self) -> None:
+        """No token of the step stays."""
+        if self._open:
+            self._close([0] * len(self.seqs))
+
     def accept(self, paths: Sequence[Sequence[int]]) -> None:
         """The tokens on each sequence's path (increasing places within its tree; may
         be empty) stay, in every layer; the others are dropped."""
@@ -324,6 +342,8 @@ class PagedKVCache:
         self.k = torch.empty(shape, dtype=dtype, device=device)
         self.v = torch.empty(shape, dtype=dtype, device=device)
         self.device = self.k.device
+        self._open: Dict[int, "weakref.ref[CacheStep]"] = {}  # each sequence's last step
+        self._moves = 0
 
     def new_sequence(self) -> int:
         return self.table.new()
@@ -331,11 +351,19 @@ class PagedKVCache:
     def fork(self, seq: int) -> int:
         return self.table.fork(seq)
 
+    def _idle(self, seq: int) -> None:
+        step = self._open.get(seq, lambda: None)()
+        if step is not None and step._open:
+            raise RuntimeError(f"sequence {seq} has an open step: commit, accept or cancel it first")
+
     def free(self, seq: int) -> None:
+        self._idle(seq)
         self.table.free(seq)
+        self._open.pop(seq, None)
 
     def truncate(self, seq: int, length: int) -> None:
         """Drop the tokens of a sequence behind ``length``."""
+        self._idle(seq)
         self.table.truncate(seq, length)
 
     def length(self, seq: int) -> int:
@@ -347,7 +375,10 @@ class PagedKVCache:
 
     def defragment(self) -> int:
         """Move the pages in use to the front of the pool; returns how many there are.
-        Steps that are still open must not be used afterwards."""
+        No step may be open."""
+        for seq in self.table.sequences():
+            self._idle(seq)
+        self._moves += 1
         src, dst = self.table.compact()
         if src:
             paged.copy_pages(self.k, self.v, src, dst)

@@ -45,6 +45,8 @@ WAIT_SITES = {
     1: "q_full", 2: "k_full", 3: "v_full", 4: "k_empty", 5: "v_empty", 6: "s_full",
     7: "p_full", 8: "o_ready", 9: "block_ready", 10: "peer_ready", 11: "peer_consumed",
     12: "copy_slice", 13: "ring_flag", 14: "test", 15: "pv_done", 16: "item_queue",
+    # what a kernel of the paged cache skipped (status code 2)
+    201: "bad_page", 202: "bad_position", 203: "bad_path", 204: "bad_parent",
 }
 
 

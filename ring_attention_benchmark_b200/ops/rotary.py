@@ -90,38 +90,6 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str = "n
     return inv.to(device) if device is not None else inv, scale
 
 
-class _RotaryFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, positions, inv_freq, interleaved, scale, inverse):
-        ctx.save_for_backward(positions, inv_freq)
-        ctx.args = (interleaved, scale, inverse)
-        qo, ko = load().rotary(q, k, positions, inv_freq, interleaved, scale, inverse)
-        return qo, ko
-
-    @staticmethod
-    def backward(ctx, gq, gk):
-        # the transposed rotation: the same pass by the negative angle.  It goes
-        # through the operator again, so it has a gradient of its own.
-        positions, inv_freq = ctx.saved_tensors
-        interleaved, scale, inverse = ctx.args
-        need_q, need_k = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        args = (positions, inv_freq)
-        kw = dict(interleaved=interleaved, scale=scale, inverse=not inverse)
-        dq = dk = None
-        if need_q and need_k:
-            dq, dk = apply_rotary(_rows(gq), _rows(gk), *args, **kw)
-        elif need_q:
-            dq = apply_rotary(_rows(gq), None, *args, **kw)
-        elif need_k:
-            dk = apply_rotary(_rows(gk), None, *args, **kw)
-        return dq, dk, None, None, None, None, None
-
-
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """A gradient may be expanded or transposed; the kernel needs adjacent elements."""
-    return t if t.stride(-1) == 1 or t.size(-1) == 1 else t.contiguous()
-
-
 def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
                  inv_freq: torch.Tensor, *, interleaved: bool = False, scale: float = 1.0,
                  inverse: bool = False,
@@ -140,7 +108,7 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         if out is not None:
             raise ValueError("apply_rotary: out= is not offered where a gradient is needed")
-        qo, ko = _RotaryFn.apply(q, k, positions, inv_freq, interleaved, scale, inverse)
+        qo, ko = load().rotary_autograd(q, k, positions, inv_freq, interleaved, scale, inverse)
         return qo if k is None else (qo, ko)
     if out is None:
         qo, ko = load().rotary(q, k, positions, inv_freq, interleaved, scale, inverse)

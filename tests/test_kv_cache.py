@@ -148,6 +148,29 @@ def test_step_tensors_and_refusals():
         cache.step([], [])
 
 
+def test_one_open_step_per_sequence():
+    cache = PagedKVCache(1, 8, 1, 64, page_size=16, device="cpu")
+    a, b = cache.new_sequence(), cache.new_sequence()
+    step = cache.step([a], [20])
+    for call in (lambda: cache.step([b, a], [1, 1]), lambda: cache.free(a),
+                 lambda: cache.truncate(a, 0), cache.defragment):
+        with pytest.raises(RuntimeError, match="step"):
+            call()
+    assert cache.table.free_pages == 6  # the refused calls took nothing
+    fork = cache.fork(a)  # holds what is committed: nothing
+    assert cache.length(fork) == 0 and cache.table.pages(fork) == ()
+    step.cancel()
+    step.cancel()  # again: nothing
+    assert cache.table.free_pages == 8 and cache.length(a) == 0
+    with pytest.raises(RuntimeError, match="committed"):
+        step.commit()
+    cache.step([a], [3])  # dropped without a word: it does not block the sequence
+    step = cache.step([a], [5])
+    step.commit()
+    assert cache.length(a) == 5 and cache.defragment() == 1
+    cache.free(a)
+
+
 # ------------------------------------------------------------------ together (GPU)
 class _Plain:
     """What each sequence holds, layer by layer, as lists of 64-bit rows."""
