@@ -17,6 +17,8 @@ import json
 import torch
 
 from .._ext import load
+from .paged import append_kv, copy_pages, tree_attention
+from .rotary import apply_rotary, rotary_frequencies
 from ..utils.roofline import load_peaks
 
 
@@ -109,6 +111,32 @@ def main(argv=None) -> int:
                max(1, a.iters // 2), flush)
     # the exact-max pass recomputes QK^T: 6*sq*sk*d FLOPs issued, 4*sq*sk*d useful
     report("simt_partial_attention_4096", ms, flops=4.0 * 4096 * 4096 * 64)
+
+    # positions, and a paged cache of bf16 heads: written, copied, attended to
+    heads, hk = 16, 4
+    tokens = max(64, rows // 64)
+    inv, _ = rotary_frequencies(d, device=dev)
+    q = torch.randn(tokens, heads, d, device=dev).bfloat16()
+    k = torch.randn(tokens, hk, d, device=dev).bfloat16()
+    pos = torch.arange(tokens, device=dev)
+    ms = _time(lambda: apply_rotary(q, k, pos, inv), a.iters, flush)
+    report("rotary_bf16", ms, nbytes=(q.numel() + k.numel()) * 4)
+    if d in (64, 128):
+        pages = tokens // 64
+        kp = torch.zeros(2 * pages, hk, 64, d, device=dev, dtype=torch.bfloat16)
+        vp = torch.zeros_like(kp)
+        table = torch.randperm(pages, device=dev).int().view(1, -1)
+        none = torch.zeros(1, device=dev, dtype=torch.int32)
+        full = pages * 64
+        ms = _time(lambda: append_kv(k[:full], k[:full], kp, vp, table, none, inv_freq=inv),
+                   a.iters, flush)
+        report("append_kv_bf16", ms, nbytes=4 * full * hk * d * 2)
+        src = list(range(pages))
+        ms = _time(lambda: copy_pages(kp, vp, src, [p + pages for p in src]), a.iters, flush)
+        report("copy_pages_bf16", ms, nbytes=4 * full * hk * d * 2)
+        ctx = torch.full((1,), full - 1, device=dev, dtype=torch.int32)
+        ms = _time(lambda: tree_attention(q[:1], kp, vp, table, ctx), a.iters, flush)
+        report("tree_attention_one_token_bf16", ms, nbytes=2 * full * hk * d * 2)
 
     if a.json:
         print(json.dumps(results))
