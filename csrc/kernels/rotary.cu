@@ -256,10 +256,168 @@ __global__ void __launch_bounds__(kRopeThreads, 8)
   }
 }
 
+constexpr int kJointTokens = 64;       // tokens of a block of the kernel below, at most
+constexpr int kJointSmem = 32 * 1024;  // and bytes of their cosines and sines
+
+// The same for few heads: a block takes all operands of `tb` tokens, a thread to a
+// token while they are placed.
+template <typename T, int VEC, bool kInter>
+__global__ void __launch_bounds__(kRopeThreads, 8)
+    rope_joint_kernel(const __grid_constant__ RopeParams p, int tasks, int tb) {
+  using P = Pack<T, VEC>;
+  extern __shared__ __align__(16) float2 s_cs[];  // [tb][rotary_dim / 2]
+  // a token's place in the pool, and what may be done with it: 1 read, 2 written to the pool
+  __shared__ int s_page[kJointTokens], s_in[kJointTokens], s_ok[kJointTokens];
+  __shared__ int64_t s_pos[kJointTokens];
+  let_successor_start();
+  const int token0 = blockIdx.x * tb, tokens = min(tb, p.tokens - token0);
+  const int rows_step = kRopeThreads / tasks;
+  const int task = threadIdx.x % tasks, sub = threadIdx.x / tasks;
+  const int half = p.rotary_dim / 2;
+  wait_for_predecessor();
+  // where the tokens lie in the cache, and their positions
+  if (threadIdx.x < tokens) {
+    const int mine = threadIdx.x, token = token0 + mine;
+    int req = 0;
+    if (p.ctx != nullptr) {
+      if (p.cu == nullptr) {
+        req = token / p.uniform;
+      } else {
+        int hi = p.batch;  // the last request that starts at or before the token
+        while (hi - req > 1) {
+          const int mid = (req + hi) >> 1;
+          if (p.cu[mid] <= token) req = mid;
+          else hi = mid;
+        }
+      }
+    }
+    int64_t at = 0;
+    int ok = 3, page = 0, in = 0;
+    if (p.ctx != nullptr) {
+      int first = req * p.uniform;
+      if (p.cu != nullptr) {
+        first = p.cu[req];
+        if (token < first || token >= p.cu[req + 1]) ok = 0;  // behind the last request
+      }
+      if (ok) {
+        at = static_cast<int64_t>(p.ctx[req]) + (token - first);
+        if (at < 0 || at >= static_cast<int64_t>(p.table_w) * p.page_size) {
+          ok = 1;
+          st_record(p.status, kStatusBadArgs, kBadPosition, token);
+        } else {
+          const uint32_t entry = static_cast<uint32_t>(at) / static_cast<uint32_t>(p.page_size);
+          page = p.table[static_cast<int64_t>(req) * p.table_stride + entry];
+          in = static_cast<int>(static_cast<uint32_t>(at) - entry * p.page_size) * p.dim;
+          if (page < 0 || page >= p.num_pages) {
+            ok = 1;
+            st_record(p.status, kStatusBadArgs, kBadPage, page);
+          }
+        }
+      }
+    }
+    if (p.positions != nullptr)
+      at = p.positions64 ? static_cast<const int64_t*>(p.positions)[token]
+                         : static_cast<int64_t>(static_cast<const int*>(p.positions)[token]);
+    s_page[mine] = page;
+    s_in[mine] = in;
+    s_ok[mine] = ok;
+    s_pos[mine] = at;
+  }
+  if (half > 0) {
+    const int pair = threadIdx.x % half, t_step = kRopeThreads / half;
+    const uint64_t step = phase_step(p.inv_freq[pair]);
+    __syncthreads();
+    for (int u = threadIdx.x / half; u < tokens && threadIdx.x < t_step * half; u += t_step) {
+      const uint64_t phase = static_cast<uint64_t>(s_pos[u]) * step;
+      const int top = static_cast<int>((phase + 0x80000000ull) >> 32);
+      float sn, cs;
+      sincospif(static_cast<float>(top) * 0x1p-31f, &sn, &cs);
+      s_cs[u * half + cs_slot<VEC>(pair, half)] = make_float2(cs * p.scale, sn * p.scale * p.sign);
+    }
+  }
+  __syncthreads();
+
+  for (int o = 0; o < p.n_op; ++o) {
+    const RopeOperand& op = p.op[o];
+    const int heads = op.heads;
+    const int rot_tasks = op.rotate ? half / VEC : 0;
+    const bool rot = task < rot_tasks;
+    int ea, eb;
+    if (rot && !kInter) {
+      ea = task * VEC;
+      eb = half + task * VEC;
+    } else {  // pairs side by side, or elements behind the rotated ones
+      ea = task * 2 * VEC;
+      eb = ea + VEC;
+    }
+    const bool two = eb < p.dim;
+    const int need = op.paged ? 2 : 1;
+    const T* in = static_cast<const T*>(op.in) + static_cast<int64_t>(token0) * op.in_t;
+    T* out = static_cast<T*>(op.out);
+    const int step_t = rows_step / heads, step_h = rows_step - step_t * heads;
+    int t = sub < rows_step ? sub / heads : tokens, h = sub - sub / heads * heads;
+    while (t < tokens) {
+      if (s_ok[t] & need) {
+        const T* r = in + static_cast<int64_t>(t) * op.in_t + static_cast<int64_t>(h) * op.in_h;
+        P a = *reinterpret_cast<const P*>(r + ea), b;
+        if (two) b = *reinterpret_cast<const P*>(r + eb);
+        if (rot) {
+          float cs[VEC], sn[VEC];
+          const float2* c = s_cs + t * half;
+          if constexpr (VEC == 1) {
+            cs[0] = c[task].x;
+            sn[0] = c[task].y;
+          } else {
+#pragma unroll
+            for (int i = 0; i < VEC; i += 2) {
+              const float4 v = *reinterpret_cast<const float4*>(c + i * rot_tasks + 2 * task);
+              cs[i] = v.x;
+              sn[i] = v.y;
+              cs[i + 1] = v.z;
+              sn[i + 1] = v.w;
+            }
+          }
+          rotate<T, VEC, kInter>(a, b, cs, sn);
+        }
+        T* w = out + static_cast<int64_t>(h) * op.out_h +
+               (op.paged ? static_cast<int64_t>(s_page[t]) * op.out_t + s_in[t]
+                         : static_cast<int64_t>(token0 + t) * op.out_t);
+        *reinterpret_cast<P*>(w + ea) = a;
+        if (two) *reinterpret_cast<P*>(w + eb) = b;
+      }
+      t += step_t;
+      h += step_h;
+      if (h >= heads) {
+        h -= heads;
+        ++t;
+      }
+    }
+  }
+}
+
 template <typename T, int VEC, bool kInter>
 int rope_run(const RopeParams& p, cudaStream_t stream) {
   // a row's tasks: two vectors each; one more when the dims leave a single vector over
   const int tasks = (p.dim + 2 * VEC - 1) / (2 * VEC);
+  if constexpr (VEC > 1) {
+    // Few heads and many tokens: sines formed once for all operands, and enough tokens
+    // to a block that its widest operand gives every thread a row.  262144 tokens of
+    // one q and one k head x 64 take 40 us, 207 with a block per eight tokens and
+    // operand; 16 q and 4 k heads x 64 19 against 23, but 32 and 8 heads x 128 62
+    // against 56: many rows want the short loop.
+    const int rows_step = kRopeThreads / tasks;
+    int most = 1;
+    for (int i = 0; i < p.n_op; ++i) most = p.op[i].heads > most ? p.op[i].heads : most;
+    if (2 * most < rows_step && p.tokens >= 148 * 16) {
+      int tb = rows_step / most;
+      tb = tb < 16 ? 16 : (tb > kJointTokens ? kJointTokens : tb);
+      while (tb > 8 && tb * p.rotary_dim * static_cast<int>(sizeof(float)) > kJointSmem) tb >>= 1;
+      while (tb > 8 && (p.tokens + tb - 1) / tb < 148 * 4) tb >>= 1;
+      const size_t smem = static_cast<size_t>(tb) * (p.rotary_dim / 2) * sizeof(float2);
+      return launch_overlapped(rope_joint_kernel<T, VEC, kInter>, dim3((p.tokens + tb - 1) / tb),
+                               kRopeThreads, smem, stream, &p, &tasks, &tb);
+    }
+  }
   // Tokens of a block: as many as leave eight blocks per SM, down to one (a block
   // forms its sines itself, which is cheap beside idle SMs), whose heads are then
   // cut so that every thread has one row.

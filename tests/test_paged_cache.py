@@ -130,6 +130,7 @@ def _append_oracle(k, v, kp, vp, table, ctx, counts, inv=None, inter=False, posi
     ([5, 0, 31, 16], [1, 0, 3, 33], 8, 2, 128, 16, 64),
     ([100, 7, 0], [0, 17, 0], 3, 3, 64, 32, 32),
     ([3, 15], [20, 1], 6, 2, 80, 5, 10),
+    ([0, 9, 2, 700], [1200, 0, 1, 1700], 2, 1, 64, 16, 32),  # many tokens of few heads
 ])
 def test_append_values(ext, cuda_device, dtype, inter, ctx, counts, H, Hk, D, page, r):
     T, extra = sum(counts), 2
@@ -195,6 +196,32 @@ def test_append_skips_and_reports_bad_places(ext, cuda_device):
         check_status(st)
     kp[0, :, 2], vp[0, :, 2] = k[0], v[0]
     assert torch.equal(kd.cpu(), kp) and torch.equal(vd.cpu(), vp)
+
+
+@pytest.mark.gpu
+def test_append_of_many_tokens_skips_bad_places(ext, cuda_device):
+    """As above where one block holds many tokens: q is turned all the same."""
+    T, D, page = 2400, 64, 16
+    g = torch.Generator().manual_seed(8)
+    q, k, v = (torch.randn(T + 3, 1, D, generator=g) for _ in range(3))
+    inv = rotary_frequencies(64)[0]
+    kp, vp = _pool(200, 1, page, D, torch.float32)
+    table = torch.arange(140).int().view(1, 140).clone()  # room for 2240 places
+    table[0, 7] = 200
+    kd, vd = kp.cuda(), vp.cuda()
+    st = new_status("cuda")
+    qo = torch.full_like(q, 4.0).cuda()
+    append_kv(k.cuda(), v.cuda(), kd, vd, table.cuda(), torch.zeros(1, dtype=torch.int32).cuda(),
+              _cu([T]).cuda(), inv_freq=inv.cuda(), q=q.cuda(), q_out=qo, status=st)
+    with pytest.raises(DeviceTimeout, match="code=2"):
+        check_status(st)
+    pos = torch.arange(T)
+    assert ((qo[:T].cpu().double() - O.rotate(q[:T], pos, inv, False)).abs()
+            <= O.rotate_bound(q[:T], inv, False, 1.0, torch.float32, pos)).all()
+    assert (qo[T:] == 4.0).all()
+    kept = [i for i in range(2240) if i // page != 7]
+    vp[torch.tensor(kept) // page, 0, torch.tensor(kept) % page] = v[kept, 0]
+    assert torch.equal(vd.cpu(), vp)
 
 
 # ------------------------------------------------------------------ copies (GPU)

@@ -114,7 +114,10 @@ def _close(got, x, positions, inv, inter, scale, inverse=False):
 @pytest.mark.parametrize("inter", [False, True])
 @pytest.mark.parametrize("T,H,Hk,D,r", [(1, 1, 1, 64, 64), (7, 8, 2, 128, 128), (33, 3, 1, 128, 64),
                                         (5, 2, 2, 80, 32), (3, 5, 1, 96, 10), (2, 2, 1, 63, 2),
-                                        (1025, 4, 4, 64, 48), (2, 1, 1, 512, 512), (3, 40, 17, 64, 64)])
+                                        (1025, 4, 4, 64, 48), (2, 1, 1, 512, 512), (3, 40, 17, 64, 64),
+                                        # many tokens of few heads: all operands of a token in one block
+                                        (3001, 1, 1, 64, 64), (2500, 3, 2, 128, 64), (2400, 1, 1, 512, 512),
+                                        (9999, 2, 1, 64, 32)])
 def test_rotary_values(ext, cuda_device, dtype, inter, T, H, Hk, D, r):
     q, k = _inputs(T, H, Hk, D, dtype)
     inv, _ = rotary_frequencies(r)
