@@ -110,7 +110,8 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     ``q`` is ``[tokens, heads, dim]`` with dim 64 or 128 and heads a multiple of
     the cache's; page sizes 16 to 256, powers of two.  ``max_q`` is the most new
     tokens of any request where the caller knows it; it only steers the choice of
-    kernel.  Returns ``out``, or ``(out, lse)`` with the natural-log sums
+    kernel.  ``timeout_s`` bounds the kernel's waits for its own loads and products;
+    one that runs out is reported in ``status``.  Returns ``out``, or ``(out, lse)`` with the natural-log sums
     ``[tokens, heads]`` in fp32.
     """
     o, lse = load().tree_attention(q, k_pages, v_pages, block_table, context_lens, cu_q, max_q,

@@ -381,3 +381,126 @@ def test_empty_call(ext, cuda_device):
     case = _case([5], [0], 2, 1, 64, 16, torch.bfloat16)
     out, lse = _run(*case, [5], [0])
     assert out.shape == (0, 2, 64) and lse.shape == (0, 2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_replayed_call_follows_its_lengths(ext, cuda_device, dtype):
+    """Lengths, borders, pages and masks are read on the GPU: one captured call serves
+    every later step of the same shapes, filled in place."""
+    ctx, counts = [300, 40], [5, 3]
+    case = _case(ctx, counts, 4, 2, 64, 16, dtype, seed=13)
+    q, kp, vp, table = (x.cuda() for x in case)
+    ctx_t = torch.tensor(ctx, dtype=torch.int32).cuda()
+    cu = torch.tensor([0] + counts).cumsum(0).int().cuda()
+    mask = torch.zeros(8, 1, dtype=torch.int32, device="cuda")
+    tree_attention(q, kp, vp, table, ctx_t, cu, mask=mask)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = tree_attention(q, kp, vp, table, ctx_t, cu, mask=mask, return_lse=True)
+    for ctx2, counts2, seed in (([300, 40], [5, 3], 1), ([7, 290], [1, 7], 2), ([0, 100], [8, 0], 3)):
+        _, masks, rows, _ = _trees([max(c, 1) for c in counts2], seed)
+        rows = torch.cat([torch.nn.functional.pad(m[:c], (0, 32 - m.shape[1]))
+                          for m, c in zip(masks, counts2)])
+        ctx_t.copy_(torch.tensor(ctx2, dtype=torch.int32))
+        cu.copy_(torch.tensor([0] + counts2).cumsum(0).int())
+        mask.copy_(pack_mask(rows.cuda()))
+        graph.replay()
+        torch.cuda.synchronize()
+        tab = torch.nn.functional.pad(case[3], (0, 4))
+        # the table has room for the first request's 305 places in both rows
+        if ctx2[1] > 40:
+            table.copy_(case[3][[0, 0]])
+            graph.replay()
+            torch.cuda.synchronize()
+            tab = tab[[0, 0]]
+        _check(out, lse, (case[0], case[1], case[2], tab), ctx2, counts2,
+               [m[:c, :c] for m, c in zip(masks, counts2)])
+        table.copy_(case[3])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("page", [16, 256])
+def test_a_million_tokens(ext, cuda_device, dtype, page):
+    """2^20 cached tokens of one request that are 2048 keys 512 times over: the outputs
+    are theirs, and the sums 512 times as large."""
+    keys, times, D = 2048, 512, 128
+    case = _case([keys], [2], 4, 2, D, page, dtype, seed=14)
+    q, kp, vp, table = case
+    n = keys // page
+    long = torch.cat((table[0, :n].repeat(times), table[0, n:n + 2])).view(1, -1)
+    out, lse = tree_attention(q.cuda(), kp.cuda(), vp.cuda(), long.cuda(),
+                              torch.tensor([keys * times], dtype=torch.int32).cuda(), return_lse=True,
+                              mask=torch.zeros(2, 1, dtype=torch.bool, device="cuda"))
+    blank = [torch.zeros(2, 2, dtype=torch.bool)]
+    ref, rlse, mag, smax = O.attention(q, kp, vp, table, [keys], [2], blank)
+    rlse = rlse + math.log(times)
+    bo, bl = O.attention_bound(ref, mag, smax, dtype, keys * times, D)
+    assert ((out.cpu().double() - ref).abs() <= bo).all()
+    assert ((lse.cpu().double() - rlse).abs() <= bl + 2.0 ** -22 * rlse.abs()).all()
+    # the sums of so many keys are bounded loosely; a wrong key would show here
+    assert ((out.cpu().double() - ref).abs().max() <= (2.0 ** -16 + 2 * O.half_step(dtype)) * mag.max())
+
+
+@pytest.mark.gpu
+def test_pools_past_two_to_the_31(ext, cuda_device):
+    """Pages whose elements lie beyond 2^31: written, copied, compacted and attended to."""
+    from ring_attention_benchmark_b200.ops.paged import append_kv, compact_path, copy_pages
+
+    pages, Hk, page, D = 33000, 8, 128, 64  # 2.16e9 elements, 4.3 GB a pool
+    kp = torch.empty(pages, Hk, page, D, dtype=torch.bfloat16, device="cuda")
+    vp = torch.empty_like(kp)
+    ids = [pages - 1, 5, pages - 7, pages - 2]
+    q, k, v = (torch.randn(300, h, D, generator=torch.Generator().manual_seed(h)).bfloat16() for h in (8, 8, 8))
+    v = v + 1
+    table = torch.tensor([ids[:3]], dtype=torch.int32).cuda()
+    zero = torch.zeros(1, dtype=torch.int32).cuda()
+    append_kv(k.cuda(), v.cuda(), kp, vp, table, zero)
+    copy_pages(kp, vp, [ids[2]], [ids[3]])
+    table[0, 2] = ids[3]
+    ctx = torch.tensor([290], dtype=torch.int32).cuda()
+    compact_path(kp, vp, table, ctx, torch.tensor([[2, 5, 9]], dtype=torch.int32).cuda(),
+                 torch.tensor([3], dtype=torch.int32).cuda())
+    out, lse = tree_attention(q[:1].cuda(), kp, vp, table, torch.tensor([292], dtype=torch.int32).cuda(),
+                              return_lse=True)
+    keep = list(range(290)) + [292, 295, 299]
+    one = lambda x: x[keep].permute(1, 0, 2).reshape(1, Hk, len(keep), D)  # noqa: E731
+    ref, rlse, mag, smax = O.attention(q[:1], one(k), one(v), torch.zeros(1, 1, dtype=torch.int32), [292], [1])
+    bo, bl = O.attention_bound(ref, mag, smax, torch.bfloat16, 293, D)
+    assert ((out.cpu().double() - ref).abs() <= bo).all()
+    assert ((lse.cpu().double() - rlse).abs() <= bl + 2.0 ** -22 * rlse.abs()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_an_event_between_overlapped_launches_is_waited_for(ext, cuda_device, dtype):
+    """A launch may start while its predecessor in the stream runs, but not before an
+    event of another stream that it was told to wait for."""
+    from ring_attention_benchmark_b200.ops.paged import append_kv, copy_pages
+
+    ctx, counts = [150], [4]
+    q, kp, vp, table = (x.cuda() for x in _case(ctx, counts, 4, 2, 64, 16, dtype, seed=15))
+    ctx_t = torch.tensor(ctx, dtype=torch.int32).cuda()
+    want = tree_attention(q, kp, vp, table, ctx_t)
+    side, main = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        late, pool = torch.zeros_like(q), torch.zeros_like(kp)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(2_000_000)  # about a millisecond
+            late.copy_(q)
+            pool.copy_(kp)
+            ready = side.record_event()
+        with torch.cuda.stream(main):
+            copy_pages(kp, vp, [], [])
+            scratch = torch.zeros_like(kp)
+            append_kv(torch.zeros(4, 2, 64, dtype=dtype, device="cuda"),
+                      torch.zeros(4, 2, 64, dtype=dtype, device="cuda"), scratch,
+                      torch.zeros_like(vp), table, ctx_t)
+            main.wait_event(ready)
+            got = tree_attention(late, pool, vp, table, ctx_t)
+            late.zero_()  # an ordinary launch behind the overlapped ones
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
