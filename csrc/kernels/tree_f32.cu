@@ -8,19 +8,29 @@
 // with the running maximum m and the sums in fp32.  A row that sees nothing
 // gives 0 and lse = -inf.
 //
-// One CTA per SM takes its even share of the work (tree_sched.cuh), 8 rows of a kv
-// head at a time: the width of a small tensor-core product, whose other side is
-// keys (scores) or columns of V (outputs), so a decoding step reads the cache once
-// at fp32-level accuracy and stays bound by that (more rows read it again, from L2
-// where it fits).  Products are 3xTF32: x = hi + lo, hi rounded to 11 bits, and
-// hi*hi + lo*hi + hi*lo; what is left out is 2^-22 of a product.
+// One CTA per SM takes its even share of the work (tree_sched.cuh), 8, 16 or 32 rows of
+// a kv head at a time: the widths of one, two or four small tensor-core products, whose
+// other side is keys (scores) or columns of V (outputs).  A decoding step so reads the
+// cache once at fp32-level accuracy and stays bound by that.  Products are 3xTF32:
+// x = hi + lo, hi rounded to 11 bits, and hi*hi + lo*hi + hi*lo; what is left out is
+// 2^-22 of a product.
 //
 // Warp 8 walks the pieces and brings tiles of 64 KB (K and V of 128 keys at dim 64,
-// 64 keys at dim 128) by TMA into a ring of three.  Warps 0-7 take an eighth of a
-// tile's keys each, with their own running maximum, sum and outputs in registers,
-// joined once per piece.  Inside a product the order of the summed index is free:
-// it is chosen so that every read of K, V and the weights is 8 or 16 bytes wide and
-// the lanes of one pass meet different banks.
+// 64 keys at dim 128) by TMA into a ring.  Warps 0-7 take shares of a tile's keys (and,
+// of many rows at dim 128, a half of the rows) with their own running maximum, sum and
+// outputs in registers, joined once per piece.  Inside a product the order of the summed
+// index is free: it is chosen so that every read of K, V and the weights is 8 or 16
+// bytes wide and the lanes of one pass meet different banks.
+//
+// Up to eight rows (f32_narrow) the split queries stay in registers and the ring has
+// three stages; more (f32_wide) read them from shared memory, use each split of K and V
+// two or four times, and are bound by the tensor core: 17 cycles per product of a
+// scheduler, 16 being its rate.  us with units of 8 / 16 / 32 rows, 8 kv heads:
+//   rows of a kv head:      8          16            32           2000 (causal chunk)
+//   8000 keys, dim 64    14/-/-   19 / 17 / 23   30 / - / 25   1324 / - / 726
+//   8000 keys, dim 128   24/-/-   40 / 30 / 37   67 / - / 41   3003 / - / 1512
+//   4 x 32000, dim 128            367 / 275 / 371   804 / - / 372
+// hence 8, 16 or 32 by the rows of the longest request.
 //
 // 3 trees over 4096 to 16384 keys, 8 heads x 64 (126 MB, 19 us at the copy rate): 32
 // us with the merge, against 39 us with the products on the CUDA cores, which issue
@@ -43,10 +53,7 @@ using namespace tree_detail;
 
 namespace {
 
-constexpr int kF32Threads = 288;
-constexpr int kF32Rows = 8;
 constexpr int kF32Warps = 8;   // that compute
-constexpr int kF32Stages = 3;
 constexpr int kF32Items = 4;   // queue of pieces
 constexpr float kLn2f = 0.69314718055994530942f;
 
@@ -65,29 +72,42 @@ __device__ __forceinline__ __half cast_out<__half>(float x) {
   return __float2half_rn(x);
 }
 
-template <int D>
+template <int D, int kRows>
 struct F32Cfg {
-  static constexpr int kTile = 8192 / D;           // keys: 32 KB of K
-  static constexpr int kKeys = kTile / kF32Warps;  // of a warp: 16, or 8 (half a product's height)
+  static constexpr bool kWide = kRows > 8;
+  // whole warpgroups where they pass registers to the computing warps
+  static constexpr int kThreads = kWide ? 384 : 288;
+  static constexpr int kStages = kWide ? 2 : 3;
+  static constexpr int kTile = 8192 / D;  // keys: 32 KB of K
   static constexpr int kHalf = kTile * D * 4;  // bytes of K (or V) of a tile
   static constexpr int kStage = 2 * kHalf;
+  // a warp's keys: 16, or 8 (half a product's height) with eight rows of dim 128; more
+  // rows of dim 128 go to the two halves of the warps instead
+  static constexpr int kSplit = kWide ? kF32Warps * 16 / kTile : 1;
+  static constexpr int kKeys = kTile * kSplit / kF32Warps;
+  static constexpr int kGroups = kRows / 8 / kSplit;  // of eight rows, a warp's
   // floats of a warp: weights [row][key] in the tiles, [row][dim] outputs at a piece's end
-  static constexpr int kOwn = kF32Rows * D;
+  static constexpr int kOwn = kGroups * 8 * D;
   static constexpr int kPRow = kKeys + 4;  // between the weights of two rows
-  static constexpr int kMlOff = kF32Stages * kStage + kF32Warps * kOwn * 4;  // float2 [warps][rows]
-  static constexpr int kItemOff = kMlOff + kF32Warps * kF32Rows * 8;
+  static constexpr int kOwnOff = kStages * kStage;
+  // split queries, [row / 8][dim / 16][hi, lo][lane] fragments; eight rows stay in registers
+  static constexpr int kQOff = kOwnOff + kF32Warps * kOwn * 4;
+  static constexpr int kQGroup = D / 16 * 1024;  // bytes of eight rows
+  static constexpr int kMlOff = kQOff + (kWide ? kRows / 8 * kQGroup : 0);  // float2 [warps][own rows]
+  static constexpr int kItemOff = kMlOff + kF32Warps * kGroups * 8 * 8;
   static constexpr int kBarOff = kItemOff + kF32Items * 48;
-  static constexpr int kBars = 2 * kF32Stages + 2 * kF32Items + 2;
+  static constexpr int kBars = 2 * kStages + 2 * kF32Items + 2;
   static constexpr int kDirtyOff = kBarOff + kBars * 8;  // int [2]
   static constexpr int kSmem = kDirtyOff + 8;
   static_assert(kSmem <= 232448 && kBarOff % 8 == 0, "shared memory");
+  static_assert(!kWide || (kKeys == 16 && kGroups >= 1), "rows of a unit");
 };
 
 // byte offset of element `col` of row `key` in a tile of [dim / 32][keys][32 floats],
 // 16-byte chunks swizzled by the row within 128 bytes
 template <int D>
 __device__ __forceinline__ int tile_at(int key, int col) {
-  return (col >> 5) * (F32Cfg<D>::kTile * 128) + key * 128 + ((((col >> 2) & 7) ^ (key & 7)) << 4) +
+  return (col >> 5) * (8192 / D * 128) + key * 128 + ((((col >> 2) & 7) ^ (key & 7)) << 4) +
          (col & 3) * 4;
 }
 
@@ -147,149 +167,150 @@ __device__ __noinline__ void add_left_out(const TreeParams& p, const Piece& c, i
   }
 }
 
+// the barriers and the queue of a block
+template <typename C>
+struct F32Block {
+  uint8_t* smem;
+  __device__ __forceinline__ uint64_t* bars() const {
+    return reinterpret_cast<uint64_t*>(smem + C::kBarOff);
+  }
+  __device__ __forceinline__ uint64_t* full(int i) const { return bars() + i; }
+  __device__ __forceinline__ uint64_t* empty(int i) const { return bars() + C::kStages + i; }
+  __device__ __forceinline__ uint64_t* item_full(int w) const {
+    return bars() + 2 * C::kStages + w % kF32Items;
+  }
+  __device__ __forceinline__ uint64_t* item_empty(int w) const {
+    return item_full(w) + kF32Items;
+  }
+  __device__ __forceinline__ uint64_t* joined() const {
+    return bars() + 2 * C::kStages + 2 * kF32Items;
+  }
+  __device__ __forceinline__ uint64_t* released() const { return joined() + 1; }
+  __device__ __forceinline__ Piece* item(int w) const {
+    return reinterpret_cast<Piece*>(smem + C::kItemOff + (w % kF32Items) * 48);
+  }
+  // [2], by the piece's parity
+  __device__ __forceinline__ volatile int* dirty() const {
+    return reinterpret_cast<int*>(smem + C::kDirtyOff);
+  }
+  __device__ __forceinline__ float* own(int warp) const {
+    return reinterpret_cast<float*>(smem + C::kOwnOff) + warp * C::kOwn;
+  }
+  // maximum and sum of row r of warp u
+  __device__ __forceinline__ float2& ml(int u, int r) const {
+    return reinterpret_cast<float2*>(smem + C::kMlOff)[u * (C::kGroups * 8) + r];
+  }
+};
+
+// One warp: walks the pieces and loads their tiles.
+template <int D, int kRows>
+__device__ __forceinline__ void f32_walk(const TreeParams& p, const CUtensorMap& tmK,
+                                         const CUtensorMap& tmV,
+                                         const F32Block<F32Cfg<D, kRows>>& blk) {
+  using C = F32Cfg<D, kRows>;
+  using namespace sm100;
+  constexpr int kTile = C::kTile;
+  const int lane = lane_id();
+  DeviceStatus* st = p.status;
+  const uint64_t tmo = p.timeout_ns;
+  if (lane == 0) {
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+    p.meta[blockIdx.x * kMetaInts] = 0;
+  }
+  Range range;
+  Start first;
+  const int walker = find_range<kTile, kRows>(p, &range, &first);
+  Walk<kTile, kRows> walk;
+  if (lane == walker) walk.start(p, range, first);
+  const int rows_box = min(p.page_size, kTile);
+  const int boxes = kTile / rows_box * (D / 32);
+  int n = 0;  // tiles loaded
+  bool ok = true;
+  for (int w = 0; ok; ++w) {
+    if (w >= kF32Items)
+      ok = __all_sync(0xffffffffu, mbar_wait(blk.item_empty(w),
+                                             (w / kF32Items - 1) & 1, st, kSiteItemQueue, tmo));
+    if (!ok) break;
+    Piece* slot = blk.item(w);
+    if (lane == walker) {
+      Piece c;
+      if (walk.next(p, range, &c)) {
+        if (walk.merges) write_meta(p, c, true, walk.merge_c0);
+      } else {
+        c.request = -1;
+      }
+      *slot = c;
+    }
+    __syncwarp();
+    const Piece c = *slot;
+    if (lane == 0) mbar_arrive(blk.item_full(w));
+    if (c.request < 0) break;
+    const int* table = p.table + static_cast<int64_t>(c.request) * p.table_stride;
+    const int last_entry = (c.keys - 1) >> p.page_shift;
+    for (int tile = c.tile_begin; tile < c.tile_end; ++tile) {
+      // this lane's box: page, rows within the tile, 32-column segment
+      const int seg = lane % (D / 32), part = lane / (D / 32);
+      int page = p.num_pages, token = 0;
+      if (lane < boxes) {
+        const int key = tile * kTile + part * rows_box;
+        const int entry = key >> p.page_shift;
+        token = key & (p.page_size - 1);
+        if (entry <= last_entry) {  // behind it: a coordinate past the pool loads zeros
+          page = table[entry];
+          if (page < 0 || page >= p.num_pages) {
+            if (seg == 0) st_record(st, kStatusBadArgs, kBadPage, static_cast<uint32_t>(page));
+            page = p.num_pages;
+          }
+        }
+      }
+      const int stage = n % C::kStages;
+      ok = __all_sync(0xffffffffu, mbar_wait(blk.empty(stage), ((n / C::kStages) & 1) ^ 1, st,
+                                             kSiteKEmpty, tmo));
+      if (!ok) break;
+      if (lane == 0) mbar_arrive_expect_tx(blk.full(stage), C::kStage);
+      __syncwarp();
+      if (lane < boxes) {
+        uint8_t* dst = blk.smem + stage * C::kStage + seg * (kTile * 128) + part * rows_box * 128;
+        tma_load_4d(dst, &tmK, blk.full(stage), seg * 32, token, c.head_kv, page);
+        tma_load_4d(dst + C::kHalf, &tmV, blk.full(stage), seg * 32, token, c.head_kv, page);
+      }
+      ++n;
+    }
+  }
+  // the loads in flight land before the block gives its memory back
+  for (int i = 0; i < C::kStages && i < n; ++i) {
+    const int k = n - 1 - i;
+    mbar_wait(blk.full(k % C::kStages), (k / C::kStages) & 1, nullptr, kSiteKFull, 100000000ull);
+  }
+}
+
+// A computing warp, eight rows to a unit.
+// Fragments of a 16 x 8 x 8 product: lane = 4 g + t.  Scores: rows are keys, columns
+// query rows, the summed index is dim; this lane's sums are keys g and g + 8 (of the
+// warp's, in the order key_of) of query rows 2t and 2t + 1.  Outputs: rows are columns
+// of V, the summed index is keys; this lane's are dims 32 h + 4 g + 0..3 of query rows
+// 2t and 2t + 1.
 template <int D>
-__global__ void __launch_bounds__(kF32Threads, 1)
-    tree_f32_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap tmK,
-                     const __grid_constant__ CUtensorMap tmV) {
-  using C = F32Cfg<D>;
+__device__ __forceinline__ void f32_narrow(const TreeParams& p, const F32Block<F32Cfg<D, 8>>& blk) {
+  using C = F32Cfg<D, 8>;
   using namespace sm100;
   constexpr int kTile = C::kTile, kKeys = C::kKeys;
-  extern __shared__ __align__(1024) uint8_t smem[];
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
-  uint64_t* empty = full + kF32Stages;
-  uint64_t* item_full = empty + kF32Stages;
-  uint64_t* item_empty = item_full + kF32Items;
-  uint64_t* joined = item_empty + kF32Items;
-  uint64_t* released = joined + 1;
-  volatile int* s_dirty = reinterpret_cast<int*>(smem + C::kDirtyOff);  // [2], by the piece's parity
-  auto item_slot = [&](int w) {
-    return reinterpret_cast<Piece*>(smem + C::kItemOff + (w % kF32Items) * 48);
-  };
   const int warp = warp_id(), lane = lane_id();
   DeviceStatus* st = p.status;
   const uint64_t tmo = p.timeout_ns;
-  if ((smem_u32(smem) & 1023u) != 0) {  // the swizzle counts from 1024-byte boundaries
-    wait_for_predecessor();
-    if (threadIdx.x == 0) {
-      p.meta[blockIdx.x * kMetaInts] = 0;
-      st_record(st, kStatusBadArgs, kSiteNone);
-    }
-    return;
-  }
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < kF32Stages; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], kF32Warps);
-    }
-    for (int i = 0; i < kF32Items; ++i) {
-      mbar_init(&item_full[i], 1);
-      mbar_init(&item_empty[i], kF32Warps);
-    }
-    mbar_init(joined, kF32Warps);
-    mbar_init(released, kF32Warps);
-    s_dirty[0] = s_dirty[1] = 0;
-    fence_barrier_init();
-  }
-  let_successor_start();
-  __syncthreads();
-  wait_for_predecessor();
-
-  if (warp == kF32Warps) {
-    // -------------------------------------------------------- pieces and loads
-    if (lane == 0) {
-      tma_prefetch_desc(&tmK);
-      tma_prefetch_desc(&tmV);
-      p.meta[blockIdx.x * kMetaInts] = 0;
-    }
-    Range range;
-    Start first;
-    const int walker = find_range<kTile, kF32Rows>(p, &range, &first);
-    Walk<kTile, kF32Rows> walk;
-    if (lane == walker) walk.start(p, range, first);
-    const int rows_box = min(p.page_size, kTile);
-    const int boxes = kTile / rows_box * (D / 32);
-    int n = 0;  // tiles loaded
-    bool ok = true;
-    for (int w = 0; ok; ++w) {
-      if (w >= kF32Items)
-        ok = __all_sync(0xffffffffu, mbar_wait(&item_empty[w % kF32Items],
-                                               (w / kF32Items - 1) & 1, st, kSiteItemQueue, tmo));
-      if (!ok) break;
-      Piece* slot = item_slot(w);
-      if (lane == walker) {
-        Piece c;
-        if (walk.next(p, range, &c)) {
-          if (walk.merges) write_meta(p, c, true, walk.merge_c0);
-        } else {
-          c.request = -1;
-        }
-        *slot = c;
-      }
-      __syncwarp();
-      const Piece c = *slot;
-      if (lane == 0) mbar_arrive(&item_full[w % kF32Items]);
-      if (c.request < 0) break;
-      const int* table = p.table + static_cast<int64_t>(c.request) * p.table_stride;
-      const int last_entry = (c.keys - 1) >> p.page_shift;
-      for (int tile = c.tile_begin; tile < c.tile_end; ++tile) {
-        // this lane's box: page, rows within the tile, 32-column segment
-        const int seg = lane % (D / 32), part = lane / (D / 32);
-        int page = p.num_pages, token = 0;
-        if (lane < boxes) {
-          const int key = tile * kTile + part * rows_box;
-          const int entry = key >> p.page_shift;
-          token = key & (p.page_size - 1);
-          if (entry <= last_entry) {  // behind it: a coordinate past the pool loads zeros
-            page = table[entry];
-            if (page < 0 || page >= p.num_pages) {
-              if (seg == 0) st_record(st, kStatusBadArgs, kBadPage, static_cast<uint32_t>(page));
-              page = p.num_pages;
-            }
-          }
-        }
-        const int stage = n % kF32Stages;
-        ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], ((n / kF32Stages) & 1) ^ 1, st,
-                                               kSiteKEmpty, tmo));
-        if (!ok) break;
-        if (lane == 0) mbar_arrive_expect_tx(&full[stage], C::kStage);
-        __syncwarp();
-        if (lane < boxes) {
-          uint8_t* dst = smem + stage * C::kStage + seg * (kTile * 128) + part * rows_box * 128;
-          tma_load_4d(dst, &tmK, &full[stage], seg * 32, token, c.head_kv, page);
-          tma_load_4d(dst + C::kHalf, &tmV, &full[stage], seg * 32, token, c.head_kv, page);
-        }
-        ++n;
-      }
-    }
-    // the loads in flight land before the block gives its memory back
-    for (int i = 0; i < kF32Stages && i < n; ++i) {
-      const int k = n - 1 - i;
-      mbar_wait(&full[k % kF32Stages], (k / kF32Stages) & 1, nullptr, kSiteKFull, 100000000ull);
-    }
-    return;
-  }
-
-  // ------------------------------------------------------------------ arithmetic
-  // Fragments of a 16 x 8 x 8 product: lane = 4 g + t.  Scores: rows are keys, columns
-  // query rows, the summed index is dim; this lane's sums are keys g and g + 8 (of the
-  // warp's, in the order key_of) of query rows 2t and 2t + 1.  Outputs: rows are columns
-  // of V, the summed index is keys; this lane's are dims 32 h + 4 g + 0..3 of query rows
-  // 2t and 2t + 1.
-  float* own = reinterpret_cast<float*>(smem + kF32Stages * C::kStage) + warp * C::kOwn;
+  float* own = blk.own(warp);
   float* s_p = own;
-  auto s_ml = [&](int u, int r) -> float2& {  // maximum and sum of warp u's row r
-    return reinterpret_cast<float2*>(smem + C::kMlOff)[u * kF32Rows + r];
-  };
   const int g = lane >> 2, t = lane & 3;
   // rows g and g + 1 of one pass lie four keys apart: their swizzled words meet no bank twice
   const int key_g = (g >> 1) + 4 * (g & 1);
   int n = 0;  // tiles taken
   bool ok = true;
   for (int w = 0; ok; ++w) {
-    ok = __all_sync(0xffffffffu, mbar_wait(&item_full[w % kF32Items], (w / kF32Items) & 1, st,
+    ok = __all_sync(0xffffffffu, mbar_wait(blk.item_full(w), (w / kF32Items) & 1, st,
                                            kSiteItemQueue, tmo));
     if (!ok) break;
-    const Piece c = *item_slot(w);
+    const Piece c = *blk.item(w);
     if (c.request < 0) break;
     // queries of row g, scaled to base-2 exponents; dim 16 b + 4 t + 0..3 is summed at
     // places t, t + 4 of step 2 b and t, t + 4 of step 2 b + 1
@@ -314,7 +335,7 @@ __global__ void __launch_bounds__(kF32Threads, 1)
         for (int i = 0; i < 2; ++i) split3x(q_hi[b][i], q_hi[b][i], q_lo[b][i]);
     }
     if (w > 0) {  // the piece before has been read out of every warp's outputs
-      ok = __all_sync(0xffffffffu, mbar_wait(released, (w - 1) & 1, st, kSiteOReady, tmo));
+      ok = __all_sync(0xffffffffu, mbar_wait(blk.released(), (w - 1) & 1, st, kSiteOReady, tmo));
       if (!ok) break;
     }
     float acc[D / 16][4];  // [4 h + i]: dims 64 h + 32 e + 4 g + i of rows 2t + r at 2 e + r
@@ -326,11 +347,11 @@ __global__ void __launch_bounds__(kF32Threads, 1)
     bool dirty = false;
 
     for (int tile = c.tile_begin; tile < c.tile_end; ++tile, ++n) {
-      const int stage = n % kF32Stages;
-      ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], (n / kF32Stages) & 1, st, kSiteKFull,
+      const int stage = n % C::kStages;
+      ok = __all_sync(0xffffffffu, mbar_wait(blk.full(stage), (n / C::kStages) & 1, st, kSiteKFull,
                                              tmo));
       if (!ok) break;
-      const uint8_t* sk = smem + stage * C::kStage;
+      const uint8_t* sk = blk.smem + stage * C::kStage;
       const uint8_t* sv = sk + C::kHalf;
       // even and odd steps are summed apart, so that products do not wait for one
       // another, and so are the small products (below)
@@ -458,7 +479,7 @@ __global__ void __launch_bounds__(kF32Threads, 1)
         }
       }
       __syncwarp();  // s_p and the stage have been read
-      if (lane == 0) mbar_arrive(&empty[stage]);
+      if (lane == 0) mbar_arrive(blk.empty(stage));
 #pragma unroll
       for (int b = 0; b < D / 16; ++b)
 #pragma unroll
@@ -467,12 +488,12 @@ __global__ void __launch_bounds__(kF32Threads, 1)
     if (!ok) break;
 
     // join the warps
-    if (dirty) s_dirty[w & 1] = w + 1;
+    if (dirty) blk.dirty()[w & 1] = w + 1;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], d);
-      if (g == 0) s_ml(warp, 2 * t + i) = make_float2(m[i], l[i]);
+      if (g == 0) blk.ml(warp, 2 * t + i) = make_float2(m[i], l[i]);
     }
 #pragma unroll
     for (int h = 0; h < D / 64; ++h)
@@ -484,21 +505,21 @@ __global__ void __launch_bounds__(kF32Threads, 1)
               make_float4(acc[4 * h][2 * e + i], acc[4 * h + 1][2 * e + i],
                           acc[4 * h + 2][2 * e + i], acc[4 * h + 3][2 * e + i]);
     __syncwarp();
-    if (lane == 0) mbar_arrive(joined);
-    ok = __all_sync(0xffffffffu, mbar_wait(joined, w & 1, st, kSiteOReady, tmo));
+    if (lane == 0) mbar_arrive(blk.joined());
+    ok = __all_sync(0xffffffffu, mbar_wait(blk.joined(), w & 1, st, kSiteOReady, tmo));
     if (!ok) break;
-    const float* all = reinterpret_cast<const float*>(smem + kF32Stages * C::kStage);
+    const float* all = blk.own(0);
     // row `warp` of the eight, four columns at a time
     if (warp < c.rows) {
       const int r = warp;
       float top = -INFINITY;
 #pragma unroll
-      for (int u = 0; u < kF32Warps; ++u) top = fmaxf(top, s_ml(u, r).x);
+      for (int u = 0; u < kF32Warps; ++u) top = fmaxf(top, blk.ml(u, r).x);
       const float use = top == -INFINITY ? 0.f : top;
       float sum = 0.f, f[kF32Warps];
 #pragma unroll
       for (int u = 0; u < kF32Warps; ++u) {
-        const float2 ml = s_ml(u, r);
+        const float2 ml = blk.ml(u, r);
         f[u] = ex2_approx(ml.x - use);
         sum += f[u] * ml.y;
       }
@@ -507,7 +528,7 @@ __global__ void __launch_bounds__(kF32Threads, 1)
       const float inv = c.record >= 0 ? 1.f : (sum == 0.f ? 0.f : 1.f / sum);
       // a record is [dim / 4][rows][4], the rows of the unit side by side
       float* rec = c.record >= 0
-                       ? p.rec_acc + static_cast<int64_t>(c.record) * (kF32Rows * D) + r * 4
+                       ? p.rec_acc + static_cast<int64_t>(c.record) * (8 * D) + r * 4
                        : nullptr;
       float* out = static_cast<float*>(p.out) + static_cast<int64_t>(c.first + tok) * p.out_t +
                    static_cast<int64_t>(h) * p.out_h;
@@ -523,13 +544,13 @@ __global__ void __launch_bounds__(kF32Threads, 1)
         }
         o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
         *reinterpret_cast<float4*>(rec != nullptr ? rec + lane * 4 * c.rows : out + lane * 4) = o;
-        if (s_dirty[w & 1] == w + 1)
+        if (blk.dirty()[w & 1] == w + 1)
           add_left_out(p, c, tok, kTile, lane * 4, lane * 4 + 4, D, rec, out);
       }
       if (lane == 0) {
         if (c.record >= 0) {
-          p.rec_m[c.record * kF32Rows + r] = top;
-          p.rec_l[c.record * kF32Rows + r] = sum;
+          p.rec_m[c.record * 8 + r] = top;
+          p.rec_l[c.record * 8 + r] = sum;
         } else if (p.lse != nullptr) {
           p.lse[static_cast<int64_t>(c.first + tok) * p.heads + h] =
               sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2f;
@@ -538,9 +559,362 @@ __global__ void __launch_bounds__(kF32Threads, 1)
     }
     __syncwarp();
     if (lane == 0) {
-      mbar_arrive(released);
-      mbar_arrive(&item_empty[w % kF32Items]);
+      mbar_arrive(blk.released());
+      mbar_arrive(blk.item_empty(w));
     }
+  }
+}
+
+// A computing warp, 16 or 32 rows to a unit: the fragments of f32_narrow, with every
+// split of K and V used for the warp's kGroups groups of eight rows.  Warp u takes the
+// groups of the unit from (u / key warps) * kGroups on.
+template <int D, int kRows>
+__device__ __forceinline__ void f32_wide(const TreeParams& p,
+                                         const F32Block<F32Cfg<D, kRows>>& blk) {
+  using C = F32Cfg<D, kRows>;
+  using namespace sm100;
+  constexpr int kTile = C::kTile, kKeys = C::kKeys, G = C::kGroups;
+  constexpr int kKeyWarps = kF32Warps / C::kSplit;
+  const int warp = warp_id(), lane = lane_id();
+  DeviceStatus* st = p.status;
+  const uint64_t tmo = p.timeout_ns;
+  float* own = blk.own(warp);
+  float* s_p = own;
+  const int g = lane >> 2, t = lane & 3;
+  const int key_g = (g >> 1) + 4 * (g & 1);
+  const int key0 = warp % kKeyWarps * kKeys;      // this warp's first key of a tile
+  const int row_w = warp / kKeyWarps * (8 * G);   // and its first row of the unit
+  int n = 0;  // tiles taken
+  bool ok = true;
+  for (int w = 0; ok; ++w) {
+    ok = __all_sync(0xffffffffu,
+                    mbar_wait(blk.item_full(w), (w / kF32Items) & 1, st, kSiteItemQueue, tmo));
+    if (!ok) break;
+    const Piece c = *blk.item(w);
+    if (c.request < 0) break;
+    // The warps split the unit's queries, scaled to base-2 exponents: this one the 16
+    // columns b of every eight rows.  Every warp has left the piece before (`joined`).
+    for (int b = warp; b < D / 16; b += kF32Warps) {
+#pragma unroll
+      for (int u = 0; u < kRows / 8; ++u) {
+        const int row = c.row0 + min(8 * u + g, c.rows - 1), tok = row / p.group;
+        const int h = c.head_kv * p.group + row - tok * p.group;
+        const float4 v = *reinterpret_cast<const float4*>(
+            static_cast<const float*>(p.q) + static_cast<int64_t>(c.first + tok) * p.q_t +
+            static_cast<int64_t>(h) * p.q_h + 16 * b + 4 * t);
+        float4 hi, lo;
+        split3x(v.x * p.scale_log2, hi.x, lo.x);
+        split3x(v.y * p.scale_log2, hi.y, lo.y);
+        split3x(v.z * p.scale_log2, hi.z, lo.z);
+        split3x(v.w * p.scale_log2, hi.w, lo.w);
+        float4* dst =
+            reinterpret_cast<float4*>(blk.smem + C::kQOff + u * C::kQGroup + b * 1024) + lane;
+        dst[0] = hi;
+        dst[32] = lo;
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(blk.released());
+    // the queries are there, and the piece before has been read out of every warp's outputs
+    ok = __all_sync(0xffffffffu, mbar_wait(blk.released(), w & 1, st, kSiteOReady, tmo));
+    if (!ok) break;
+    float acc[G][D / 16][4];
+    float m[G][2], l[G][2];
+#pragma unroll
+    for (int u = 0; u < G; ++u) {
+#pragma unroll
+      for (int b = 0; b < D / 16; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[u][b][i] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        m[u][i] = -INFINITY;
+        l[u][i] = 0.f;
+      }
+    }
+    bool dirty = false;
+
+    for (int tile = c.tile_begin; tile < c.tile_end; ++tile, ++n) {
+      const int stage = n % C::kStages;
+      ok = __all_sync(0xffffffffu, mbar_wait(blk.full(stage), (n / C::kStages) & 1, st,
+                                             kSiteKFull, tmo));
+      if (!ok) break;
+      const uint8_t* sk = blk.smem + stage * C::kStage;
+      const uint8_t* sv = sk + C::kHalf;
+      const float4* sq =
+          reinterpret_cast<const float4*>(blk.smem + C::kQOff + row_w / 8 * C::kQGroup) + lane;
+      float s[G][4] = {}, s_lo[G][4] = {};
+#pragma unroll
+      for (int b = 0; b < D / 16; ++b) {
+        float k_hi[2][4], k_lo[2][4];
+#pragma unroll
+        for (int hlf = 0; hlf < 2; ++hlf) {
+          const float4 v = *reinterpret_cast<const float4*>(
+              sk + tile_at<D>(key0 + key_g + 8 * hlf, 16 * b + 4 * t));
+          split3x(v.x, k_hi[0][hlf], k_lo[0][hlf]);
+          split3x(v.y, k_hi[0][2 + hlf], k_lo[0][2 + hlf]);
+          split3x(v.z, k_hi[1][hlf], k_lo[1][hlf]);
+          split3x(v.w, k_hi[1][2 + hlf], k_lo[1][2 + hlf]);
+        }
+        float4 hi[G], lo[G];
+#pragma unroll
+        for (int u = 0; u < G; ++u) {
+          hi[u] = sq[u * (C::kQGroup / 16) + b * 64];
+          lo[u] = sq[u * (C::kQGroup / 16) + b * 64 + 32];
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int u = 0; u < G; ++u) mma_tf32(s_lo[u], k_lo[e], e == 0 ? &hi[u].x : &hi[u].z);
+#pragma unroll
+          for (int u = 0; u < G; ++u) mma_tf32(s[u], k_hi[e], e == 0 ? &hi[u].x : &hi[u].z);
+#pragma unroll
+          for (int u = 0; u < G; ++u) mma_tf32(s_lo[u], k_hi[e], e == 0 ? &lo[u].x : &lo[u].z);
+        }
+      }
+      const int j0 = tile * kTile + key0;
+      const bool tail = (tile + 1) * kTile > c.ctx;  // new tokens, or past the end
+      float alpha[G][2];
+#pragma unroll
+      for (int u = 0; u < G; ++u) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[u][i] += s_lo[u][i];  // [2 key + row]
+        if (tail) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int r = row_w + 8 * u + 2 * t + i;
+            const int tok = (c.row0 + r) / p.group;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const int j = j0 + key_g + 8 * x, rel = j - c.ctx;
+              if (rel < 0) continue;
+              bool sees = j < c.keys && r < c.rows;
+              if (sees)
+                sees = p.mask == nullptr
+                           ? rel <= tok
+                           : (rel >> 5) < p.mask_w &&
+                                 ((p.mask[static_cast<int64_t>(c.first + tok) * p.mask_stride +
+                                          (rel >> 5)] >>
+                                   (rel & 31)) &
+                                  1u);
+              if (!sees) s[u][2 * x + i] = -INFINITY;
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float mx = fmaxf(s[u][i], s[u][2 + i]);
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+          const float mn = fmaxf(m[u][i], mx);
+          const float use = mn == -INFINITY ? 0.f : mn;
+          alpha[u][i] = ex2_approx(m[u][i] - use);  // m = -inf: 0
+          m[u][i] = mn;
+          l[u][i] *= alpha[u][i];
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const float e = ex2_approx(s[u][2 * x + i] - use);
+            l[u][i] += e;
+            s_p[(8 * u + 2 * t + i) * C::kPRow + key_g + 8 * x] = e;
+          }
+        }
+      }
+      __syncwarp();
+      // keys 8 step + 2t and + 1 are summed at places t and t + 4 of a step
+      float w_hi[2][G][2], w_lo[2][G][2];
+#pragma unroll
+      for (int step = 0; step < 2; ++step)
+#pragma unroll
+        for (int u = 0; u < G; ++u) {
+          const float2 w2 = *reinterpret_cast<const float2*>(s_p + (8 * u + g) * C::kPRow +
+                                                             8 * step + 2 * t);
+          split3x(w2.x, w_hi[step][u][0], w_lo[step][u][0]);
+          split3x(w2.y, w_hi[step][u][1], w_lo[step][u][1]);
+        }
+#pragma unroll
+      for (int h = 0; h < D / 64; ++h) {
+        float v[2][2][2][4];  // [step][key][columns 64 h + 32 e + 4 g ..]
+#pragma unroll
+        for (int step = 0; step < 2; ++step)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int k = key0 + 8 * step + 2 * t + x;
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              *reinterpret_cast<float4*>(v[step][x][e]) =
+                  *reinterpret_cast<const float4*>(sv + tile_at<D>(k, 64 * h + 32 * e + 4 * g));
+            if (tail) {
+              // rows past the end count for nothing, whatever they hold; what is not
+              // finite among the new tokens is left out here and added at the end
+              const int rel = tile * kTile + k - c.ctx;
+              if (rel >= 0) {
+                const bool past = tile * kTile + k >= c.keys;
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) {
+                    dirty |= !past && !isfinite(v[step][x][e][i]);
+                    if (past || !isfinite(v[step][x][e][i])) v[step][x][e][i] = 0.f;
+                  }
+              }
+            }
+          }
+        // four sums at once, so that products do not wait for one another
+        constexpr int kI = G >= 4 ? 1 : 4 / G;
+#pragma unroll
+        for (int i0 = 0; i0 < 4; i0 += kI) {
+          float part[kI][G][4] = {};
+#pragma unroll
+          for (int step = 0; step < 2; ++step) {
+            float a[kI][4], a_lo[kI][4];
+#pragma unroll
+            for (int i = 0; i < kI; ++i)
+#pragma unroll
+              for (int x = 0; x < 4; ++x)
+                split3x(v[step][x >> 1][x & 1][i0 + i], a[i][x], a_lo[i][x]);
+#pragma unroll
+            for (int i = 0; i < kI; ++i)
+#pragma unroll
+              for (int u = 0; u < G; ++u) mma_tf32(part[i][u], a_lo[i], w_hi[step][u]);
+#pragma unroll
+            for (int i = 0; i < kI; ++i)
+#pragma unroll
+              for (int u = 0; u < G; ++u) mma_tf32(part[i][u], a[i], w_lo[step][u]);
+#pragma unroll
+            for (int i = 0; i < kI; ++i)
+#pragma unroll
+              for (int u = 0; u < G; ++u) mma_tf32(part[i][u], a[i], w_hi[step][u]);
+          }
+#pragma unroll
+          for (int i = 0; i < kI; ++i)
+#pragma unroll
+            for (int u = 0; u < G; ++u)
+#pragma unroll
+              for (int x = 0; x < 4; ++x)
+                acc[u][4 * h + i0 + i][x] =
+                    fmaf(acc[u][4 * h + i0 + i][x], alpha[u][x & 1], part[i][u][x]);
+        }
+      }
+      __syncwarp();  // s_p and the stage have been read
+      if (lane == 0) mbar_arrive(blk.empty(stage));
+    }
+    if (!ok) break;
+
+    // join the key warps
+    if (dirty) blk.dirty()[w & 1] = w + 1;
+#pragma unroll
+    for (int u = 0; u < G; ++u) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[u][i] += __shfl_xor_sync(0xffffffffu, l[u][i], d);
+        if (g == 0) blk.ml(warp, 8 * u + 2 * t + i) = make_float2(m[u][i], l[u][i]);
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            *reinterpret_cast<float4*>(own + (8 * u + 2 * t + i) * D + 64 * h + 32 * e + 4 * g) =
+                make_float4(acc[u][4 * h][2 * e + i], acc[u][4 * h + 1][2 * e + i],
+                            acc[u][4 * h + 2][2 * e + i], acc[u][4 * h + 3][2 * e + i]);
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(blk.joined());
+    ok = __all_sync(0xffffffffu, mbar_wait(blk.joined(), w & 1, st, kSiteOReady, tmo));
+    if (!ok) break;
+    // four columns of a row at a time
+    for (int x = warp * 32 + lane; x < c.rows * (D / 4); x += kF32Warps * 32) {
+      const int r = x / (D / 4), x4 = x % (D / 4);
+      const int u0 = r / (8 * G) * kKeyWarps, r_w = r % (8 * G);
+      float top = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < kKeyWarps; ++u) top = fmaxf(top, blk.ml(u0 + u, r_w).x);
+      const float use = top == -INFINITY ? 0.f : top;
+      float sum = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int u = 0; u < kKeyWarps; ++u) {
+        const float2 ml = blk.ml(u0 + u, r_w);
+        const float f = ex2_approx(ml.x - use);
+        const float4 a =
+            *reinterpret_cast<const float4*>(blk.own(u0 + u) + r_w * D + x4 * 4);
+        sum += f * ml.y;
+        o.x += f * a.x;
+        o.y += f * a.y;
+        o.z += f * a.z;
+        o.w += f * a.w;
+      }
+      const int row = c.row0 + r, tok = row / p.group;
+      const int h = c.head_kv * p.group + row - tok * p.group;
+      const float inv = c.record >= 0 ? 1.f : (sum == 0.f ? 0.f : 1.f / sum);
+      // a record is [dim / 4][rows][4], the rows of the unit side by side
+      float* rec = c.record >= 0
+                       ? p.rec_acc + static_cast<int64_t>(c.record) * (kRows * D) + r * 4
+                       : nullptr;
+      float* out = static_cast<float*>(p.out) + static_cast<int64_t>(c.first + tok) * p.out_t +
+                   static_cast<int64_t>(h) * p.out_h;
+      o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+      *reinterpret_cast<float4*>(rec != nullptr ? rec + x4 * 4 * c.rows : out + x4 * 4) = o;
+      if (blk.dirty()[w & 1] == w + 1)
+        add_left_out(p, c, tok, kTile, x4 * 4, x4 * 4 + 4, D, rec, out);
+      if (x4 == 0) {
+        if (c.record >= 0) {
+          p.rec_m[c.record * kRows + r] = top;
+          p.rec_l[c.record * kRows + r] = sum;
+        } else if (p.lse != nullptr) {
+          p.lse[static_cast<int64_t>(c.first + tok) * p.heads + h] =
+              sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2f;
+        }
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(blk.item_empty(w));
+  }
+}
+
+template <int D, int kRows>
+__global__ void __launch_bounds__(F32Cfg<D, kRows>::kThreads, 1)
+    tree_f32_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap tmK,
+                     const __grid_constant__ CUtensorMap tmV) {
+  using C = F32Cfg<D, kRows>;
+  using namespace sm100;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const F32Block<C> blk{smem};
+  if ((smem_u32(smem) & 1023u) != 0) {  // the swizzle counts from 1024-byte boundaries
+    wait_for_predecessor();
+    if (threadIdx.x == 0) {
+      p.meta[blockIdx.x * kMetaInts] = 0;
+      st_record(p.status, kStatusBadArgs, kSiteNone);
+    }
+    return;
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::kStages; ++i) {
+      mbar_init(blk.full(i), 1);
+      mbar_init(blk.empty(i), kF32Warps);
+    }
+    for (int i = 0; i < kF32Items; ++i) {
+      mbar_init(blk.item_full(i), 1);
+      mbar_init(blk.item_empty(i), kF32Warps);
+    }
+    mbar_init(blk.joined(), kF32Warps);
+    mbar_init(blk.released(), kF32Warps);
+    blk.dirty()[0] = blk.dirty()[1] = 0;
+    fence_barrier_init();
+  }
+  let_successor_start();
+  __syncthreads();
+  wait_for_predecessor();
+
+  if (warp_id() >= kF32Warps) {
+    // the wide sums take 216 registers: 2 x 216 + 72 is the block's 3 x 168
+    if constexpr (C::kWide) warpgroup_reg_dec<72>();
+    if (warp_id() == kF32Warps) f32_walk<D, kRows>(p, tmK, tmV, blk);
+  } else if constexpr (C::kWide) {
+    warpgroup_reg_inc<216>();
+    f32_wide<D, kRows>(p, blk);
+  } else {
+    f32_narrow<D>(p, blk);
   }
 }
 
@@ -641,15 +1015,15 @@ __global__ void __launch_bounds__(kMergeThreads, 4)
   }
 }
 
-template <int D>
+template <int D, int kRows>
 int run_f32(const TreeParams& p, cudaStream_t stream) {
-  using C = F32Cfg<D>;
+  using C = F32Cfg<D, kRows>;
   static bool done[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !done[dev]) {
     const cudaError_t err = cudaFuncSetAttribute(
-        tree_f32_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+        tree_f32_kernel<D, kRows>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
     if (err != cudaSuccess) return static_cast<int>(err);
     if (dev >= 0 && dev < 64) done[dev] = true;
   }
@@ -663,8 +1037,15 @@ int run_f32(const TreeParams& p, cudaStream_t stream) {
     return make_tmap(base, TmapDtype::kF32, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
   };
   const CUtensorMap k = pool_map(p.k, p.k_page), v = pool_map(p.v, p.v_page);
-  return launch_overlapped(tree_f32_kernel<D>, dim3(p.grid), kF32Threads, C::kSmem, stream, &p,
+  return launch_overlapped(tree_f32_kernel<D, kRows>, dim3(p.grid), C::kThreads, C::kSmem, stream, &p,
                            &k, &v);
+}
+
+template <int D>
+int run_f32_rows(const TreeParams& p, int rows, cudaStream_t stream) {
+  return rows == 8    ? run_f32<D, 8>(p, stream)
+         : rows == 16 ? run_f32<D, 16>(p, stream)
+                      : run_f32<D, 32>(p, stream);
 }
 
 template <typename T, int D>
@@ -732,8 +1113,11 @@ __global__ void pack_mask_kernel(const uint8_t* in, int64_t in_t, int total, int
 TreePlan tree_plan(Elem elem, const TreeParams& p, int max_q, int sms) {
   TreePlan plan;
   if (elem == Elem::kF32) {
-    plan.rows_per_unit = kF32Rows;
-    plan.tile_keys = p.dim == 64 ? F32Cfg<64>::kTile : F32Cfg<128>::kTile;
+    // the least width that holds the rows: a wider one computes on empty rows, a
+    // narrower one reads and splits the cache again (times at the file's head)
+    const int64_t rows = static_cast<int64_t>(max_q) * p.group;
+    plan.rows_per_unit = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
+    plan.tile_keys = 8192 / p.dim;
   } else {
     // one row tile keeps two key tiles in the air per CTA and suits what reading
     // the cache bounds; from the second row tile on, both share every key tile
@@ -755,7 +1139,7 @@ int tree_launch(Elem elem, const TreeParams& p, const TreePlan& plan, cudaStream
   const int rows = plan.rows_per_unit;
   int err;
   if (elem == Elem::kF32)
-    err = p.dim == 64 ? run_f32<64>(p, stream) : run_f32<128>(p, stream);
+    err = p.dim == 64 ? run_f32_rows<64>(p, rows, stream) : run_f32_rows<128>(p, rows, stream);
   else
     err = tree_sm100_launch(elem, p, rows, stream);
   if (err != 0) return err;

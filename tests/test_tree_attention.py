@@ -200,6 +200,49 @@ def test_tree_values(ext, cuda_device, dtype, ctx, counts, H, Hk, D, page):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("rows", [8, 9, 15, 16, 17, 24, 32, 33])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_around_the_widths_of_a_unit(ext, cuda_device, dtype, rows, D):
+    """Row counts about the widths that units have, whole and in pieces, alone and beside shorter requests."""
+    for ctx, counts in (([5000], [rows]), ([70, 0, 300], [rows, 1, rows - 1])):
+        case = _case(ctx, counts, 2, 2, D, 32, dtype, seed=rows)
+        st = new_status("cuda")
+        out, lse = _run(*case, ctx, counts, status=st)
+        _check(out, lse, case, ctx, counts)
+        _, masks, seen, _ = _trees(counts, seed=rows)
+        out, lse = _run(*case, ctx, counts, mask=seen.cuda(), max_q=max(counts), status=st)
+        check_status(st)
+        _check(out, lse, case, ctx, counts, masks)
+        again, lse2 = _run(*case, ctx, counts, mask=seen.cuda(), max_q=max(counts), status=st)
+        assert torch.equal(out, again) and torch.equal(lse, lse2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("tokens, ctx", [(5, 37), (12, 130), (30, 4000)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_values_that_are_not_finite_reach_their_rows(ext, cuda_device, dtype, tokens, ctx, D):
+    """An infinite V of a new token is in the results of the rows that see it, and in no others."""
+    case = _case([ctx], [tokens], 1, 1, D, 16, dtype, seed=tokens)
+    q, kp, vp, table = case
+    j = ctx + 2
+    vp[table[0, j // 16], 0, j % 16, D - 3] = math.inf
+    mask = torch.ones(tokens, tokens, dtype=torch.bool).tril()
+    mask[4, 2] = False
+    out, lse = _run(*case, [ctx], [tokens], mask=mask.cuda())
+    sees = mask[:, 2]
+    out = out.cpu()
+    assert (out[sees, 0, D - 3] == math.inf).all() and torch.isfinite(out[~sees]).all()
+    clean = (q, kp, vp.nan_to_num(posinf=0.0), table)
+    ref, _, mag, smax = O.attention(*clean, [ctx], [tokens], [mask])
+    bo, _ = O.attention_bound(ref, mag, smax, dtype, ctx + tokens, D)
+    good = torch.ones(out.shape, dtype=torch.bool)
+    good[sees, 0, D - 3] = False
+    assert ((out.double() - ref).abs() <= bo)[good].all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_uniform_borders_scale_and_out(ext, cuda_device, dtype):
     ctx, counts = [40, 41, 7], [2, 2, 2]
