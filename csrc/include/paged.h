@@ -135,7 +135,9 @@ struct TreePlan {
 
 TreePlan tree_plan(Elem elem, const TreeParams& p, int max_q, int sms);
 int tree_launch(Elem elem, const TreeParams& p, const TreePlan& plan, cudaStream_t stream);
-// the tensor-core kernel of bf16 and fp16 (tree_launch calls it); 128 or 256 rows per unit
+// the kernels of bf16 and fp16 (tree_launch calls them): 8, 16 or 32 rows per unit, and
+// 128 or 256
+int tree_few_launch(Elem elem, const TreeParams& p, int rows_per_unit, cudaStream_t stream);
 int tree_sm100_launch(Elem elem, const TreeParams& p, int rows_per_unit, cudaStream_t stream);
 
 // ancestor bits and depths of drafted trees from parent indices

@@ -35,17 +35,7 @@
 // 3 trees over 4096 to 16384 keys, 8 heads x 64 (126 MB, 19 us at the copy rate): 32
 // us with the merge, against 39 us with the products on the CUDA cores, which issue
 // three times the instructions.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_runtime.h>
-
-#include <cstdint>
-
-#include "launch.h"
-#include "paged.h"
-#include "sm100.cuh"
-#include "tmap.h"
-#include "tree_sched.cuh"
+#include "tree_warp.cuh"
 
 namespace rab {
 
@@ -53,27 +43,9 @@ using namespace tree_detail;
 
 namespace {
 
-constexpr int kF32Warps = 8;   // that compute
-constexpr int kF32Items = 4;   // queue of pieces
-constexpr float kLn2f = 0.69314718055994530942f;
-
-template <typename T>
-__device__ __forceinline__ T cast_out(float x);
-template <>
-__device__ __forceinline__ float cast_out<float>(float x) {
-  return x;
-}
-template <>
-__device__ __forceinline__ __nv_bfloat16 cast_out<__nv_bfloat16>(float x) {
-  return __float2bfloat16_rn(x);
-}
-template <>
-__device__ __forceinline__ __half cast_out<__half>(float x) {
-  return __float2half_rn(x);
-}
-
-template <int D, int kRows>
+template <int D, int kRowsT>
 struct F32Cfg {
+  static constexpr int kD = D, kBytes = 4, kRows = kRowsT;
   static constexpr bool kWide = kRows > 8;
   // whole warpgroups where they pass registers to the computing warps
   static constexpr int kThreads = kWide ? 384 : 288;
@@ -83,20 +55,21 @@ struct F32Cfg {
   static constexpr int kStage = 2 * kHalf;
   // a warp's keys: 16, or 8 (half a product's height) with eight rows of dim 128; more
   // rows of dim 128 go to the two halves of the warps instead
-  static constexpr int kSplit = kWide ? kF32Warps * 16 / kTile : 1;
-  static constexpr int kKeys = kTile * kSplit / kF32Warps;
+  static constexpr int kSplit = kWide ? kWarps * 16 / kTile : 1;
+  static constexpr int kKeys = kTile * kSplit / kWarps;
   static constexpr int kGroups = kRows / 8 / kSplit;  // of eight rows, a warp's
   // floats of a warp: weights [row][key] in the tiles, [row][dim] outputs at a piece's end
+  static constexpr int kOwnRow = D;
   static constexpr int kOwn = kGroups * 8 * D;
   static constexpr int kPRow = kKeys + 4;  // between the weights of two rows
   static constexpr int kOwnOff = kStages * kStage;
   // split queries, [row / 8][dim / 16][hi, lo][lane] fragments; eight rows stay in registers
-  static constexpr int kQOff = kOwnOff + kF32Warps * kOwn * 4;
+  static constexpr int kQOff = kOwnOff + kWarps * kOwn * 4;
   static constexpr int kQGroup = D / 16 * 1024;  // bytes of eight rows
   static constexpr int kMlOff = kQOff + (kWide ? kRows / 8 * kQGroup : 0);  // float2 [warps][own rows]
-  static constexpr int kItemOff = kMlOff + kF32Warps * kGroups * 8 * 8;
-  static constexpr int kBarOff = kItemOff + kF32Items * 48;
-  static constexpr int kBars = 2 * kStages + 2 * kF32Items + 2;
+  static constexpr int kItemOff = kMlOff + kWarps * kGroups * 8 * 8;
+  static constexpr int kBarOff = kItemOff + kItems * 48;
+  static constexpr int kBars = 2 * kStages + 2 * kItems + 2;
   static constexpr int kDirtyOff = kBarOff + kBars * 8;  // int [2]
   static constexpr int kSmem = kDirtyOff + 8;
   static_assert(kSmem <= 232448 && kBarOff % 8 == 0, "shared memory");
@@ -140,151 +113,6 @@ __device__ __forceinline__ void mma_3x(float* c, float* c_lo, const float* a, co
   mma_tf32(c, a, b);
 }
 
-// Columns [k0, k1) of a result that this thread has just written take what was left
-// out of V among the new tokens of the piece, for the keys that token t sees.
-__device__ __noinline__ void add_left_out(const TreeParams& p, const Piece& c, int t, int tile, int k0,
-                                          int k1, int dim, float* rec, float* dst) {
-  const int* table = p.table + static_cast<int64_t>(c.request) * p.table_stride;
-  const int lo = max(c.ctx, c.tile_begin * tile), hi = min(c.keys, c.tile_end * tile);
-  for (int key = lo; key < hi; ++key) {
-    const int rel = key - c.ctx;
-    const bool sees =
-        p.mask == nullptr
-            ? rel <= t
-            : (rel >> 5) < p.mask_w &&
-                  ((p.mask[static_cast<int64_t>(c.first + t) * p.mask_stride + (rel >> 5)] >>
-                    (rel & 31)) &
-                   1u);
-    const int page = table[key >> p.page_shift];
-    if (!sees || page < 0 || page >= p.num_pages) continue;
-    const float* src = static_cast<const float*>(p.v) + page * p.v_page +
-                       (static_cast<int64_t>(c.head_kv) * p.page_size + (key & (p.page_size - 1))) * dim;
-    for (int k = k0; k < k1; ++k) {
-      if (isfinite(src[k])) continue;
-      if (rec != nullptr) rec[(k & ~3) * c.rows + (k & 3)] += src[k];
-      else dst[k] += src[k];
-    }
-  }
-}
-
-// the barriers and the queue of a block
-template <typename C>
-struct F32Block {
-  uint8_t* smem;
-  __device__ __forceinline__ uint64_t* bars() const {
-    return reinterpret_cast<uint64_t*>(smem + C::kBarOff);
-  }
-  __device__ __forceinline__ uint64_t* full(int i) const { return bars() + i; }
-  __device__ __forceinline__ uint64_t* empty(int i) const { return bars() + C::kStages + i; }
-  __device__ __forceinline__ uint64_t* item_full(int w) const {
-    return bars() + 2 * C::kStages + w % kF32Items;
-  }
-  __device__ __forceinline__ uint64_t* item_empty(int w) const {
-    return item_full(w) + kF32Items;
-  }
-  __device__ __forceinline__ uint64_t* joined() const {
-    return bars() + 2 * C::kStages + 2 * kF32Items;
-  }
-  __device__ __forceinline__ uint64_t* released() const { return joined() + 1; }
-  __device__ __forceinline__ Piece* item(int w) const {
-    return reinterpret_cast<Piece*>(smem + C::kItemOff + (w % kF32Items) * 48);
-  }
-  // [2], by the piece's parity
-  __device__ __forceinline__ volatile int* dirty() const {
-    return reinterpret_cast<int*>(smem + C::kDirtyOff);
-  }
-  __device__ __forceinline__ float* own(int warp) const {
-    return reinterpret_cast<float*>(smem + C::kOwnOff) + warp * C::kOwn;
-  }
-  // maximum and sum of row r of warp u
-  __device__ __forceinline__ float2& ml(int u, int r) const {
-    return reinterpret_cast<float2*>(smem + C::kMlOff)[u * (C::kGroups * 8) + r];
-  }
-};
-
-// One warp: walks the pieces and loads their tiles.
-template <int D, int kRows>
-__device__ __forceinline__ void f32_walk(const TreeParams& p, const CUtensorMap& tmK,
-                                         const CUtensorMap& tmV,
-                                         const F32Block<F32Cfg<D, kRows>>& blk) {
-  using C = F32Cfg<D, kRows>;
-  using namespace sm100;
-  constexpr int kTile = C::kTile;
-  const int lane = lane_id();
-  DeviceStatus* st = p.status;
-  const uint64_t tmo = p.timeout_ns;
-  if (lane == 0) {
-    tma_prefetch_desc(&tmK);
-    tma_prefetch_desc(&tmV);
-    p.meta[blockIdx.x * kMetaInts] = 0;
-  }
-  Range range;
-  Start first;
-  const int walker = find_range<kTile, kRows>(p, &range, &first);
-  Walk<kTile, kRows> walk;
-  if (lane == walker) walk.start(p, range, first);
-  const int rows_box = min(p.page_size, kTile);
-  const int boxes = kTile / rows_box * (D / 32);
-  int n = 0;  // tiles loaded
-  bool ok = true;
-  for (int w = 0; ok; ++w) {
-    if (w >= kF32Items)
-      ok = __all_sync(0xffffffffu, mbar_wait(blk.item_empty(w),
-                                             (w / kF32Items - 1) & 1, st, kSiteItemQueue, tmo));
-    if (!ok) break;
-    Piece* slot = blk.item(w);
-    if (lane == walker) {
-      Piece c;
-      if (walk.next(p, range, &c)) {
-        if (walk.merges) write_meta(p, c, true, walk.merge_c0);
-      } else {
-        c.request = -1;
-      }
-      *slot = c;
-    }
-    __syncwarp();
-    const Piece c = *slot;
-    if (lane == 0) mbar_arrive(blk.item_full(w));
-    if (c.request < 0) break;
-    const int* table = p.table + static_cast<int64_t>(c.request) * p.table_stride;
-    const int last_entry = (c.keys - 1) >> p.page_shift;
-    for (int tile = c.tile_begin; tile < c.tile_end; ++tile) {
-      // this lane's box: page, rows within the tile, 32-column segment
-      const int seg = lane % (D / 32), part = lane / (D / 32);
-      int page = p.num_pages, token = 0;
-      if (lane < boxes) {
-        const int key = tile * kTile + part * rows_box;
-        const int entry = key >> p.page_shift;
-        token = key & (p.page_size - 1);
-        if (entry <= last_entry) {  // behind it: a coordinate past the pool loads zeros
-          page = table[entry];
-          if (page < 0 || page >= p.num_pages) {
-            if (seg == 0) st_record(st, kStatusBadArgs, kBadPage, static_cast<uint32_t>(page));
-            page = p.num_pages;
-          }
-        }
-      }
-      const int stage = n % C::kStages;
-      ok = __all_sync(0xffffffffu, mbar_wait(blk.empty(stage), ((n / C::kStages) & 1) ^ 1, st,
-                                             kSiteKEmpty, tmo));
-      if (!ok) break;
-      if (lane == 0) mbar_arrive_expect_tx(blk.full(stage), C::kStage);
-      __syncwarp();
-      if (lane < boxes) {
-        uint8_t* dst = blk.smem + stage * C::kStage + seg * (kTile * 128) + part * rows_box * 128;
-        tma_load_4d(dst, &tmK, blk.full(stage), seg * 32, token, c.head_kv, page);
-        tma_load_4d(dst + C::kHalf, &tmV, blk.full(stage), seg * 32, token, c.head_kv, page);
-      }
-      ++n;
-    }
-  }
-  // the loads in flight land before the block gives its memory back
-  for (int i = 0; i < C::kStages && i < n; ++i) {
-    const int k = n - 1 - i;
-    mbar_wait(blk.full(k % C::kStages), (k / C::kStages) & 1, nullptr, kSiteKFull, 100000000ull);
-  }
-}
-
 // A computing warp, eight rows to a unit.
 // Fragments of a 16 x 8 x 8 product: lane = 4 g + t.  Scores: rows are keys, columns
 // query rows, the summed index is dim; this lane's sums are keys g and g + 8 (of the
@@ -292,7 +120,7 @@ __device__ __forceinline__ void f32_walk(const TreeParams& p, const CUtensorMap&
 // of V, the summed index is keys; this lane's are dims 32 h + 4 g + 0..3 of query rows
 // 2t and 2t + 1.
 template <int D>
-__device__ __forceinline__ void f32_narrow(const TreeParams& p, const F32Block<F32Cfg<D, 8>>& blk) {
+__device__ __forceinline__ void f32_narrow(const TreeParams& p, const WarpBlock<F32Cfg<D, 8>>& blk) {
   using C = F32Cfg<D, 8>;
   using namespace sm100;
   constexpr int kTile = C::kTile, kKeys = C::kKeys;
@@ -307,7 +135,7 @@ __device__ __forceinline__ void f32_narrow(const TreeParams& p, const F32Block<F
   int n = 0;  // tiles taken
   bool ok = true;
   for (int w = 0; ok; ++w) {
-    ok = __all_sync(0xffffffffu, mbar_wait(blk.item_full(w), (w / kF32Items) & 1, st,
+    ok = __all_sync(0xffffffffu, mbar_wait(blk.item_full(w), (w / kItems) & 1, st,
                                            kSiteItemQueue, tmo));
     if (!ok) break;
     const Piece c = *blk.item(w);
@@ -508,55 +336,7 @@ __device__ __forceinline__ void f32_narrow(const TreeParams& p, const F32Block<F
     if (lane == 0) mbar_arrive(blk.joined());
     ok = __all_sync(0xffffffffu, mbar_wait(blk.joined(), w & 1, st, kSiteOReady, tmo));
     if (!ok) break;
-    const float* all = blk.own(0);
-    // row `warp` of the eight, four columns at a time
-    if (warp < c.rows) {
-      const int r = warp;
-      float top = -INFINITY;
-#pragma unroll
-      for (int u = 0; u < kF32Warps; ++u) top = fmaxf(top, blk.ml(u, r).x);
-      const float use = top == -INFINITY ? 0.f : top;
-      float sum = 0.f, f[kF32Warps];
-#pragma unroll
-      for (int u = 0; u < kF32Warps; ++u) {
-        const float2 ml = blk.ml(u, r);
-        f[u] = ex2_approx(ml.x - use);
-        sum += f[u] * ml.y;
-      }
-      const int row = c.row0 + r, tok = row / p.group;
-      const int h = c.head_kv * p.group + row - tok * p.group;
-      const float inv = c.record >= 0 ? 1.f : (sum == 0.f ? 0.f : 1.f / sum);
-      // a record is [dim / 4][rows][4], the rows of the unit side by side
-      float* rec = c.record >= 0
-                       ? p.rec_acc + static_cast<int64_t>(c.record) * (8 * D) + r * 4
-                       : nullptr;
-      float* out = static_cast<float*>(p.out) + static_cast<int64_t>(c.first + tok) * p.out_t +
-                   static_cast<int64_t>(h) * p.out_h;
-      if (lane < D / 4) {
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int u = 0; u < kF32Warps; ++u) {
-          const float4 a = *reinterpret_cast<const float4*>(all + u * C::kOwn + r * D + lane * 4);
-          o.x += f[u] * a.x;
-          o.y += f[u] * a.y;
-          o.z += f[u] * a.z;
-          o.w += f[u] * a.w;
-        }
-        o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-        *reinterpret_cast<float4*>(rec != nullptr ? rec + lane * 4 * c.rows : out + lane * 4) = o;
-        if (blk.dirty()[w & 1] == w + 1)
-          add_left_out(p, c, tok, kTile, lane * 4, lane * 4 + 4, D, rec, out);
-      }
-      if (lane == 0) {
-        if (c.record >= 0) {
-          p.rec_m[c.record * 8 + r] = top;
-          p.rec_l[c.record * 8 + r] = sum;
-        } else if (p.lse != nullptr) {
-          p.lse[static_cast<int64_t>(c.first + tok) * p.heads + h] =
-              sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2f;
-        }
-      }
-    }
+    write_results<C, float>(p, blk, c, w);
     __syncwarp();
     if (lane == 0) {
       mbar_arrive(blk.released());
@@ -570,11 +350,11 @@ __device__ __forceinline__ void f32_narrow(const TreeParams& p, const F32Block<F
 // groups of the unit from (u / key warps) * kGroups on.
 template <int D, int kRows>
 __device__ __forceinline__ void f32_wide(const TreeParams& p,
-                                         const F32Block<F32Cfg<D, kRows>>& blk) {
+                                         const WarpBlock<F32Cfg<D, kRows>>& blk) {
   using C = F32Cfg<D, kRows>;
   using namespace sm100;
   constexpr int kTile = C::kTile, kKeys = C::kKeys, G = C::kGroups;
-  constexpr int kKeyWarps = kF32Warps / C::kSplit;
+  constexpr int kKeyWarps = kWarps / C::kSplit;
   const int warp = warp_id(), lane = lane_id();
   DeviceStatus* st = p.status;
   const uint64_t tmo = p.timeout_ns;
@@ -588,13 +368,13 @@ __device__ __forceinline__ void f32_wide(const TreeParams& p,
   bool ok = true;
   for (int w = 0; ok; ++w) {
     ok = __all_sync(0xffffffffu,
-                    mbar_wait(blk.item_full(w), (w / kF32Items) & 1, st, kSiteItemQueue, tmo));
+                    mbar_wait(blk.item_full(w), (w / kItems) & 1, st, kSiteItemQueue, tmo));
     if (!ok) break;
     const Piece c = *blk.item(w);
     if (c.request < 0) break;
     // The warps split the unit's queries, scaled to base-2 exponents: this one the 16
     // columns b of every eight rows.  Every warp has left the piece before (`joined`).
-    for (int b = warp; b < D / 16; b += kF32Warps) {
+    for (int b = warp; b < D / 16; b += kWarps) {
 #pragma unroll
       for (int u = 0; u < kRows / 8; ++u) {
         const int row = c.row0 + min(8 * u + g, c.rows - 1), tok = row / p.group;
@@ -822,51 +602,7 @@ __device__ __forceinline__ void f32_wide(const TreeParams& p,
     if (lane == 0) mbar_arrive(blk.joined());
     ok = __all_sync(0xffffffffu, mbar_wait(blk.joined(), w & 1, st, kSiteOReady, tmo));
     if (!ok) break;
-    // four columns of a row at a time
-    for (int x = warp * 32 + lane; x < c.rows * (D / 4); x += kF32Warps * 32) {
-      const int r = x / (D / 4), x4 = x % (D / 4);
-      const int u0 = r / (8 * G) * kKeyWarps, r_w = r % (8 * G);
-      float top = -INFINITY;
-#pragma unroll
-      for (int u = 0; u < kKeyWarps; ++u) top = fmaxf(top, blk.ml(u0 + u, r_w).x);
-      const float use = top == -INFINITY ? 0.f : top;
-      float sum = 0.f;
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int u = 0; u < kKeyWarps; ++u) {
-        const float2 ml = blk.ml(u0 + u, r_w);
-        const float f = ex2_approx(ml.x - use);
-        const float4 a =
-            *reinterpret_cast<const float4*>(blk.own(u0 + u) + r_w * D + x4 * 4);
-        sum += f * ml.y;
-        o.x += f * a.x;
-        o.y += f * a.y;
-        o.z += f * a.z;
-        o.w += f * a.w;
-      }
-      const int row = c.row0 + r, tok = row / p.group;
-      const int h = c.head_kv * p.group + row - tok * p.group;
-      const float inv = c.record >= 0 ? 1.f : (sum == 0.f ? 0.f : 1.f / sum);
-      // a record is [dim / 4][rows][4], the rows of the unit side by side
-      float* rec = c.record >= 0
-                       ? p.rec_acc + static_cast<int64_t>(c.record) * (kRows * D) + r * 4
-                       : nullptr;
-      float* out = static_cast<float*>(p.out) + static_cast<int64_t>(c.first + tok) * p.out_t +
-                   static_cast<int64_t>(h) * p.out_h;
-      o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-      *reinterpret_cast<float4*>(rec != nullptr ? rec + x4 * 4 * c.rows : out + x4 * 4) = o;
-      if (blk.dirty()[w & 1] == w + 1)
-        add_left_out(p, c, tok, kTile, x4 * 4, x4 * 4 + 4, D, rec, out);
-      if (x4 == 0) {
-        if (c.record >= 0) {
-          p.rec_m[c.record * kRows + r] = top;
-          p.rec_l[c.record * kRows + r] = sum;
-        } else if (p.lse != nullptr) {
-          p.lse[static_cast<int64_t>(c.first + tok) * p.heads + h] =
-              sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2f;
-        }
-      }
-    }
+    write_results<C, float>(p, blk, c, w);
     __syncwarp();
     if (lane == 0) mbar_arrive(blk.item_empty(w));
   }
@@ -879,37 +615,13 @@ __global__ void __launch_bounds__(F32Cfg<D, kRows>::kThreads, 1)
   using C = F32Cfg<D, kRows>;
   using namespace sm100;
   extern __shared__ __align__(1024) uint8_t smem[];
-  const F32Block<C> blk{smem};
-  if ((smem_u32(smem) & 1023u) != 0) {  // the swizzle counts from 1024-byte boundaries
-    wait_for_predecessor();
-    if (threadIdx.x == 0) {
-      p.meta[blockIdx.x * kMetaInts] = 0;
-      st_record(p.status, kStatusBadArgs, kSiteNone);
-    }
-    return;
-  }
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < C::kStages; ++i) {
-      mbar_init(blk.full(i), 1);
-      mbar_init(blk.empty(i), kF32Warps);
-    }
-    for (int i = 0; i < kF32Items; ++i) {
-      mbar_init(blk.item_full(i), 1);
-      mbar_init(blk.item_empty(i), kF32Warps);
-    }
-    mbar_init(blk.joined(), kF32Warps);
-    mbar_init(blk.released(), kF32Warps);
-    blk.dirty()[0] = blk.dirty()[1] = 0;
-    fence_barrier_init();
-  }
-  let_successor_start();
-  __syncthreads();
-  wait_for_predecessor();
+  const WarpBlock<C> blk{smem};
+  if (!start_block<C>(p, blk)) return;
 
-  if (warp_id() >= kF32Warps) {
+  if (warp_id() >= kWarps) {
     // the wide sums take 216 registers: 2 x 216 + 72 is the block's 3 x 168
     if constexpr (C::kWide) warpgroup_reg_dec<72>();
-    if (warp_id() == kF32Warps) f32_walk<D, kRows>(p, tmK, tmV, blk);
+    if (warp_id() == kWarps) walk_and_load<C>(p, tmK, tmV, blk);
   } else if constexpr (C::kWide) {
     warpgroup_reg_inc<216>();
     f32_wide<D, kRows>(p, blk);
@@ -1017,28 +729,8 @@ __global__ void __launch_bounds__(kMergeThreads, 4)
 
 template <int D, int kRows>
 int run_f32(const TreeParams& p, cudaStream_t stream) {
-  using C = F32Cfg<D, kRows>;
   static bool done[64] = {};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64 || !done[dev]) {
-    const cudaError_t err = cudaFuncSetAttribute(
-        tree_f32_kernel<D, kRows>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
-    if (err != cudaSuccess) return static_cast<int>(err);
-    if (dev >= 0 && dev < 64) done[dev] = true;
-  }
-  auto pool_map = [&](const void* base, int64_t page_stride) {
-    const uint64_t page = p.page_size;
-    uint64_t dims[4] = {D, page, static_cast<uint64_t>(p.heads_kv),
-                        static_cast<uint64_t>(p.num_pages)};
-    uint64_t strides[3] = {D * 4, page * D * 4, static_cast<uint64_t>(page_stride) * 4};
-    uint32_t box[4] = {32, static_cast<uint32_t>(p.page_size < C::kTile ? p.page_size : C::kTile),
-                       1, 1};
-    return make_tmap(base, TmapDtype::kF32, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
-  };
-  const CUtensorMap k = pool_map(p.k, p.k_page), v = pool_map(p.v, p.v_page);
-  return launch_overlapped(tree_f32_kernel<D, kRows>, dim3(p.grid), C::kThreads, C::kSmem, stream, &p,
-                           &k, &v);
+  return launch_warp_kernel<F32Cfg<D, kRows>>(tree_f32_kernel<D, kRows>, done, p, stream);
 }
 
 template <int D>
@@ -1112,25 +804,25 @@ __global__ void pack_mask_kernel(const uint8_t* in, int64_t in_t, int total, int
 
 TreePlan tree_plan(Elem elem, const TreeParams& p, int max_q, int sms) {
   TreePlan plan;
+  const int64_t rows = static_cast<int64_t>(max_q) * p.group;
   if (elem == Elem::kF32) {
     // the least width that holds the rows: a wider one computes on empty rows, a
     // narrower one reads and splits the cache again (times at the file's head)
-    const int64_t rows = static_cast<int64_t>(max_q) * p.group;
     plan.rows_per_unit = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
     plan.tile_keys = 8192 / p.dim;
   } else {
-    // one row tile keeps two key tiles in the air per CTA and suits what reading
-    // the cache bounds; from the second row tile on, both share every key tile
-    plan.rows_per_unit = static_cast<int64_t>(max_q) * p.group > 128 ? 256 : 128;
-    plan.tile_keys = 128;
+    // few rows: tree_few.cu (times at its head); above them, one row tile of the large
+    // tensor cores keeps two key tiles in the air per CTA and suits what reading the
+    // cache bounds, and from the second row tile on, both share every key tile
+    plan.rows_per_unit = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 128 ? 128 : 256;
+    plan.tile_keys = rows > 8 && rows <= 32 ? 64 : 128;
   }
   plan.grid = sms;
   // rows of the largest unit that can occur (max_q is a hint: the merge loops)
-  const int64_t most = static_cast<int64_t>(max_q) * p.group;
-  plan.merge_rows = static_cast<int>(most < plan.rows_per_unit ? most : plan.rows_per_unit);
-  const size_t rows = static_cast<size_t>(2) * plan.grid * plan.rows_per_unit;
-  plan.acc_floats = rows * p.dim;
-  plan.ml_floats = 2 * rows;
+  plan.merge_rows = static_cast<int>(rows < plan.rows_per_unit ? rows : plan.rows_per_unit);
+  const size_t recs = static_cast<size_t>(2) * plan.grid * plan.rows_per_unit;
+  plan.acc_floats = recs * p.dim;
+  plan.ml_floats = 2 * recs;
   plan.meta_ints = static_cast<size_t>(plan.grid) * kMetaInts;
   return plan;
 }
@@ -1140,6 +832,8 @@ int tree_launch(Elem elem, const TreeParams& p, const TreePlan& plan, cudaStream
   int err;
   if (elem == Elem::kF32)
     err = p.dim == 64 ? run_f32_rows<64>(p, rows, stream) : run_f32_rows<128>(p, rows, stream);
+  else if (rows <= 32)
+    err = tree_few_launch(elem, p, rows, stream);
   else
     err = tree_sm100_launch(elem, p, rows, stream);
   if (err != 0) return err;

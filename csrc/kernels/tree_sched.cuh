@@ -115,7 +115,8 @@ struct Start {
 // warps to it.  Every CTA reaches the same totals.  Returns the lane that holds the
 // range's first request (its `start` is the one filled in) and goes on to walk the
 // range.  A decoding step waits for this before its first load, so up to 32
-// requests take one read and one scan; more are read again to find the first.
+// requests take one read and one scan; more are shared out in runs, and the run that
+// holds the first is read again.
 template <int kTile, int kRows>
 __device__ __forceinline__ int find_range(const TreeParams& p, Range* range, Start* start) {
   const int lane = threadIdx.x & 31;
@@ -138,14 +139,17 @@ __device__ __forceinline__ int find_range(const TreeParams& p, Range* range, Sta
     }
     return v;
   };
+  // a lane's requests lie side by side: the second reading is of one lane's only
+  const int per = (p.batch + 31) >> 5, mine_0 = lane * per;
   int mine = 0, inc;
-  if (p.batch <= 32) {
+  if (per == 1) {
     mine = places(lane);
     inc = scan(mine);
   } else {
     int sum = 0;
 #pragma unroll 4
-    for (int b = lane; b < p.batch; b += 32) sum += places(b);
+    for (int b = mine_0; b < mine_0 + per; ++b) sum += places(b);
+    mine = sum;
     inc = scan(sum);
   }
   g.total = __shfl_sync(0xffffffffu, inc, 31);
@@ -158,12 +162,16 @@ __device__ __forceinline__ int find_range(const TreeParams& p, Range* range, Sta
   *range = g;
   if (g.begin >= g.end) return 0;
   int before = 0;
-  for (int b0 = 0; p.batch > 32; b0 += 32) {  // ends: the range begins below the total
-    mine = places(b0 + lane);
-    inc = scan(mine);
-    const int all = __shfl_sync(0xffffffffu, inc, 31);
-    if (g.begin < before + all) break;
-    before += all;
+  if (per > 1) {
+    const int in = __ffs(__ballot_sync(0xffffffffu, g.begin < inc)) - 1;
+    before = __shfl_sync(0xffffffffu, inc - mine, in);
+    for (int b0 = in * per;; b0 += 32) {  // ends: the range begins below the total
+      mine = places(b0 + lane);
+      inc = scan(mine);
+      const int all = __shfl_sync(0xffffffffu, inc, 31);
+      if (g.begin < before + all) break;
+      before += all;
+    }
   }
   start->at = before + inc - mine;
   return __ffs(__ballot_sync(0xffffffffu, g.begin < before + inc)) - 1;
