@@ -135,8 +135,8 @@ struct TreePlan {
 
 TreePlan tree_plan(Elem elem, const TreeParams& p, int max_q, int sms);
 int tree_launch(Elem elem, const TreeParams& p, const TreePlan& plan, cudaStream_t stream);
-// the kernels of bf16 and fp16 (tree_launch calls them): 8, 16 or 32 rows per unit, and
-// 128 or 256
+// the kernels of bf16 and fp16 (tree_launch calls them): 8 or 16 rows per unit, and 128
+// or 256
 int tree_few_launch(Elem elem, const TreeParams& p, int rows_per_unit, cudaStream_t stream);
 int tree_sm100_launch(Elem elem, const TreeParams& p, int rows_per_unit, cudaStream_t stream);
 

@@ -179,6 +179,12 @@ __device__ __forceinline__ void f32_narrow(const TreeParams& p, const WarpBlock<
       ok = __all_sync(0xffffffffu, mbar_wait(blk.full(stage), (n / C::kStages) & 1, st, kSiteKFull,
                                              tmo));
       if (!ok) break;
+      const int j0 = tile * kTile + warp * kKeys;
+      if (j0 >= c.keys) {  // no key for this warp
+        if (lane == 0) mbar_arrive(blk.empty(stage));
+        continue;
+      }
+      const bool tail = j0 + kKeys > c.ctx;  // this warp has new tokens, or keys past the end
       const uint8_t* sk = blk.smem + stage * C::kStage;
       const uint8_t* sv = sk + C::kHalf;
       // even and odd steps are summed apart, so that products do not wait for one
@@ -213,8 +219,6 @@ __device__ __forceinline__ void f32_narrow(const TreeParams& p, const WarpBlock<
 #pragma unroll
         for (int i = 0; i < 2; ++i)
           s[u][i] = s2[0][2 * u + i] + s2[1][2 * u + i] + s_lo[2 * u + i];
-      const int j0 = tile * kTile + warp * kKeys;
-      const bool tail = (tile + 1) * kTile > c.ctx;  // new tokens, or past the end
       if (tail) {
 #pragma unroll
         for (int u = 0; u < kMine; ++u) {
@@ -419,6 +423,12 @@ __device__ __forceinline__ void f32_wide(const TreeParams& p,
       ok = __all_sync(0xffffffffu, mbar_wait(blk.full(stage), (n / C::kStages) & 1, st,
                                              kSiteKFull, tmo));
       if (!ok) break;
+      const int j0 = tile * kTile + key0;
+      if (j0 >= c.keys) {  // no key for this warp
+        if (lane == 0) mbar_arrive(blk.empty(stage));
+        continue;
+      }
+      const bool tail = j0 + kKeys > c.ctx;  // this warp has new tokens, or keys past the end
       const uint8_t* sk = blk.smem + stage * C::kStage;
       const uint8_t* sv = sk + C::kHalf;
       const float4* sq =
@@ -452,8 +462,6 @@ __device__ __forceinline__ void f32_wide(const TreeParams& p,
           for (int u = 0; u < G; ++u) mma_tf32(s_lo[u], k_hi[e], e == 0 ? &lo[u].x : &lo[u].z);
         }
       }
-      const int j0 = tile * kTile + key0;
-      const bool tail = (tile + 1) * kTile > c.ctx;  // new tokens, or past the end
       float alpha[G][2];
 #pragma unroll
       for (int u = 0; u < G; ++u) {
@@ -814,8 +822,8 @@ TreePlan tree_plan(Elem elem, const TreeParams& p, int max_q, int sms) {
     // few rows: tree_few.cu (times at its head); above them, one row tile of the large
     // tensor cores keeps two key tiles in the air per CTA and suits what reading the
     // cache bounds, and from the second row tile on, both share every key tile
-    plan.rows_per_unit = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 128 ? 128 : 256;
-    plan.tile_keys = rows > 8 && rows <= 32 ? 64 : 128;
+    plan.rows_per_unit = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 128 ? 128 : 256;
+    plan.tile_keys = 128;
   }
   plan.grid = sms;
   // rows of the largest unit that can occur (max_q is a hint: the merge loops)
@@ -832,7 +840,7 @@ int tree_launch(Elem elem, const TreeParams& p, const TreePlan& plan, cudaStream
   int err;
   if (elem == Elem::kF32)
     err = p.dim == 64 ? run_f32_rows<64>(p, rows, stream) : run_f32_rows<128>(p, rows, stream);
-  else if (rows <= 32)
+  else if (rows <= 16)
     err = tree_few_launch(elem, p, rows, stream);
   else
     err = tree_sm100_launch(elem, p, rows, stream);

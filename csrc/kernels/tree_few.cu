@@ -1,10 +1,21 @@
 // tree_few.cu - attention of new tokens over a paged cache in bf16 and fp16 for up to
-// 32 rows per kv head: decoding steps and small trees (tree_sm100.cu takes more).
+// 16 rows per kv head: decoding steps and small trees (tree_sm100.cu takes more).
 //
-// Reading the cache bounds this work, so products on the small tensor instructions are
-// enough, and they save what the large ones cost a short piece: their scores, weights
-// and outputs pass between warps through TMEM, one tile after the other.  Here a warp
-// keeps its rows' maximum, sum and outputs in registers from the scores to the result.
+// The mathematics is tree_f32.cu's; weights are rounded to the element type for their
+// product with V and summed unrounded.  Reading the cache bounds this work, so products
+// on the small tensor instructions are enough, and they save what the large ones cost a
+// short piece: their scores, weights and outputs pass between warps through TMEM, one
+// tile after the other (a piece of one tile: 9200 cycles, here 5500).  A warp keeps its
+// rows' maximum, sum and outputs in registers from the scores to the result.
+//
+// us here and with tree_sm100.cu, 8 kv heads:
+//   rows, dim     4 x 32000     64 x 100-3000   24 x 10-300   1 x 300
+//    8,  64      50.8 / 64.9    44.5 / 74.4     14 / 17       10 / 14
+//   16,  64      54.1 / 64.6    51.5 / 74.4     12 / 17       14 / 13
+//    8, 128      87.3 / 89.8    75.5 / 84.9     13 / 18       10 / 14
+//   16, 128      89.4 / 90.2    77.2 / 85.6     15 / 18       12 / 14
+// (floors 40 / 31 us of bytes at dim 64, 80 / 62 at dim 128).  32 rows in this form are
+// bound by the products: 68 / 65 and 115 / 91 us over 4 x 32000.
 //
 // Products are 16 x 8 x 16.  Scores: rows are keys, columns query rows, the sum runs
 // over dim.  Outputs: rows are columns of V, the sum runs over keys; the weights leave
@@ -25,13 +36,14 @@ namespace {
 
 template <int D, int kRowsT>
 struct FewCfg {
+  static_assert(kRowsT == 8 || kRowsT == 16, "rows of a unit");
   static constexpr int kD = D, kBytes = 2, kRows = kRowsT;
   static constexpr int kThreads = 288;
-  // sixteen keys to a warp; with more than eight rows the two halves of the warps take
-  // the two halves of the rows
+  // with more than eight rows the two halves of the warps take the two halves of the rows
   static constexpr int kSplit = kRows > 8 ? 2 : 1;
   static constexpr int kGroups = kRows / 8 / kSplit;
-  static constexpr int kTile = 16 * kWarps / kSplit;
+  static constexpr int kTile = 128;  // 64 with 16 rows: 61 instead of 53 us at dim 64
+  static constexpr int kBlocks = kTile * kSplit / (16 * kWarps);  // of sixteen keys, a warp's
   static constexpr int kHalf = kTile * D * 2;
   static constexpr int kStage = 2 * kHalf;
   static constexpr int kOwnRow = D + 4;  // rows 2t and 2t + 1 of four lanes: no bank twice
@@ -109,13 +121,13 @@ __device__ __forceinline__ void few_compute(const TreeParams& p,
   using C = FewCfg<D, kRows>;
   using H = Half<T>;
   using namespace sm100;
-  constexpr int kTile = C::kTile, G = C::kGroups;
+  constexpr int kTile = C::kTile, G = C::kGroups, KB = C::kBlocks;
   constexpr int kKeyWarps = kWarps / C::kSplit;
   const int warp = warp_id(), lane = lane_id();
   DeviceStatus* st = p.status;
   const uint64_t tmo = p.timeout_ns;
   const int g = lane >> 2, t = lane & 3;
-  const int key0 = warp % kKeyWarps * 16;        // this warp's first key of a tile
+  const int key0 = warp % kKeyWarps * (16 * KB);        // this warp's first key of a tile
   const int row_w = warp / kKeyWarps * (8 * G);  // and its first row of the unit
   float* own = blk.own(warp);
   // where this lane points for K (keys 0-7, 8-15, then the next 8 columns) and V (keys
@@ -131,6 +143,7 @@ __device__ __forceinline__ void few_compute(const TreeParams& p,
   }
 
   uint32_t q[G][D / 16][2];  // columns 16 b + 2t, + 1 and + 8, + 9 of row g of a group
+  int tok_g[G];              // that row's token
   Piece c;
   // waits for piece w and asks for its queries, which are due at its first product
   auto fetch = [&](int w) -> bool {
@@ -142,6 +155,7 @@ __device__ __forceinline__ void few_compute(const TreeParams& p,
 #pragma unroll
     for (int u = 0; u < G; ++u) {
       const int row = c.row0 + min(row_w + 8 * u + g, c.rows - 1), tok = row / p.group;
+      tok_g[u] = tok;
       const int h = c.head_kv * p.group + row - tok * p.group;
       const uint32_t* src = reinterpret_cast<const uint32_t*>(
           static_cast<const T*>(p.q) + static_cast<int64_t>(c.first + tok) * p.q_t +
@@ -179,51 +193,60 @@ __device__ __forceinline__ void few_compute(const TreeParams& p,
       ok = __all_sync(0xffffffffu, mbar_wait(blk.full(stage), (n / C::kStages) & 1, st,
                                              kSiteKFull, tmo));
       if (!ok) break;
-      // even and odd steps are summed apart, so that products do not wait for one another
-      float s2[2][G][4] = {};
-#pragma unroll
-      for (int b = 0; b < D / 16; ++b) {
-        uint32_t a[4];
-        ldsm4(a, k_at + stage * C::kStage + (b >> 2) * (kTile * 128) + k_col[b & 3]);
-#pragma unroll
-        for (int u = 0; u < G; ++u) H::mma(s2[b & 1][u], a, q[u][b]);
-      }
       const int j0 = tile * kTile + key0;
-      const bool tail = (tile + 1) * kTile > c.ctx;  // new tokens, or past the end
-      uint32_t wt[G][2];  // weights of keys 2t, 2t + 1 and + 8, + 9 for row g
+      if (j0 >= c.keys) {  // no key for this warp
+        if (lane == 0) mbar_arrive(blk.empty(stage));
+        continue;
+      }
+      const bool tail = j0 + 16 * KB > c.ctx;  // this warp has new tokens, or keys past the end
+      // even and odd steps are summed apart, so that products do not wait for one another
+      float s2[2][KB][G][4] = {};
+#pragma unroll
+      for (int b = 0; b < D / 16; ++b)
+#pragma unroll
+        for (int y = 0; y < KB; ++y) {
+          uint32_t a[4];
+          ldsm4(a, k_at + stage * C::kStage + y * 2048 + (b >> 2) * (kTile * 128) + k_col[b & 3]);
+#pragma unroll
+          for (int u = 0; u < G; ++u) H::mma(s2[b & 1][y][u], a, q[u][b]);
+        }
+      uint32_t wt[G][KB][2];  // weights of keys 2t, 2t + 1 and + 8, + 9 for row g
       float alpha[G][2];
       bool moved = false;
 #pragma unroll
       for (int u = 0; u < G; ++u) {
-        float s[4];  // [2 (key / 8) + row]
+        float s[2 * KB][2];  // keys g + 8 x, rows 2t + i
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[i] = (s2[0][u][i] + s2[1][u][i]) * p.scale_log2;
+        for (int x = 0; x < 2 * KB; ++x)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int at = 2 * (x & 1) + i;
+            s[x][i] = (s2[0][x >> 1][u][at] + s2[1][x >> 1][u][at]) * p.scale_log2;
+          }
         if (tail) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const int r = row_w + 8 * u + 2 * t + i;
-            const int tok = (c.row0 + r) / p.group;
+            const int tok = __shfl_sync(0xffffffffu, tok_g[u], 4 * (2 * t + i));
+            const bool row = row_w + 8 * u + 2 * t + i < c.rows;
+            const uint32_t* words =
+                p.mask + static_cast<int64_t>(c.first + tok) * p.mask_stride;
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
+            for (int x = 0; x < 2 * KB; ++x) {
               const int j = j0 + g + 8 * x, rel = j - c.ctx;
-              if (rel < 0) continue;
-              bool sees = j < c.keys && r < c.rows;
-              if (sees)
-                sees = p.mask == nullptr
-                           ? rel <= tok
-                           : (rel >> 5) < p.mask_w &&
-                                 ((p.mask[static_cast<int64_t>(c.first + tok) * p.mask_stride +
-                                          (rel >> 5)] >>
-                                   (rel & 31)) &
-                                  1u);
-              if (!sees) s[2 * x + i] = -INFINITY;
+              bool sees = row && j < c.keys;
+              if (p.mask == nullptr)
+                sees &= rel <= tok;
+              else if (sees && rel >= 0)
+                sees = (rel >> 5) < p.mask_w && ((words[rel >> 5] >> (rel & 31)) & 1u);
+              if (!sees) s[x][i] = -INFINITY;
             }
           }
         }
-        float e[4];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float mx = fmaxf(s[i], s[2 + i]);
+          float mx = s[0][i];
+#pragma unroll
+          for (int x = 1; x < 2 * KB; ++x) mx = fmaxf(mx, s[x][i]);
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
           const float mn = fmaxf(m[u][i], mx);
@@ -231,12 +254,17 @@ __device__ __forceinline__ void few_compute(const TreeParams& p,
           alpha[u][i] = ex2_approx(m[u][i] - use);  // m = -inf: 0
           moved |= mn != m[u][i];
           m[u][i] = mn;
-          e[i] = ex2_approx(s[i] - use);
-          e[2 + i] = ex2_approx(s[2 + i] - use);
-          l[u][i] = l[u][i] * alpha[u][i] + (e[i] + e[2 + i]);  // the weights unrounded
+          float sum = 0.f;  // of the weights unrounded
+#pragma unroll
+          for (int x = 0; x < 2 * KB; ++x) {
+            s[x][i] = ex2_approx(s[x][i] - use);
+            sum += s[x][i];
+          }
+          l[u][i] = l[u][i] * alpha[u][i] + sum;
         }
-        wt[u][0] = transpose8(H::pack(e[0], e[1]));
-        wt[u][1] = transpose8(H::pack(e[2], e[3]));
+#pragma unroll
+        for (int x = 0; x < 2 * KB; ++x)
+          wt[u][x >> 1][x & 1] = transpose8(H::pack(s[x][0], s[x][1]));
       }
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
@@ -247,28 +275,40 @@ __device__ __forceinline__ void few_compute(const TreeParams& p,
             for (int i = 0; i < 4; ++i) acc[u][b][i] *= alpha[u][i & 1];
       }
 #pragma unroll
-      for (int b = 0; b < D / 16; ++b) {
-        uint32_t a[4];  // columns g and g + 8 of keys 2t, 2t + 1, then of keys 8 later
-        ldsm4_t(a, v_at + stage * C::kStage + (b >> 2) * (kTile * 128) + v_col[b & 3]);
-        if (tail) {
-          // rows past the end count for nothing, whatever they hold; what is not finite
-          // among the new tokens is left out here and added at the end
+      for (int y = 0; y < KB; ++y) {
+        const int jb = j0 + 16 * y;
+        const bool clean = jb + 16 > c.ctx;
+        // Rows past the end count for nothing, whatever they hold; what is not finite
+        // among the new tokens is left out here and added at the end.  By halves of a
+        // register, keys 2t and 2t + 1, and + 8 in the second:
+        uint32_t keep[2] = {0xffffffffu, 0xffffffffu}, fresh[2] = {};
+        if (clean) {
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
-#pragma unroll
-            for (int hlf = 0; hlf < 2; ++hlf) {
-              const int j = j0 + 8 * (x >> 1) + 2 * t + hlf;
-              const uint32_t bits = hlf ? 0xffff0000u : 0x0000ffffu;
-              const uint32_t ex = hlf ? H::kExp << 16 : H::kExp;
-              const bool past = j >= c.keys, bad = (a[x] & ex) == ex;
-              if (j >= c.ctx && (past || bad)) {
-                dirty |= !past;
-                a[x] &= ~bits;
-              }
-            }
+          for (int x = 0; x < 4; ++x) {
+            const int j = jb + 8 * (x >> 1) + 2 * t + (x & 1);
+            const uint32_t bits = x & 1 ? 0xffff0000u : 0x0000ffffu;
+            if (j >= c.keys) keep[x >> 1] &= ~bits;
+            if (j >= c.ctx) fresh[x >> 1] |= bits & (H::kExp * 0x10001u);
+          }
         }
 #pragma unroll
-        for (int u = 0; u < G; ++u) H::mma(acc[u][b], a, wt[u]);
+        for (int b = 0; b < D / 16; ++b) {
+          uint32_t a[4];  // columns g and g + 8 of keys 2t, 2t + 1, then of keys 8 later
+          ldsm4_t(a, v_at + stage * C::kStage + y * 2048 + (b >> 2) * (kTile * 128) + v_col[b & 3]);
+          if (clean) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              a[x] &= keep[x >> 1];
+              // an exponent of ones and its lowest bit carry into the sign's place
+              const uint32_t hit =
+                  ((a[x] & fresh[x >> 1]) + (H::kExp & -H::kExp) * 0x10001u) & 0x80008000u;
+              a[x] &= ~((hit >> 15) * 0xffffu);
+              dirty |= hit != 0u;
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < G; ++u) H::mma(acc[u][b], a, wt[u][y]);
+        }
       }
       __syncwarp();  // the stage has been read
       if (lane == 0) mbar_arrive(blk.empty(stage));
@@ -332,9 +372,7 @@ int run(const TreeParams& p, cudaStream_t stream) {
 
 template <typename T, int D>
 int run_rows(const TreeParams& p, int rows, cudaStream_t stream) {
-  return rows == 8    ? run<T, D, 8>(p, stream)
-         : rows == 16 ? run<T, D, 16>(p, stream)
-                      : run<T, D, 32>(p, stream);
+  return rows == 8 ? run<T, D, 8>(p, stream) : run<T, D, 16>(p, stream);
 }
 
 }  // namespace

@@ -2,8 +2,9 @@
 // cores (bf16 and fp16), for B200 (sm_100a).
 //
 // The rows of a unit are the (new token, query head) pairs that share a kv head,
-// token-major, so a decoding step of 8 query heads fills 8 of the 128 rows of an
-// MMA and K and V are still read once for all of them.  Up to 128 rows the work is
+// token-major, and K and V are read once for all of them (up to 16 rows are
+// tree_few.cu's, unless the caller's longest request was a wrong hint).  Up to 128 rows
+// the work is
 // bound by reading the cache; a tile of 128 keys (64 KB at dim 128) takes an SM
 // about 1.5 us at the measured 6.55 TB/s, while QK, softmax and PV of the tile
 // follow one another and take longer than that in a row.  So two chains run side
