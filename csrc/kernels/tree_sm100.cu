@@ -2,10 +2,9 @@
 // cores (bf16 and fp16), for B200 (sm_100a).
 //
 // The rows of a unit are the (new token, query head) pairs that share a kv head,
-// token-major, and K and V are read once for all of them (up to 16 rows are
-// tree_few.cu's, unless the caller's longest request was a wrong hint).  Up to 128 rows
-// the work is
-// bound by reading the cache; a tile of 128 keys (64 KB at dim 128) takes an SM
+// token-major, and K and V are read once for all of them (calls of up to 16 rows are
+// tree_few.cu's).  Up to 128 rows the work is bound by reading the cache; a tile of 128
+// keys (64 KB at dim 128) takes an SM
 // about 1.5 us at the measured 6.55 TB/s, while QK, softmax and PV of the tile
 // follow one another and take longer than that in a row.  So two chains run side
 // by side in one CTA:
@@ -475,22 +474,36 @@ __global__ void __launch_bounds__(kThreads, 1)
         // Rows behind the unit's last are zeros: an MMA row is its own, but products of
         // zeros draw less power, which bounds the clock (32 trees, row tiles 58 % full:
         // 1455 instead of 1402 MHz and 318 instead of 323 us at the 1000 W cap).
-        constexpr int kChunks = D / 8;
-        const uint32_t qb = smem_u32(sQ);
-        const int h0 = c.head_kv * p.group;
-        for (int i = tid; i < max(c.rows, filled) * kChunks; i += 64) {
-          const int r = i / kChunks, x = i % kChunks;
-          const uint32_t at = qb + (r / kM) * (kM * D * 2) + (x / 8) * (kM * 128) +
-                              (r % kM) * 128 + (((x % 8) ^ (r & 7)) << 4);
-          if (r >= c.rows) {
-            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
-            continue;
+        // A thread copies one 16-byte column of every kStep-th row; token and head move on
+        // by additions (a division per copy held the first scores up by 5 us).
+        constexpr int kChunks = D / 8, kStep = 64 / kChunks;
+        const int x = tid % kChunks;
+        const uint32_t qb = smem_u32(sQ) + (x / 8) * (kM * 128);
+        auto place = [&](int r) {
+          return qb + (r / kM) * (kM * D * 2) + (r % kM) * 128 + (((x % 8) ^ (r & 7)) << 4);
+        };
+        const int dt = kStep / p.group, dh = kStep - dt * p.group;
+        int r = tid / kChunks;
+        const int t0 = (c.row0 + r) / p.group;
+        int h = c.row0 + r - t0 * p.group;
+        const uint16_t* src = static_cast<const uint16_t*>(p.q) +
+                              static_cast<int64_t>(c.first + t0) * p.q_t +
+                              static_cast<int64_t>(c.head_kv * p.group + h) * p.q_h + x * 8;
+        const int64_t step = dt * p.q_t + dh * p.q_h, wrap = p.q_t - p.group * p.q_h;
+#pragma unroll 4
+        for (; r < c.rows; r += kStep) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(place(r)), "l"(src)
+                       : "memory");
+          src += step;
+          h += dh;
+          if (h >= p.group) {
+            h -= p.group;
+            src += wrap;
           }
-          const int row = c.row0 + r, t = row / p.group, h = h0 + row - t * p.group;
-          const uint16_t* src = static_cast<const uint16_t*>(p.q) +
-                                static_cast<int64_t>(c.first + t) * p.q_t + h * p.q_h + x * 8;
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(src) : "memory");
         }
+        for (; r < filled; r += kStep)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(place(r)), "r"(0)
+                       : "memory");
         filled = c.rows;
         asm volatile("cp.async.wait_all;" ::: "memory");
         fence_proxy_async_smem();
