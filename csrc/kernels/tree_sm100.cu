@@ -541,6 +541,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m_run = -INFINITY, l_run = 0.f;
       for (int j = kTwoRows ? 0 : x; j < n; j += kTwoRows ? 1 : 2) {
         const bool tail = (j + 1) * kN > old_keys;
+        uint32_t bits[4];  // seen columns, looked up while the scores form
+        if (tail && active) {
+          const int token = min(c->row0 + r, c->row0 + c->rows - 1) / p.group;
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            bits[q] = seen_bits(p, c, token, j * kN + 32 * q - old_keys);
+        }
         ok = __all_sync(0xffffffffu, mbar_wait(&s_full[x], sx & 1, st, kSiteSFull, tmo));
         if (!ok) break;
         ++sx;
@@ -556,13 +563,13 @@ __global__ void __launch_bounds__(kThreads, 1)
               sr[k] = __float_as_uint(__uint_as_float(sr[k]) * p.scale_log2);
           }
           if (tail) {
-            const int token = min(c->row0 + r, c->row0 + c->rows - 1) / p.group;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-              const uint32_t bits = seen_bits(p, c, token, j * kN + 32 * q - old_keys);
+              // past over where every row sees all: this code is long and seldom run
+              if (__all_sync(0xffffffffu, bits[q] == 0xffffffffu)) continue;
 #pragma unroll
               for (int k = 0; k < 32; ++k)
-                if (!((bits >> k) & 1u)) sr[32 * q + k] = 0xff800000u;  // -inf
+                if (!((bits[q] >> k) & 1u)) sr[32 * q + k] = 0xff800000u;  // -inf
             }
           }
           float pm[8];
