@@ -39,7 +39,6 @@
 #include "launch.h"
 #include "paged.h"
 #include "sm100.cuh"
-#include "tmap.h"
 #include "tree_sched.cuh"
 
 namespace rab {
@@ -781,20 +780,10 @@ int launch(const TreeParams& p, const CUtensorMap& k, const CUtensorMap& v, cuda
                            stream, &p, &k, &v);
 }
 
-CUtensorMap pool_map(const TreeParams& p, const void* base, int64_t page_stride) {
-  const uint64_t d = p.dim, page = p.page_size;
-  uint64_t dims[4] = {d, page, static_cast<uint64_t>(p.heads_kv),
-                      static_cast<uint64_t>(p.num_pages)};
-  uint64_t strides[3] = {d * 2, page * d * 2, static_cast<uint64_t>(page_stride) * 2};
-  uint32_t box[4] = {64, static_cast<uint32_t>(p.page_size < kN ? p.page_size : kN), 1, 1};
-  // 16-bit elements are copied, not read, so one type serves bf16 and fp16
-  return make_tmap(base, TmapDtype::kBF16, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
-}
-
 }  // namespace
 
 int tree_sm100_launch(Elem elem, const TreeParams& p, int rows_per_unit, cudaStream_t stream) {
-  const CUtensorMap k = pool_map(p, p.k, p.k_page), v = pool_map(p, p.v, p.v_page);
+  const CUtensorMap k = pool_map(p, p.k, p.k_page, 2, kN), v = pool_map(p, p.v, p.v_page, 2, kN);
   const bool two = rows_per_unit == 256;
   if (elem == Elem::kBF16) {
     if (p.dim == 64)

@@ -21,7 +21,6 @@
 #include "launch.h"
 #include "paged.h"
 #include "sm100.cuh"
-#include "tmap.h"
 #include "tree_sched.cuh"
 
 namespace rab {
@@ -291,20 +290,6 @@ __device__ __forceinline__ void write_results(const TreeParams& p, const WarpBlo
       }
     }
   }
-}
-
-// a pool's tiles: boxes of 128 bytes of columns and a page's rows, at most a tile's
-inline CUtensorMap pool_map(const TreeParams& p, const void* base, int64_t page_stride, int bytes,
-                            int tile) {
-  const uint64_t d = p.dim, page = p.page_size;
-  uint64_t dims[4] = {d, page, static_cast<uint64_t>(p.heads_kv),
-                      static_cast<uint64_t>(p.num_pages)};
-  uint64_t strides[3] = {d * bytes, page * d * bytes, static_cast<uint64_t>(page_stride) * bytes};
-  uint32_t box[4] = {static_cast<uint32_t>(128 / bytes),
-                     static_cast<uint32_t>(p.page_size < tile ? p.page_size : tile), 1, 1};
-  // 16-bit elements are copied, not read, so one type serves bf16 and fp16
-  return make_tmap(base, bytes == 4 ? TmapDtype::kF32 : TmapDtype::kBF16, 4, dims, strides, box,
-                   CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 // launches a kernel of this frame; its shared memory is allowed once per device

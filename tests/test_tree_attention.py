@@ -243,6 +243,31 @@ def test_values_that_are_not_finite_reach_their_rows(ext, cuda_device, dtype, to
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("tokens", [10, 24, 150])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_scales_empty_rows_and_large_scores_at_every_width(ext, cuda_device, dtype, tokens, D):
+    """Requests of few, some and many rows: any scale, rows that see nothing, scores of some hundreds."""
+    ctx, counts = [90, 0, 33], [tokens, tokens - 1, 2]
+    case = _case(ctx, counts, 2, 2, D, 16, dtype, seed=tokens)
+    for scale in (0.03, -0.5, 0.0):
+        out, lse = _run(*case, ctx, counts, scale=scale)
+        _check(out, lse, case, ctx, counts, scale=scale)
+    _, masks, _, _ = _trees(counts, seed=tokens)
+    for m in masks:
+        m[m.shape[0] // 2] = False
+        m[-1] = False
+    width = max(m.shape[1] for m in masks)
+    masks = [torch.nn.functional.pad(m, (0, width - m.shape[1])) for m in masks]
+    out, lse = _run(*case, ctx, counts, mask=torch.cat(masks).cuda())
+    _check(out, lse, case, ctx, counts, masks)
+    assert (lse.reshape(-1, 2)[tokens + tokens - 2] == -math.inf).all()
+    case = _case(ctx, counts, 2, 2, D, 16, dtype, seed=tokens + 1, spread=40.0)
+    out, lse = _run(*case, ctx, counts)
+    _check(out, lse, case, ctx, counts)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_uniform_borders_scale_and_out(ext, cuda_device, dtype):
     ctx, counts = [40, 41, 7], [2, 2, 2]
