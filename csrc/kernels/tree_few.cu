@@ -9,11 +9,11 @@
 // rows' maximum, sum and outputs in registers from the scores to the result.
 //
 // us here and with tree_sm100.cu, 8 kv heads:
-//   rows, dim     4 x 32000     64 x 100-3000   24 x 10-300   1 x 300
-//    8,  64      50.8 / 64.9    44.5 / 74.4     14 / 17       10 / 14
-//   16,  64      54.1 / 64.6    51.5 / 74.4     12 / 17       14 / 13
-//    8, 128      87.3 / 89.8    75.5 / 84.9     13 / 18       10 / 14
-//   16, 128      89.4 / 90.2    77.2 / 85.6     15 / 18       12 / 14
+//   rows, dim     4 x 32000     64 x 100-3000   24 x 10-300
+//    8,  64      50.8 / 64.9    44.5 / 74.4     14 / 17
+//   16,  64      54.1 / 64.6    51.5 / 74.4     12 / 17
+//    8, 128      87.3 / 89.8    75.5 / 84.9     13 / 18
+//   16, 128      89.4 / 90.2    77.2 / 85.6     15 / 18
 // (floors 40 / 31 us of bytes at dim 64, 80 / 62 at dim 128).  32 rows in this form are
 // bound by the products: 68 / 65 and 115 / 91 us over 4 x 32000.
 //
