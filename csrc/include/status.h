@@ -56,7 +56,7 @@ enum BadArgSite : uint32_t {
 };
 
 struct DeviceStatus {
-  uint32_t code;       // StatusCode, first error wins
+  uint32_t code;       // StatusCode, first error wins; any other replaces kStatusBadArgs
   uint32_t where;      // WaitSite of the first error
   uint32_t block;      // blockIdx.x that recorded it
   uint32_t detail;     // site-specific (step, tile, peer...)
@@ -68,16 +68,23 @@ struct DeviceStatus {
 };
 
 #ifdef __CUDACC__
+// The error that ends everybody's waits, or 0.  kStatusBadArgs is none: whoever
+// records it skips an entry and goes on, and the word may hold it from a call before.
 __device__ __forceinline__ uint32_t st_read_error(DeviceStatus* st) {
   if (st == nullptr) return 0;
-  return *reinterpret_cast<volatile uint32_t*>(&st->code);
+  const uint32_t code = *reinterpret_cast<volatile uint32_t*>(&st->code);
+  return code == kStatusBadArgs ? 0u : code;
 }
 
 __device__ __forceinline__ void st_record(DeviceStatus* st, uint32_t code, uint32_t where,
                                           uint32_t detail = 0) {
   if (st == nullptr) return;
   atomicAdd(&st->n_errors, 1u);
-  if (atomicCAS(&st->code, 0u, code) == 0u) {
+  uint32_t old = atomicCAS(&st->code, 0u, code);
+  if (old == kStatusBadArgs && code != kStatusBadArgs &&
+      atomicCAS(&st->code, static_cast<uint32_t>(kStatusBadArgs), code) == kStatusBadArgs)
+    old = 0u;
+  if (old == 0u) {
     st->where = where;
     st->block = blockIdx.x;
     st->detail = detail;

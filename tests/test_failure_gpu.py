@@ -56,3 +56,13 @@ def test_rank_leaving_between_steps_is_detected():
     r = subprocess.run(cmd, cwd=ROOT, env=env, capture_output=True, text=True, timeout=180)
     assert r.returncode == 0, r.stdout + r.stderr
     assert "rank 0 detected" in r.stdout, r.stdout
+
+
+def test_a_wait_that_runs_out_outranks_a_skipped_entry(ext, cuda_device):
+    """A report of a skipped entry (code 2) neither ends waits early nor hides that one ran out."""
+    flag = torch.zeros(1, dtype=torch.int64, device="cuda")
+    status = torch.zeros(8, dtype=torch.int32, device="cuda")
+    status[0], status[1] = 2, 201
+    ext.wait_selftest(flag, 1, 0.2, status)
+    torch.cuda.synchronize()
+    assert status[:2].tolist() == [1, 14]

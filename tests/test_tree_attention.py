@@ -572,3 +572,33 @@ def test_an_event_between_overlapped_launches_is_waited_for(ext, cuda_device, dt
             late.zero_()  # an ordinary launch behind the overlapped ones
         torch.cuda.synchronize()
         assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [1, 12, 40, 150])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_bad_request_leaves_the_others_whole(ext, cuda_device, dtype, tokens):
+    """A page outside the pool and a context longer than its table are reported, and every
+    row of the healthy request beside them is right; so is a later call that is given the
+    status word with the report still in it."""
+    ctx, counts = [60, 60, 3000], [tokens, 1, tokens]
+    case = _case(ctx, counts, 2, 1, 64, 16, dtype, seed=20)
+    q, kp, vp, table = case
+    broken = table.clone()
+    broken[0, 1] = 10 ** 6
+    at = torch.tensor(ctx, dtype=torch.int32)
+    at[1] = 2 ** 31 - 7
+    cu = torch.tensor([0] + counts).cumsum(0).int().cuda()
+    ref, rlse, mag, smax = O.attention(q, kp, vp, table, ctx, counts)
+    bo, bl = O.attention_bound(ref, mag, smax, dtype, 3000 + tokens, 64)
+    st = new_status("cuda")
+    good = slice(sum(counts[:2]), None)
+    for tab, lens, rows in ((broken, at, good), (table, torch.tensor(ctx, dtype=torch.int32), slice(None))):
+        out = torch.full(q.shape, 77.0, dtype=dtype, device="cuda")
+        got, lse = tree_attention(q.cuda(), kp.cuda(), vp.cuda(), tab.cuda(), lens.cuda(), cu, out=out,
+                                  max_q=tokens, return_lse=True, status=st)
+        with pytest.raises(DeviceTimeout, match="code=2"):
+            check_status(st)
+        assert ((got.cpu().double() - ref).abs() <= bo)[rows].all()
+        assert ((lse.cpu().double() - rlse).abs() <= bl + 2.0 ** -22 * rlse.abs())[rows].all()
+        assert (got != 77.0).any(-1).all()  # every row was written
