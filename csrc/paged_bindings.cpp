@@ -554,7 +554,9 @@ std::tuple<torch::Tensor, OptTensor> tree_attention(torch::Tensor q, torch::Tens
   TreeParams p{};
   p.status = status_of(status, q);
   const c10::cuda::CUDAGuard guard(q.device());
-  if (!rows_aligned(q)) q = q.contiguous();
+  // the kernels read q 4 to 16 bytes at a time; contiguous() would hand a contiguous tensor
+  // at an odd place back as it is
+  if (!rows_aligned(q)) q = q.clone(at::MemoryFormat::Contiguous);
   torch::Tensor o = out ? *out : fresh({total, heads, dim}, q.scalar_type(), q);
   OptTensor lse;
   if (return_lse) lse = fresh({total, heads}, torch::kFloat32, q);

@@ -602,3 +602,26 @@ def test_a_bad_request_leaves_the_others_whole(ext, cuda_device, dtype, tokens):
         assert ((got.cpu().double() - ref).abs() <= bo)[rows].all()
         assert ((lse.cpu().double() - rlse).abs() <= bl + 2.0 ** -22 * rlse.abs())[rows].all()
         assert (got != 77.0).any(-1).all()  # every row was written
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [1, 3, 12, 40, 150])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_queries_at_odd_places_in_memory(ext, cuda_device, dtype, tokens):
+    """Contiguous queries whose first element is not on a 16-byte boundary, and rows cut from
+    a wider tensor at every offset, give what aligned ones give."""
+    ctx, H, D = [100], 2, 64
+    q, kp, vp, table = (x.cuda() for x in _case(ctx, [tokens], H, 2, D, 16, dtype, seed=40))
+    ctx_t = torch.tensor(ctx, dtype=torch.int32).cuda()
+    want = tree_attention(q, kp, vp, table, ctx_t)
+    n = q.numel()
+    for shift in range(1, 9):
+        flat = torch.zeros(n + 16, dtype=dtype, device="cuda")
+        at = flat[shift:shift + n].view(tokens, H, D)
+        at.copy_(q)
+        assert at.is_contiguous()
+        assert torch.equal(tree_attention(at, kp, vp, table, ctx_t), want)
+        wide = torch.zeros(tokens, H * D + 16, dtype=dtype, device="cuda")
+        rows = wide[:, shift:shift + H * D].unflatten(1, (H, D))
+        rows.copy_(q)
+        assert torch.equal(tree_attention(rows, kp, vp, table, ctx_t), want)
