@@ -27,7 +27,7 @@ struct RopeOperand {
   const void* in;
   void* out;
   int64_t in_t, in_h, out_t, out_h;
-  int heads;
+  int heads;  // 1 or more
   int rotate;
   int paged;
 };

@@ -443,6 +443,8 @@ int rope_layout(const RopeParams& p, cudaStream_t stream) {
 
 int rope_launch(Elem elem, const RopeParams& p, bool vectors, cudaStream_t stream) {
   if (p.tokens == 0) return 0;
+  for (int i = 0; i < p.n_op; ++i)
+    if (p.op[i].heads < 1) return static_cast<int>(cudaErrorInvalidValue);
   switch (elem) {
     case Elem::kBF16:
       return vectors ? rope_layout<__nv_bfloat16, 8>(p, stream)

@@ -167,14 +167,17 @@ std::tuple<torch::Tensor, OptTensor> rotary(torch::Tensor q, OptTensor k, torch:
   p.interleaved = interleaved;
   p.scale = static_cast<float>(scale);
   p.sign = inverse ? -1.f : 1.f;
-  p.op[p.n_op++] = dense_operand(q, qo);
-  bool vec = rope_vectors(e, q.size(2), p.rotary_dim, interleaved) && rows_aligned(q) &&
-             rows_aligned(qo);
+  // an operand without heads has no rows: the kernels share their threads out by heads
+  bool vec = rope_vectors(e, q.size(2), p.rotary_dim, interleaved);
+  if (q.size(1) > 0) {
+    p.op[p.n_op++] = dense_operand(q, qo);
+    vec = vec && rows_aligned(q) && rows_aligned(qo);
+  }
   if (k && k->size(1) > 0) {
     p.op[p.n_op++] = dense_operand(*k, *ko);
     vec = vec && rows_aligned(*k) && rows_aligned(*ko);
   }
-  const int err = q.numel() == 0 && !(k && k->numel() > 0) ? 0 : rope_launch(e, p, vec, cur_stream());
+  const int err = p.n_op == 0 ? 0 : rope_launch(e, p, vec, cur_stream());
   RAB_CHECK(err == 0, "rotary launch failed: %s", cudaGetErrorString(static_cast<cudaError_t>(err)));
   return {qo, ko};
 }

@@ -278,3 +278,26 @@ def test_ring_attention_rotates_its_shard(ext, cuda_device):
     q2, k2 = rot(q, k, pos)
     with RingAttention(S, heads=H, head_dim=D, heads_kv=Hk, dtype=torch.bfloat16, causal=True) as attn:
         assert torch.equal(attn(q2, k2, v), got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [3, 2367, 2368, 3000])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_operands_without_heads(ext, cuda_device, dtype, T):
+    """q or k may have no heads, at any number of tokens; the other is rotated."""
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(T, 1, 64, generator=g).to(dtype)
+    none = torch.zeros(T, 0, 64, dtype=dtype, device="cuda")
+    pos, inv = torch.arange(T), rotary_frequencies(64)[0]
+    qo, ko = apply_rotary(none, x.cuda(), pos.cuda(), inv.cuda())
+    assert qo.shape == none.shape
+    _close(ko, x, pos, inv, False, 1.0)
+    qo, ko = apply_rotary(x.cuda(), none, pos.cuda(), inv.cuda())
+    assert ko.shape == none.shape
+    _close(qo, x, pos, inv, False, 1.0)
+    qo, ko = apply_rotary(none, none, pos.cuda(), inv.cuda())
+    assert qo.shape == ko.shape == none.shape
+    learns = x.cuda().requires_grad_()
+    _, ko = apply_rotary(none, learns, pos.cuda(), inv.cuda())
+    grad, = torch.autograd.grad(ko, learns, torch.ones_like(ko))
+    _close(grad, torch.ones(T, 1, 64, dtype=dtype), pos, inv, False, 1.0, inverse=True)
