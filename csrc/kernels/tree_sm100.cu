@@ -655,10 +655,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
       // ------------------------------------------------------------ results
-      s_ml[x * kM + row] = make_float2(m_run, l_run);
       ok = __all_sync(0xffffffffu, mbar_wait(o_final, w & 1, st, kSiteOReady, tmo));
       if (!ok) break;
       tc_fence_after();
+      // Behind the wait: the piece's first product with V waited for `o_free` of the piece
+      // before, so by now every warp has read that piece's pairs.
+      s_ml[x * kM + row] = make_float2(m_run, l_run);
       __syncwarp();
       if (lane_id() == 0) mbar_arrive(joined);
       ok = __all_sync(0xffffffffu, mbar_wait(joined, w & 1, st, kSiteOReady, tmo));

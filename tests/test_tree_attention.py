@@ -625,3 +625,30 @@ def test_queries_at_odd_places_in_memory(ext, cuda_device, dtype, tokens):
         rows = wide[:, shift:shift + H * D].unflatten(1, (H, D))
         rows.copy_(q)
         assert torch.equal(tree_attention(rows, kp, vp, table, ctx_t), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_pieces_of_one_tile_behind_longer_ones(ext, cuda_device, dtype, D):
+    """Units of many tiles and of one in turn, on every SM: a piece's results take both
+    chains' halves, whatever the next piece has.  Repeats give the same bits."""
+    n = 600
+    counts = [20 + b % 3 for b in range(n)]
+    ctx = [(700, 5, 60, 1300, 0)[b % 5] for b in range(n)]
+    some = list(range(0, n, 37))
+    T, page = sum(counts), 64
+    g = torch.Generator().manual_seed(41)
+    q = torch.randn(T, 1, D, generator=g).to(dtype)
+    kp, vp = (torch.randn(50, 1, page, D, generator=g).to(dtype) for _ in "kv")
+    table = torch.randint(0, 50, (n, 22), generator=g, dtype=torch.int32)  # pages are shared and only read
+    first = [0]
+    for c in counts:
+        first.append(first[-1] + c)
+    got = [_run(q, kp, vp, table, ctx, counts, max_q=22) for _ in range(3)]
+    for out, lse in got[1:]:
+        assert torch.equal(out, got[0][0]) and torch.equal(lse, got[0][1])
+    out, lse = got[0]
+    for b in some:
+        rows = slice(first[b], first[b + 1])
+        _check(out[rows], lse[rows], (q[rows], kp, vp, table[b:b + 1]), [ctx[b]], [counts[b]])
