@@ -277,13 +277,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) {
         tma_prefetch_desc(&tmK);
         tma_prefetch_desc(&tmV);
-        p.meta[blockIdx.x * kMetaInts] = 0;
       }
       Range range;
       Start first;
       const int walker = find_range<kN, kRows>(p, &range, &first);
       Walk<kN, kRows> walk;
-      if (lane == walker) walk.start(p, range, first);
+      if (lane == walker) {
+        p.meta[blockIdx.x * kMetaInts] = 0;  // by the lane that may set it later
+        walk.start(p, range, first);
+      }
       const int rows_box = min(p.page_size, kN);
       const int boxes = kN / rows_box * (D / 64);
       int n = 0;  // loads issued (K and V tiles)

@@ -167,13 +167,15 @@ __device__ __forceinline__ void walk_and_load(const TreeParams& p, const CUtenso
   if (lane == 0) {
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
-    p.meta[blockIdx.x * kMetaInts] = 0;
   }
   Range range;
   Start first;
   const int walker = find_range<kTile, kRows>(p, &range, &first);
   Walk<kTile, kRows> walk;
-  if (lane == walker) walk.start(p, range, first);
+  if (lane == walker) {
+    p.meta[blockIdx.x * kMetaInts] = 0;  // by the lane that may set it later
+    walk.start(p, range, first);
+  }
   const int rows_box = min(p.page_size, kTile);
   const int boxes = kTile / rows_box * kSegs;
   int n = 0;  // tiles loaded

@@ -652,3 +652,17 @@ def test_pieces_of_one_tile_behind_longer_ones(ext, cuda_device, dtype, D):
     for b in some:
         rows = slice(first[b], first[b + 1])
         _check(out[rows], lse[rows], (q[rows], kp, vp, table[b:b + 1]), [ctx[b]], [counts[b]])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [1, 12, 40, 150])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_split_units_of_every_request_are_joined(ext, cuda_device, dtype, tokens):
+    """Whichever request of a batch the SMs share out, its pieces are joined: the long one
+    stands first, in the middle and last, behind requests without tokens too."""
+    for at in (0, 2, 5):
+        ctx = [2500 if b == at else 9 * b for b in range(6)]
+        counts = [0 if b == 1 else tokens if b == at else 1 for b in range(6)]
+        case = _case(ctx, counts, 1, 1, 64, 64, dtype, seed=42 + at)
+        out, lse = _run(*case, ctx, counts, max_q=tokens)
+        _check(out, lse, case, ctx, counts)
