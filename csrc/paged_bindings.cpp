@@ -72,6 +72,19 @@ bool overlaps(const torch::Tensor& t) {
   return false;
 }
 
+// A tensor that a call writes through its pointer: one that takes part in autograd's
+// bookkeeping is refused, ...
+void check_written(const torch::Tensor& t, const char* name) {
+  RAB_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()),
+            "%s is written in place and must not require a gradient", name);
+}
+
+// ... and any other counts as changed, so that a backward pass which saved it raises
+// (inference tensors keep no count)
+void mark_written(const torch::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 DeviceStatus* status_of(const OptTensor& status, const torch::Tensor& ref) {
   if (!status.has_value()) return nullptr;
   RAB_CHECK(status->scalar_type() == torch::kInt32 && status->numel() >= 8 &&
@@ -134,6 +147,7 @@ void check_rope_output(const torch::Tensor& t, const char* name, const torch::Te
   RAB_CHECK(t.scalar_type() == in.scalar_type() && t.sizes() == in.sizes(),
             "%s must have its input's shape and dtype", name);
   RAB_CHECK(!overlaps(t), "%s shares memory between its elements", name);
+  check_written(t, name);
 }
 
 constexpr int64_t kMaxRopeDim = 512;  // two elements per thread in a block of 256
@@ -179,6 +193,8 @@ std::tuple<torch::Tensor, OptTensor> rotary(torch::Tensor q, OptTensor k, torch:
   }
   const int err = p.n_op == 0 ? 0 : rope_launch(e, p, vec, cur_stream());
   RAB_CHECK(err == 0, "rotary launch failed: %s", cudaGetErrorString(static_cast<cudaError_t>(err)));
+  if (q_out) mark_written(qo);
+  if (k_out) mark_written(*ko);
   return {qo, ko};
 }
 
@@ -304,6 +320,8 @@ OptTensor append_kv(torch::Tensor k, torch::Tensor v, torch::Tensor k_pages, tor
                     OptTensor inv_freq, bool interleaved, double scale, OptTensor q,
                     OptTensor q_out, OptTensor status) {
   check_pools(k_pages, v_pages, false);
+  check_written(k_pages, "k_pages");
+  check_written(v_pages, "v_pages");
   check_rows(k, "k");
   const Elem e = elem_of(k, "k");
   RAB_CHECK(k.scalar_type() == k_pages.scalar_type(), "k and the cache must share a dtype");
@@ -369,12 +387,17 @@ OptTensor append_kv(torch::Tensor k, torch::Tensor v, torch::Tensor k_pages, tor
   const int err = rope_launch(e, p, vec, cur_stream());
   RAB_CHECK(err == 0, "append_kv launch failed: %s",
             cudaGetErrorString(static_cast<cudaError_t>(err)));
+  mark_written(k_pages);
+  mark_written(v_pages);
+  if (q_out) mark_written(qo.value());
   return qo;
 }
 
 // ---- page copies ----
 void copy_pages(torch::Tensor k_pages, torch::Tensor v_pages, torch::Tensor src, torch::Tensor dst) {
   check_pools(k_pages, v_pages, true);
+  check_written(k_pages, "k_pages");
+  check_written(v_pages, "v_pages");
   for (const torch::Tensor* t : {&src, &dst})
     RAB_CHECK(!t->is_cuda() && t->dim() == 1 && t->is_contiguous() &&
                   (t->scalar_type() == torch::kInt32 || t->scalar_type() == torch::kInt64),
@@ -458,12 +481,16 @@ void copy_pages(torch::Tensor k_pages, torch::Tensor v_pages, torch::Tensor src,
     PageCopyParams<kManyPairs> p;
     launch(p);
   }
+  mark_written(k_pages);
+  mark_written(v_pages);
 }
 
 // ---- accepted path ----
 void compact_path(torch::Tensor k_pages, torch::Tensor v_pages, torch::Tensor table,
                   torch::Tensor ctx, torch::Tensor path, torch::Tensor path_lens, OptTensor status) {
   check_pools(k_pages, v_pages, true);
+  check_written(k_pages, "k_pages");
+  check_written(v_pages, "v_pages");
   const Requests r = check_requests(table, ctx, c10::nullopt, 0);
   check_int32(path, "path", 2);
   check_int32(path_lens, "path_lens", 1);
@@ -504,6 +531,8 @@ void compact_path(torch::Tensor k_pages, torch::Tensor v_pages, torch::Tensor ta
   const int err = path_compact_launch(p, cur_stream());
   RAB_CHECK(err == 0, "compact_path launch failed: %s",
             cudaGetErrorString(static_cast<cudaError_t>(err)));
+  mark_written(k_pages);
+  mark_written(v_pages);
 }
 
 // ---- attention over the cache ----
@@ -626,6 +655,7 @@ std::tuple<torch::Tensor, OptTensor> tree_attention(torch::Tensor q, torch::Tens
   const int err = tree_launch(e, p, plan, stream);
   RAB_CHECK(err == 0, "tree_attention launch failed: %s",
             cudaGetErrorString(static_cast<cudaError_t>(err)));
+  if (out) mark_written(o);
   return {o, lse};
 }
 

@@ -98,16 +98,18 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
 
     Returns ``(q', k')``, or ``q'`` alone when ``k`` is None.  ``inverse`` turns
     the other way.  ``out=(q_out, k_out)`` takes the results; passing the inputs
-    themselves rotates in place (not where a gradient is needed).
+    themselves rotates in place (not where a gradient is needed).  What it writes
+    counts as changed in place: a backward pass that saved it raises.
 
     Forward and backward can be captured into a CUDA graph together.  As with
     every autograd operation, no eager graph that reaches the same leaves may be
     alive then: torch would wait for the eager graph's stream inside the capture
     and end it with an error.
     """
+    if out is not None and torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (q, k, *out)):
+        raise ValueError("apply_rotary: out= is not offered where a gradient is needed")
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        if out is not None:
-            raise ValueError("apply_rotary: out= is not offered where a gradient is needed")
         qo, ko = load().rotary_autograd(q, k, positions, inv_freq, interleaved, scale, inverse)
         return qo if k is None else (qo, ko)
     if out is None:

@@ -315,3 +315,40 @@ def test_compact_reports_bad_paths_and_moves_nothing(ext, cuda_device, path, n, 
     with pytest.raises(DeviceTimeout, match="code=2"):
         check_status(st)
     assert torch.equal(kd.cpu(), kp) and torch.equal(vd.cpu(), vp)
+
+
+@pytest.mark.gpu
+def test_written_tensors_change_their_version(ext, cuda_device):
+    """Pools and outputs that a call writes count as changed in place."""
+    from ring_attention_benchmark_b200.ops.paged import tree_attention
+
+    kp, vp = (x.cuda() for x in _pool(4, 1, 16, 64, torch.float16))
+    table = torch.tensor([[0, 1]], dtype=torch.int32).cuda()
+    ctx = torch.tensor([3], dtype=torch.int32).cuda()
+    q, k, v = (torch.randn(2, 1, 64, device="cuda").half() for _ in range(3))
+    path, n = torch.tensor([[1]], dtype=torch.int32).cuda(), torch.tensor([1], dtype=torch.int32).cuda()
+    out = torch.empty_like(q)
+    for call, written in (
+            (lambda: append_kv(k, v, kp, vp, table, ctx, inv_freq=rotary_frequencies(64)[0].cuda(), q=q, q_out=out),
+             (kp, vp, out)),
+            (lambda: copy_pages(kp, vp, [0], [2]), (kp, vp)),
+            (lambda: compact_path(kp, vp, table, ctx, path, n), (kp, vp)),
+            (lambda: tree_attention(q, kp, vp, table, ctx, out=out), (out,))):
+        before = [t._version for t in written]
+        call()
+        assert all(t._version > x for t, x in zip(written, before))
+
+
+def test_written_tensors_that_learn_are_refused(ext):
+    """Writing past autograd into a tensor that requires a gradient is refused, as torch does."""
+    kp, vp = _pool(4, 2, 16, 64, torch.float32)
+    one = torch.ones(1, dtype=torch.int32)
+    for a, b in ((kp.clone().requires_grad_(), vp), (kp, vp.clone().requires_grad_())):
+        with pytest.raises(RuntimeError, match="require a gradient"):
+            append_kv(**_append_args(k_pages=a, v_pages=b))
+        with pytest.raises(RuntimeError, match="require a gradient"):
+            copy_pages(a, b, [0], [1])
+        with pytest.raises(RuntimeError, match="require a gradient"):
+            compact_path(a, b, torch.zeros(1, 2, dtype=torch.int32), one, torch.zeros(1, 3, dtype=torch.int32), one)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+        copy_pages(kp.clone().requires_grad_(), vp, [0], [1])

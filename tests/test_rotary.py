@@ -301,3 +301,31 @@ def test_operands_without_heads(ext, cuda_device, dtype, T):
     _, ko = apply_rotary(none, learns, pos.cuda(), inv.cuda())
     grad, = torch.autograd.grad(ko, learns, torch.ones_like(ko))
     _close(grad, torch.ones(T, 1, 64, dtype=dtype), pos, inv, False, 1.0, inverse=True)
+
+
+@pytest.mark.gpu
+def test_rotating_in_place_is_an_in_place_operation(ext, cuda_device):
+    """A tensor that a backward pass still needs may not be rotated in place unseen, as
+    with torch's own in-place operations."""
+    pos, inv = torch.arange(5).cuda(), rotary_frequencies(64)[0].cuda()
+    x = torch.randn(5, 2, 64, device="cuda", requires_grad=True)
+    for which in (0, 1):
+        y = x * 2
+        z = (y * y).sum()  # saves y
+        with torch.no_grad():
+            before = y._version
+            other = torch.randn_like(y)
+            pair = (y, other) if which == 0 else (other, y)
+            apply_rotary(*pair, pos, inv, out=pair)
+            assert y._version > before
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            z.backward()
+    with pytest.raises(ValueError, match="gradient"):  # into a leaf that learns
+        apply_rotary(x.detach(), None, pos, inv, out=(x, None))
+    with torch.inference_mode():
+        t = torch.randn(5, 2, 64, device="cuda")
+        apply_rotary(t, None, pos, inv, out=(t, None))
+    want = O.rotate(t.cpu(), pos.cpu(), inv.cpu(), False)
+    apply_rotary(t, None, pos, inv, out=(t, None))  # an inference tensor keeps no versions
+    assert (t.cpu().double() - want).abs().max() <= O.rotate_bound(
+        want, inv.cpu(), False, 1.0, torch.float32, pos.cpu()).max() * 2
