@@ -135,6 +135,12 @@ RopeOperand dense_operand(const torch::Tensor& in, const torch::Tensor& out) {
   return o;
 }
 
+// The rotation has a gradient for backward passes alone: a tangent would be dropped.
+void check_no_tangent(const torch::Tensor& t, const char* name) {
+  RAB_CHECK(!t._fw_grad(0).defined(), "%s carries a tangent: forward-mode gradients are not offered",
+            name);
+}
+
 void check_rope_input(const torch::Tensor& t, const char* name, const torch::Tensor& ref) {
   check_rows(t, name);
   RAB_CHECK(t.scalar_type() == ref.scalar_type(), "%s has another dtype than the first tensor", name);
@@ -166,6 +172,8 @@ std::tuple<torch::Tensor, OptTensor> rotary(torch::Tensor q, OptTensor k, torch:
   RAB_CHECK(std::isfinite(scale), "scale must be finite");
   if (k) check_rope_input(*k, "k", q);
   RAB_CHECK(k || !k_out, "k_out without k");
+  check_no_tangent(q, "q");
+  if (k) check_no_tangent(*k, "k");
   if (q_out) check_rope_output(*q_out, "q_out", q);
   if (k_out) check_rope_output(*k_out, "k_out", *k);
   RAB_CHECK(q.is_cuda(), "q must be a CUDA tensor");

@@ -101,6 +101,7 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     themselves rotates in place (not where a gradient is needed).  What it writes
     counts as changed in place: a backward pass that saved it raises.
 
+    The gradient is for backward passes, and for theirs; forward-mode tangents are refused.
     Forward and backward can be captured into a CUDA graph together.  As with
     every autograd operation, no eager graph that reaches the same leaves may be
     alive then: torch would wait for the eager graph's stream inside the capture

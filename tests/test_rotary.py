@@ -329,3 +329,17 @@ def test_rotating_in_place_is_an_in_place_operation(ext, cuda_device):
     apply_rotary(t, None, pos, inv, out=(t, None))  # an inference tensor keeps no versions
     assert (t.cpu().double() - want).abs().max() <= O.rotate_bound(
         want, inv.cpu(), False, 1.0, torch.float32, pos.cpu()).max() * 2
+
+
+def test_forward_mode_is_refused(ext):
+    """A tangent is never dropped without a word, whether or not the primal learns."""
+    import torch.autograd.forward_ad as fw
+
+    a = _args()
+    for name in ("q", "k"):
+        for learns in (False, True):
+            with fw.dual_level():
+                b = dict(a)
+                b[name] = fw.make_dual(a[name].clone().requires_grad_(learns), torch.ones_like(a[name]))
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    apply_rotary(**b)
