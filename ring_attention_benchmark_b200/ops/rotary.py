@@ -80,7 +80,8 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str = "n
                 return rotary_dim * math.log(original_length / (2 * math.pi * t)) / (2 * math.log(base))
 
             lo = max(0.0, math.floor(index(fast)))
-            hi = min(float(n - 1), math.ceil(index(slow)))
+            # may lie behind the last pair: then no pair is divided by the whole factor
+            hi = min(float(rotary_dim - 1), math.ceil(index(slow)))
             keep = 1.0 - ((p - lo) / max(hi - lo, 1e-3)).clamp(0.0, 1.0)
             scale = 0.1 * math.log(factor) + 1.0
         else:

@@ -343,3 +343,24 @@ def test_forward_mode_is_refused(ext):
                 b[name] = fw.make_dual(a[name].clone().requires_grad_(learns), torch.ones_like(a[name]))
                 with pytest.raises(RuntimeError, match="forward-mode"):
                     apply_rotary(**b)
+
+
+@pytest.mark.parametrize("dim, length", [(64, 131072), (128, 65536), (128, 1 << 20), (64, 1 << 24)])
+def test_yarn_ramp_ends_where_its_turns_do(dim, length):
+    """Where even the last pair turns more than `slow` times within the original length,
+    the ramp ends behind it: no such pair is stretched by the whole factor, and the ramp
+    is linear in the pair index up to the index of `slow` turns."""
+    base, factor, fast, slow = 10000.0, 4.0, 32.0, 1.0
+    plain, _ = rotary_frequencies(dim, base=base)
+    inv, _ = rotary_frequencies(dim, base=base, scaling="yarn", factor=factor, original_length=length,
+                                fast=fast, slow=slow)
+    turns = length * plain / (2 * math.pi)
+    assert turns[-1] > slow
+    index = lambda t: dim * math.log(length / (2 * math.pi * t)) / (2 * math.log(base))  # noqa: E731
+    lo, hi = math.floor(index(fast)), min(math.ceil(index(slow)), dim - 1)
+    assert hi > dim // 2 - 1
+    for p in range(dim // 2):
+        keep = min(1.0, max(0.0, 1.0 - (p - lo) / (hi - lo)))
+        assert keep > 0
+        want = plain[p].item() * (keep + (1.0 - keep) / factor)
+        assert inv[p].item() == pytest.approx(want, rel=1e-12)
