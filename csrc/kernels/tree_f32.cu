@@ -28,8 +28,8 @@
 // scheduler, 16 being its rate.  us with units of 8 / 16 / 32 rows, 8 kv heads:
 //   rows of a kv head:      8          16            32           2000 (causal chunk)
 //   8000 keys, dim 64    14/-/-   19 / 17 / 23   30 / - / 25   1324 / - / 726
-//   8000 keys, dim 128   24/-/-   40 / 30 / 37   67 / - / 41   3003 / - / 1512
-//   4 x 32000, dim 128            367 / 275 / 371   804 / - / 372
+//   8000 keys, dim 128   24/-/-   40 / 30 / 37   67 / - / 41   3003 / - / 1474
+//   4 x 32000, dim 128            367 / 275 / 371   804 / - / 365
 // hence 8, 16 or 32 by the rows of the longest request.
 //
 // 3 trees over 4096 to 16384 keys, 8 heads x 64 (126 MB, 19 us at the copy rate): 32
@@ -86,11 +86,28 @@ __device__ __forceinline__ int tile_at(int key, int col) {
 
 // x = hi + lo for a 3xTF32 product, hi the nearest of 11 bits: rounded, lo has either
 // sign, and the product lo * lo that is left out does not add up (cut off, it is
-// always positive).  lo of an infinity is kept finite, so that it stays an infinity.
+// always positive).  An infinity stays in hi, where its product has the right sign; the
+// products of lo are summed apart and mean nothing beside it (`whole_score`).
 __device__ __forceinline__ void split3x(float x, float& hi, float& lo) {
   const float top = __uint_as_float(sm100::f32_to_tf32(x));
-  lo = fmaxf(x - top, -3.0e38f);
+  lo = x - top;
   hi = top;
+}
+
+// The same of V, whose products run into one sum: hi stays finite and lo carries an
+// infinity, so that only its product with a weight's hi, which is positive, is infinite.
+// Costs the split an instruction more: 500 tokens over 8000 keys of 128 take 1474 us, and
+// 1570 with K split so as well.
+__device__ __forceinline__ void split3x_v(float x, float& hi, float& lo) {
+  uint32_t top;
+  asm("cvt.rna.satfinite.tf32.f32 %0, %1;" : "=r"(top) : "f"(x));
+  hi = __uint_as_float(top);
+  lo = x - hi;
+}
+
+// a score from its leading products and the small ones
+__device__ __forceinline__ float whole_score(float hi, float lo) {
+  return hi + (isfinite(lo) ? lo : 0.f);
 }
 
 // c += a * b, one 16 x 8 x 8 product of 11-bit operands
@@ -218,7 +235,7 @@ __device__ __forceinline__ void f32_narrow(const TreeParams& p, const WarpBlock<
       for (int u = 0; u < kMine; ++u)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          s[u][i] = s2[0][2 * u + i] + s2[1][2 * u + i] + s_lo[2 * u + i];
+          s[u][i] = whole_score(s2[0][2 * u + i] + s2[1][2 * u + i], s_lo[2 * u + i]);
       if (tail) {
 #pragma unroll
         for (int u = 0; u < kMine; ++u) {
@@ -305,7 +322,7 @@ __device__ __forceinline__ void f32_narrow(const TreeParams& p, const WarpBlock<
           for (int i = 0; i < 4; ++i) {
             float a[4], a_lo[4];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) split3x(v[x >> 1][x & 1][i], a[x], a_lo[x]);
+            for (int x = 0; x < 4; ++x) split3x_v(v[x >> 1][x & 1][i], a[x], a_lo[x]);
             mma_3x(part[4 * h + i], part[4 * h + i], a, a_lo, w_hi, w_lo);
           }
         }
@@ -466,7 +483,7 @@ __device__ __forceinline__ void f32_wide(const TreeParams& p,
 #pragma unroll
       for (int u = 0; u < G; ++u) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[u][i] += s_lo[u][i];  // [2 key + row]
+        for (int i = 0; i < 4; ++i) s[u][i] = whole_score(s[u][i], s_lo[u][i]);  // [2 key + row]
         if (tail) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
@@ -559,7 +576,7 @@ __device__ __forceinline__ void f32_wide(const TreeParams& p,
             for (int i = 0; i < kI; ++i)
 #pragma unroll
               for (int x = 0; x < 4; ++x)
-                split3x(v[step][x >> 1][x & 1][i0 + i], a[i][x], a_lo[i][x]);
+                split3x_v(v[step][x >> 1][x & 1][i0 + i], a[i][x], a_lo[i][x]);
 #pragma unroll
             for (int i = 0; i < kI; ++i)
 #pragma unroll

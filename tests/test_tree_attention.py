@@ -666,3 +666,37 @@ def test_split_units_of_every_request_are_joined(ext, cuda_device, dtype, tokens
         case = _case(ctx, counts, 1, 1, 64, 64, dtype, seed=42 + at)
         out, lse = _run(*case, ctx, counts, max_q=tokens)
         _check(out, lse, case, ctx, counts)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("tokens", [1, 12, 24, 150])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_infinities_among_the_cached_keys(ext, cuda_device, dtype, tokens, D):
+    """An infinite V of a cached key is in its own column of every row's result; an infinite
+    K takes all weight from its key where the product is -inf, and makes the row NaN where
+    it is +inf.  Everything else is as without them."""
+    ctx, at, col = 500, (40, 333), 7
+    case = _case([ctx], [tokens], 1, 1, D, 16, dtype, seed=30 + tokens)
+    q, kp, vp, table = case
+    ref, _, mag, smax = O.attention(*case, [ctx], [tokens])
+    bo, _ = O.attention_bound(ref, mag, smax, dtype, ctx + tokens, D)
+    rest = torch.arange(D) != col
+    for signs, want in (((1, 1), math.inf), ((-1, -1), -math.inf), ((1, -1), math.nan)):
+        bad = vp.clone()
+        for j, s in zip(at, signs):
+            bad[table[0, j // 16], 0, j % 16, col] = s * math.inf
+        got = _run(q, kp, bad, table, [ctx], [tokens])[0].cpu().double()
+        assert ((got - ref).abs() <= bo)[..., rest].all()
+        c = got[..., col]
+        assert (c.isnan() if math.isnan(want) else c == want).all()
+    bad = kp.clone()
+    for j in at:
+        bad[table[0, j // 16], 0, j % 16, col] = math.inf
+    got, lse = (x.cpu().double() for x in _run(q, bad, vp, table, [ctx], [tokens]))
+    low = q[:, 0, col] < 0
+    assert got[~low].isnan().all() and lse[~low].isnan().all()
+    ref2, rlse2, mag2, _ = O.attention(q, bad, vp, table, [ctx], [tokens])
+    bo2, bl2 = O.attention_bound(ref2, mag2, smax, dtype, ctx + tokens, D)  # sizes of the finite scores
+    assert ((got - ref2).abs() <= bo2)[low].all()
+    assert ((lse - rlse2).abs() <= bl2 + 2.0 ** -22 * rlse2.abs())[low].all()
