@@ -67,6 +67,7 @@ struct Half;
 template <>
 struct Half<__nv_bfloat16> {
   static constexpr uint32_t kExp = 0x7f80u;
+  static constexpr float kLift = 0.f;
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     return sm100::pack_bf16x2(lo, hi);
   }
@@ -80,6 +81,10 @@ struct Half<__nv_bfloat16> {
 template <>
 struct Half<__half> {
   static constexpr uint32_t kExp = 0x7c00u;
+  // Weights are formed 2^15 times larger: fp16 holds nothing below 2^-25, and a quarter
+  // million keys of such weights add up to a percent.  The sums and the merge carry the
+  // factor in the maximum, lowered by it.
+  static constexpr float kLift = 15.f;
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -249,7 +254,7 @@ __device__ __forceinline__ void few_compute(const TreeParams& p,
           for (int x = 1; x < 2 * KB; ++x) mx = fmaxf(mx, s[x][i]);
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-          const float mn = fmaxf(m[u][i], mx);
+          const float mn = fmaxf(m[u][i], mx - H::kLift);
           const float use = mn == -INFINITY ? 0.f : mn;
           alpha[u][i] = ex2_approx(m[u][i] - use);  // m = -inf: 0
           moved |= mn != m[u][i];

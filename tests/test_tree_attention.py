@@ -700,3 +700,37 @@ def test_infinities_among_the_cached_keys(ext, cuda_device, dtype, tokens, D):
     bo2, bl2 = O.attention_bound(ref2, mag2, smax, dtype, ctx + tokens, D)  # sizes of the finite scores
     assert ((got - ref2).abs() <= bo2)[low].all()
     assert ((lse - rlse2).abs() <= bl2 + 2.0 ** -22 * rlse2.abs())[low].all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens, n", [(1, 1 << 20), (12, 1 << 18), (20, 1 << 17), (130, 1 << 17)])
+def test_many_small_weights_in_fp16(ext, cuda_device, tokens, n):
+    """Keys whose weights lie 2^-26 below the largest add up over a long context.
+
+    As many requests as there are SMs, so that hardly a unit is cut; all share the same pages:
+    first one whose keys j % 16 == 0 score 0 with a V of zero, then the same page over and
+    over, of keys that score -18 with a V of one.  A weight below 2^-14 is held to steps of
+    2^-24, after a factor of 2^7 at least over the row's largest: off by 2^-32 of that each,
+    n of them over a sum of 8.  fp32 sums: n terms of 2^-24 relative, and the exponential 2^-21.
+    """
+    D, page, few = 64, 128, 8
+    batch = torch.cuda.get_device_properties(0).multi_processor_count
+    kp, vp = torch.zeros(3, 1, page, D).half(), torch.zeros(3, 1, page, D).half()
+    kp[:2, 0, :, 0] = -18.0
+    kp[0, 0, ::16, 0] = 0.0
+    vp[:2] = 1.0
+    vp[0, 0, ::16] = 0.0
+    table = torch.ones(n // page + 2, dtype=torch.int32)
+    table[0], table[-2:] = 0, 2
+    q = torch.zeros(batch * tokens, 1, D).half()
+    q[..., 0] = 1.0
+    ctx = torch.full((batch,), n, dtype=torch.int32)
+    blank = torch.zeros(batch * tokens, 1, dtype=torch.bool)
+    out, lse = tree_attention(q.cuda(), kp.cuda(), vp.cuda(), table.cuda().expand(batch, -1), ctx.cuda(),
+                              mask=blank.cuda(), scale=1.0, return_lse=True)
+    small = (n - few) * math.exp(-18.0)
+    want = small / (few + small)
+    tol = want * (O.half_step(torch.float16) * 2 + n * 2.0 ** -24 + 2.0 ** -20) + n * 2.0 ** -32 / few
+    assert tol < want / 4
+    assert (out.cpu().double() - want).abs().max().item() <= tol
+    assert (lse.cpu().double() - math.log(few + small)).abs().max().item() <= n * 2.0 ** -24 + 2.0 ** -20
