@@ -10,6 +10,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <numeric>
 #include <vector>
 
 #include "bind_util.h"
@@ -65,11 +66,80 @@ bool rows_aligned(const torch::Tensor& t) {
   return aligned16(t.data_ptr()) && t.stride(0) * e % 16 == 0 && t.stride(1) * e % 16 == 0;
 }
 
-// two elements of `t` share an address (an expanded tensor): not a place to write to
+// Strides and sizes in bytes of the dimensions that step through memory.
+struct Steps {
+  int64_t stride[10], count[10];
+  int n = 0;
+  void add(const torch::Tensor& t) {
+    for (int64_t d = 0; d < t.dim(); ++d)
+      if (t.size(d) > 1) {
+        stride[n] = t.stride(d) * t.element_size();
+        count[n++] = t.size(d);
+      }
+  }
+};
+
+// bytes from the first element to the end of the last, over the steps below `limit`
+int64_t span_below(const torch::Tensor& t, int64_t limit) {
+  Steps s;
+  s.add(t);
+  int64_t bytes = t.element_size();
+  for (int i = 0; i < s.n; ++i)
+    if (s.stride[i] < limit) bytes += (s.count[i] - 1) * s.stride[i];
+  return bytes;
+}
+
+// two elements of `t` may share an address (an expanded tensor, overlapping rows): not a
+// place to write to.  Every step must clear what the smaller ones span.
 bool overlaps(const torch::Tensor& t) {
-  for (int64_t d = 0; d < t.dim(); ++d)
-    if (t.size(d) > 1 && t.stride(d) == 0) return true;
+  Steps s;
+  s.add(t);
+  for (int i = 0; i < s.n; ++i) {
+    if (s.stride[i] < span_below(t, s.stride[i])) return true;
+    for (int j = 0; j < i; ++j)
+      if (s.stride[i] == s.stride[j]) return true;
+  }
   return false;
+}
+
+bool same_view(const torch::Tensor& a, const torch::Tensor& b) {
+  if (a.data_ptr() != b.data_ptr() || a.scalar_type() != b.scalar_type() || a.sizes() != b.sizes())
+    return false;
+  for (int64_t d = 0; d < a.dim(); ++d)
+    if (a.size(d) > 1 && a.stride(d) != b.stride(d)) return false;
+  return true;
+}
+
+// An address may belong to both.  False for slices that lie between one another, like
+// the heads of one projection: where the larger steps of both are multiples of a period,
+// what the smaller steps span must lie apart within it.
+bool may_share(const torch::Tensor& a, const torch::Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  const int64_t at = static_cast<const char*>(b.data_ptr()) - static_cast<const char*>(a.data_ptr());
+  if (at >= span_below(a, INT64_MAX) || -at >= span_below(b, INT64_MAX)) return false;
+  Steps s;
+  s.add(a);
+  s.add(b);
+  for (int i = 0; i < s.n; ++i) {
+    int64_t period = 0;
+    for (int j = 0; j < s.n; ++j)
+      if (s.stride[j] >= s.stride[i]) period = std::gcd(period, s.stride[j]);
+    if (period == 0) continue;
+    const int64_t d = (at % period + period) % period;
+    if (d >= span_below(a, s.stride[i]) && d + span_below(b, s.stride[i]) <= period) return false;
+  }
+  return true;
+}
+
+void check_apart(const torch::Tensor& written, const char* name, const torch::Tensor& other,
+                 const char* other_name) {
+  RAB_CHECK(!may_share(written, other), "%s shares memory with %s", name, other_name);
+}
+
+// a result may take its own input's place, element by element
+void check_result(const torch::Tensor& written, const char* name, const torch::Tensor& in,
+                  const char* in_name) {
+  if (!same_view(written, in)) check_apart(written, name, in, in_name);
 }
 
 // A tensor that a call writes through its pointer: one that takes part in autograd's
@@ -176,6 +246,15 @@ std::tuple<torch::Tensor, OptTensor> rotary(torch::Tensor q, OptTensor k, torch:
   if (k) check_no_tangent(*k, "k");
   if (q_out) check_rope_output(*q_out, "q_out", q);
   if (k_out) check_rope_output(*k_out, "k_out", *k);
+  if (q_out) {
+    check_result(*q_out, "q_out", q, "q");
+    if (k) check_apart(*q_out, "q_out", *k, "k");
+    if (k_out) check_apart(*q_out, "q_out", *k_out, "k_out");
+  }
+  if (k_out) {
+    check_result(*k_out, "k_out", *k, "k");
+    check_apart(*k_out, "k_out", q, "q");
+  }
   RAB_CHECK(q.is_cuda(), "q must be a CUDA tensor");
   check_same(positions, "positions", q);
   check_same(inv_freq, "inv_freq", q);
@@ -350,7 +429,15 @@ OptTensor append_kv(torch::Tensor k, torch::Tensor v, torch::Tensor k_pages, tor
   RAB_CHECK(std::isfinite(scale), "scale must be finite");
   if (q) check_rope_input(*q, "q", k);
   RAB_CHECK(q || !q_out, "q_out without q");
-  if (q_out) check_rope_output(*q_out, "q_out", *q);
+  check_apart(k_pages, "k_pages", v_pages, "v_pages");
+  if (q_out) {
+    check_rope_output(*q_out, "q_out", *q);
+    check_result(*q_out, "q_out", *q, "q");
+    check_apart(*q_out, "q_out", k, "k");
+    check_apart(*q_out, "q_out", v, "v");
+    check_apart(*q_out, "q_out", k_pages, "k_pages");
+    check_apart(*q_out, "q_out", v_pages, "v_pages");
+  }
   RAB_CHECK(k.is_cuda(), "k must be a CUDA tensor");
   check_same(v, "v", k);
   check_same(k_pages, "k_pages", k);
@@ -406,6 +493,7 @@ void copy_pages(torch::Tensor k_pages, torch::Tensor v_pages, torch::Tensor src,
   check_pools(k_pages, v_pages, true);
   check_written(k_pages, "k_pages");
   check_written(v_pages, "v_pages");
+  check_result(k_pages, "k_pages", v_pages, "v_pages");  // one pool twice is copied alike
   for (const torch::Tensor* t : {&src, &dst})
     RAB_CHECK(!t->is_cuda() && t->dim() == 1 && t->is_contiguous() &&
                   (t->scalar_type() == torch::kInt32 || t->scalar_type() == torch::kInt64),
@@ -499,6 +587,7 @@ void compact_path(torch::Tensor k_pages, torch::Tensor v_pages, torch::Tensor ta
   check_pools(k_pages, v_pages, true);
   check_written(k_pages, "k_pages");
   check_written(v_pages, "v_pages");
+  check_apart(k_pages, "k_pages", v_pages, "v_pages");
   const Requests r = check_requests(table, ctx, c10::nullopt, 0);
   check_int32(path, "path", 2);
   check_int32(path_lens, "path_lens", 1);
@@ -583,6 +672,9 @@ std::tuple<torch::Tensor, OptTensor> tree_attention(torch::Tensor q, torch::Tens
   if (out) {
     check_rope_output(*out, "out", q);
     RAB_CHECK(rows_aligned(*out), "out must have rows aligned to 16 bytes");
+    check_result(*out, "out", q, "q");
+    check_apart(*out, "out", k_pages, "k_pages");
+    check_apart(*out, "out", v_pages, "v_pages");
   }
   RAB_CHECK(timeout_s > 0 && timeout_s <= 3600, "timeout_s must be in (0, 3600]");
   RAB_CHECK(q.is_cuda(), "q must be a CUDA tensor");

@@ -352,3 +352,32 @@ def test_written_tensors_that_learn_are_refused(ext):
             compact_path(a, b, torch.zeros(1, 2, dtype=torch.int32), one, torch.zeros(1, 3, dtype=torch.int32), one)
     with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
         copy_pages(kp.clone().requires_grad_(), vp, [0], [1])
+
+
+def test_pools_and_outputs_that_overlap_are_refused(ext):
+    inv, one = rotary_frequencies(64)[0], torch.ones(1, dtype=torch.int32)
+    kp, vp = _pool(4, 2, 16, 64, torch.float32)
+    both = torch.zeros(4, 2, 2, 16, 64)  # K and V of a page side by side
+    big = torch.zeros(5, 2, 16, 64)
+    q = torch.zeros(3, 2, 64)
+    flat = torch.zeros(4, 2, 64)
+    table, path = torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, 3, dtype=torch.int32)
+    for a, b, what in ((kp, vp, "CUDA"), (both[:, 0], both[:, 1], "CUDA"), (kp, kp, "shares memory"),
+                       (big[:4], big[1:], "shares memory"), (both[:, 0], both[:, 0], "shares memory")):
+        with pytest.raises(RuntimeError, match=what):
+            append_kv(**_append_args(k_pages=a, v_pages=b))
+        with pytest.raises(RuntimeError, match=what):
+            compact_path(a, b, table, one, path, one)
+        with pytest.raises(RuntimeError, match="CUDA" if a is b or a.data_ptr() == b.data_ptr() else what):
+            copy_pages(a, b, [0], [1])
+    thin = torch.zeros(4 * 2048).as_strided((4, 2, 16, 64), (1024, 1024, 64, 1))  # pages overlap
+    with pytest.raises(RuntimeError, match="between its pages"):
+        append_kv(**_append_args(k_pages=thin))
+    args = _append_args(inv_freq=inv, q=q)
+    for out, what in ((q, "CUDA"), (torch.zeros(3, 2, 64), "CUDA"), (args["k"], "shares memory with k"),
+                      (args["v"], "shares memory with v"), (args["k_pages"][0, 0, :6].view(3, 2, 64), "k_pages"),
+                      (args["v_pages"][1, 1, 3:9].view(3, 2, 64), "v_pages")):
+        with pytest.raises(RuntimeError, match=what):
+            append_kv(**args, q_out=out)
+    with pytest.raises(RuntimeError, match="q_out shares memory with q"):
+        append_kv(**_append_args(inv_freq=inv, q=flat[:3]), q_out=flat[1:])

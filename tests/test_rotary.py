@@ -364,3 +364,34 @@ def test_yarn_ramp_ends_where_its_turns_do(dim, length):
         assert keep > 0
         want = plain[p].item() * (keep + (1.0 - keep) / factor)
         assert inv[p].item() == pytest.approx(want, rel=1e-12)
+
+
+def test_outputs_that_overlap_are_refused(ext):
+    """An output may be its own input or lie between other slices; any other shared element
+    would be read and written at the same time."""
+    pos, inv = torch.arange(4), rotary_frequencies(16)[0]
+    flat = torch.zeros(200)
+    rows = lambda at, h=1: flat[at:at + 4 * h * 16].view(4, h, 16)  # noqa: E731
+    qkv = torch.zeros(4, 6, 16)  # heads of q, k and v side by side
+    pair = torch.zeros(4, 2, 2, 16)  # q's and k's heads in turn
+    far = torch.zeros(4, 2, 16)
+    cases = [  # q, k, q_out, k_out, refused
+        (rows(0), None, rows(16), None, "q_out shares memory with q"),       # a token further on
+        (rows(0), None, rows(1), None, "q_out shares memory with q"),
+        (rows(0), None, rows(64), None, None),
+        (rows(0), rows(64), rows(64), torch.zeros(4, 1, 16), "q_out shares memory with k"),
+        (rows(0), rows(64), torch.zeros(4, 1, 16), rows(0), "k_out shares memory with q"),
+        (rows(0), rows(64), far[:, :1], far[:, :1], "q_out shares memory with k_out"),
+        (rows(0), rows(64), far[:, :1], far[:, 1:], None),
+        (rows(0), rows(0), rows(0), torch.zeros(4, 1, 16), "q_out shares memory with k"),
+        (qkv[:, :3], qkv[:, 3:5], qkv[:, :3], qkv[:, 3:5], None),            # in place, both
+        (qkv[:, :3], qkv[:, 3:5], qkv[:, :3], qkv[:, 4:6], "k_out shares memory with k"),
+        (qkv[:, :3], None, qkv[:, 3:], None, None),
+        (pair[:, :, 0], pair[:, :, 1], pair[:, :, 0], pair[:, :, 1], None),
+        (far, None, flat.as_strided((4, 2, 16), (24, 16, 1)), None, "shares memory between"),
+        (far, None, flat.as_strided((4, 2, 16), (16, 16, 1)), None, "shares memory between"),
+        (far, None, flat.as_strided((4, 2, 16), (16, 64, 1)), None, None),   # heads outside
+    ]
+    for q, k, qo, ko, what in cases:
+        with pytest.raises(RuntimeError, match=what or "CUDA"):
+            apply_rotary(q, k, pos, inv, out=(qo, ko))

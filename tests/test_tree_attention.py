@@ -734,3 +734,25 @@ def test_many_small_weights_in_fp16(ext, cuda_device, tokens, n):
     assert tol < want / 4
     assert (out.cpu().double() - want).abs().max().item() <= tol
     assert (lse.cpu().double() - math.log(few + small)).abs().max().item() <= n * 2.0 ** -24 + 2.0 ** -20
+
+
+def test_outputs_that_overlap_are_refused(ext):
+    a = _args()
+    wide = torch.zeros(2, 8, 64)
+    for q, out, what in ((a["q"], a["q"], "CUDA"), (wide[:, :4], wide[:, 4:], "CUDA"),
+                         (wide[:, :4], wide[:, 2:6], "out shares memory with q"),
+                         (a["q"], a["k_pages"][0, 0, :8].view(2, 4, 64), "with k_pages"),
+                         (a["q"], a["v_pages"][1, 0, :8].view(2, 4, 64), "with v_pages")):
+        with pytest.raises(RuntimeError, match=what):
+            tree_attention(**dict(a, q=q, out=out))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [1, 12, 40, 150])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_the_result_may_take_the_place_of_the_queries(ext, cuda_device, dtype, tokens):
+    ctx, counts = [900, 3], [tokens, tokens]
+    q, kp, vp, table = (x.cuda() for x in _case(ctx, counts, 4, 2, 64, 16, dtype, seed=43))
+    ctx_t = torch.tensor(ctx, dtype=torch.int32).cuda()
+    want = tree_attention(q, kp, vp, table, ctx_t)
+    assert torch.equal(tree_attention(q, kp, vp, table, ctx_t, out=q), want) and torch.equal(q, want)
