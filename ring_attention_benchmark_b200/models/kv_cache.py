@@ -241,11 +241,18 @@ class CacheStep:
             raise RuntimeError("the cache was defragmented: the step's table is out of date")
         return self.cache.k[layer], self.cache.v[layer]
 
+    def _rows(self, **tensors: Optional[torch.Tensor]) -> None:
+        """Every token of the step has a row; rows behind them (a padded batch) are left."""
+        for name, t in tensors.items():
+            if t is not None and t.shape[0] < self.tokens:
+                raise ValueError(f"{name} has {t.shape[0]} rows, the step {self.tokens} tokens")
+
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, rotary: Optional[Rotary] = None,
                q: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
                status: Optional[torch.Tensor] = None):
         """Write the step's K (rotated) and V of one layer; returns q rotated, if given."""
         kp, vp = self._layer(layer)
+        self._rows(k=k, v=v, q=q)
         if rotary is None:
             return paged.append_kv(k, v, kp, vp, self.block_table, self.context_lens, self.cu_q,
                                    positions=positions, q=q, status=status)
@@ -259,6 +266,7 @@ class CacheStep:
                out: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None):
         """Attention of the step's tokens over the cache (see `ops.paged.tree_attention`)."""
         kp, vp = self._layer(layer)
+        self._rows(q=q)
         return paged.tree_attention(q, kp, vp, self.block_table, self.context_lens, self.cu_q,
                                     max_q=self.max_q, mask=mask, scale=scale,
                                     return_lse=return_lse, out=out, status=status)

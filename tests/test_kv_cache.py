@@ -293,3 +293,23 @@ def test_prompt_fork_trees_and_defragmentation(ext, cuda_device, dtype, d):
     cache.free(seq)
     cache.free(two)
     assert cache.table.free_pages == 40
+
+
+def test_steps_refuse_too_few_rows(ext):
+    """A step's tensors hold all of its tokens: a missing one would leave stale rows in the
+    cache that a commit then counts.  More rows are a padded batch."""
+    cache = PagedKVCache(1, 8, 1, 64, page_size=16, device="cpu")
+    step = cache.step([cache.new_sequence(), cache.new_sequence()], [3, 2])
+    full, short = torch.zeros(5, 1, 64).bfloat16(), torch.zeros(4, 1, 64).bfloat16()
+    rot = Rotary(64, device="cpu")
+    for k, v, q in ((short, short, None), (full, short, None), (full, full, short)):
+        with pytest.raises(ValueError, match="4 rows, the step 5 tokens"):
+            step.append(0, k, v, rotary=rot, q=q)
+    with pytest.raises(ValueError, match="4 rows, the step 5 tokens"):
+        step.attend(0, short)
+    for rows in (5, 8):  # on to the operators, which want a GPU
+        x = torch.zeros(rows, 1, 64).bfloat16()
+        with pytest.raises(RuntimeError, match="CUDA"):
+            step.append(0, x, x)
+        with pytest.raises(RuntimeError, match="CUDA"):
+            step.attend(0, x)
