@@ -202,8 +202,7 @@ class CacheStep:
         table = cache.table
         if not self.seqs:
             raise ValueError("a step needs a sequence")
-        if cache.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("make the step outside a capture: its table is uploaded once")
+        cache._no_capture()
         for s in self.seqs:
             other = cache._open.get(s, lambda: None)()
             if other is not None and other._open:
@@ -223,9 +222,7 @@ class CacheStep:
             grid[i, :len(p)] = torch.tensor(p, dtype=torch.int32)
         host[:b] = torch.tensor(self.lengths, dtype=torch.int32)
         host[b + 1:2 * b + 1] = torch.tensor(self.counts, dtype=torch.int32).cumsum(0)
-        if cache.device.type == "cuda":
-            host = host.pin_memory()
-        dev = host.to(cache.device, non_blocking=True)
+        dev = cache._upload(host)
         self.context_lens = dev[:b]
         self.cu_q = dev[b:2 * b + 1]
         self.block_table = dev[2 * b + 1:].view(b, width)
@@ -280,13 +277,12 @@ class CacheStep:
                 if not -1 <= up < i:
                     raise ValueError(f"parent {up} of token {i} is no token before it")
         flat = torch.tensor([x for p in parents for x in p], dtype=torch.int32)
-        return paged.tree_mask(flat.to(self.cache.device), self.cu_q, max_q=self.max_q)
+        return paged.tree_mask(self.cache._upload(flat), self.cu_q, max_q=self.max_q)
 
     def positions(self, depth: torch.Tensor) -> torch.Tensor:
         """Rotary positions of tree tokens: cached length plus depth (int32)."""
-        return torch.repeat_interleave(
-            self.context_lens, torch.tensor(self.counts).to(self.cache.device),
-            output_size=self.tokens) + depth
+        return torch.repeat_interleave(self.context_lens, self.cu_q[1:] - self.cu_q[:-1],
+                                       output_size=self.tokens) + depth
 
     def _close(self, kept: Sequence[int]) -> None:
         for seq, n in zip(self.seqs, kept):
@@ -318,9 +314,7 @@ class CacheStep:
             for i, p in enumerate(paths):
                 host[i, 0] = len(p)
                 host[i, 1:1 + len(p)] = torch.tensor(list(p), dtype=torch.int32)
-            if self.cache.device.type == "cuda":
-                host = host.pin_memory()
-            dev = host.to(self.cache.device, non_blocking=True)
+            dev = self.cache._upload(host)
             lens = dev[:, 0].contiguous()
             paged.compact_path(self.cache.k, self.cache.v, self.block_table, self.context_lens,
                                dev[:, 1:], lens)
@@ -352,6 +346,18 @@ class PagedKVCache:
         self.device = self.k.device
         self._open: Dict[int, "weakref.ref[CacheStep]"] = {}  # each sequence's last step
         self._moves = 0
+
+    def _no_capture(self) -> None:
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("tables, trees and paths are uploaded once: make the step, its tree "
+                               "and its acceptance outside a capture")
+
+    def _upload(self, host: torch.Tensor) -> torch.Tensor:
+        """A small tensor of the host on the cache's device, without waiting for either."""
+        if self.device.type == "cuda":
+            self._no_capture()
+            host = host.pin_memory()
+        return host.to(self.device, non_blocking=True)
 
     def new_sequence(self) -> int:
         return self.table.new()

@@ -313,3 +313,52 @@ def test_steps_refuse_too_few_rows(ext):
             step.append(0, x, x)
         with pytest.raises(RuntimeError, match="CUDA"):
             step.attend(0, x)
+
+
+@pytest.mark.gpu
+def test_a_drafted_step_does_not_wait_for_the_gpu(ext, cuda_device):
+    """Tables, trees, positions and paths are handed over without a synchronisation."""
+    cache = PagedKVCache(1, 32, 1, 64, page_size=16)
+    a, b = cache.new_sequence(), cache.new_sequence()
+    prompt = cache.step([a, b], [5, 9])
+    prompt.append(0, *(torch.randn(14, 1, 64, device="cuda").bfloat16() for _ in "kv"))
+    prompt.commit()
+    parents = [[-1, 0, 0, 1], [-1, 0, 1]]
+    k = torch.randn(7, 1, 64, device="cuda").bfloat16()
+    torch.cuda.synchronize()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        step = cache.step([a, b], [4, 3])
+        mask, depth = step.tree(parents)
+        pos = step.positions(depth)
+        step.append(0, k, k)
+        out = step.attend(0, k, mask=mask)
+        step.accept([[0, 2], [0, 1, 2]])
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    assert pos.dtype == torch.int32 and pos.tolist() == [5, 6, 6, 7, 9, 10, 11]
+    assert out.isfinite().all() and cache.length(a) == 7 and cache.length(b) == 12
+    none = cache.step([a, b], [0, 0])  # nothing drafted
+    mask, depth = none.tree([[], []])
+    assert none.positions(depth).numel() == 0 and mask.shape[0] == 0
+
+
+@pytest.mark.gpu
+def test_uploads_inside_a_capture_are_refused(ext, cuda_device):
+    """A replay would copy from host memory that is long someone else's."""
+    cache = PagedKVCache(1, 32, 1, 64, page_size=16)
+    seq, other = cache.new_sequence(), cache.new_sequence()
+    step = cache.step([seq], [3])
+    x = torch.zeros(3, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = x + 1
+        for call in (lambda: step.tree([[-1, 0, 0]]), lambda: step.accept([[0, 2]]),
+                     lambda: cache.step([other], [1])):
+            with pytest.raises(RuntimeError, match="outside a capture"):
+                call()
+    graph.replay()
+    assert (y == 1).all()
+    assert cache.table.pages(other) == () and cache.length(seq) == 0
+    step.accept([[0]])  # still open
+    assert cache.length(seq) == 1
