@@ -239,7 +239,7 @@ std::tuple<torch::Tensor, OptTensor> rotary(torch::Tensor q, OptTensor k, torch:
   p.dim = static_cast<int>(q.size(2));
   set_frequencies(p, inv_freq, q.size(2));
   set_positions(p, positions, q.size(0));
-  RAB_CHECK(std::isfinite(scale), "scale must be finite");
+  RAB_CHECK(std::isfinite(static_cast<float>(scale)), "scale must be finite in fp32");
   if (k) check_rope_input(*k, "k", q);
   RAB_CHECK(k || !k_out, "k_out without k");
   check_no_tangent(q, "q");
@@ -426,7 +426,7 @@ OptTensor append_kv(torch::Tensor k, torch::Tensor v, torch::Tensor k_pages, tor
   if (inv_freq) set_frequencies(p, *inv_freq, dim);
   RAB_CHECK(inv_freq || (!positions && !q), "positions and q have no use without inv_freq");
   if (positions) set_positions(p, *positions, k.size(0));
-  RAB_CHECK(std::isfinite(scale), "scale must be finite");
+  RAB_CHECK(std::isfinite(static_cast<float>(scale)), "scale must be finite in fp32");
   if (q) check_rope_input(*q, "q", k);
   RAB_CHECK(q || !q_out, "q_out without q");
   check_apart(k_pages, "k_pages", v_pages, "v_pages");
@@ -668,7 +668,8 @@ std::tuple<torch::Tensor, OptTensor> tree_attention(torch::Tensor q, torch::Tens
     RAB_CHECK(mask->size(1) <= (1 << 24), "mask is too wide");
   }
   const double sc = scale ? *scale : 1.0 / std::sqrt(static_cast<double>(dim));
-  RAB_CHECK(std::isfinite(sc), "scale must be finite");
+  const float scale_log2 = static_cast<float>(sc * 1.4426950408889634074);
+  RAB_CHECK(std::isfinite(scale_log2), "scale must be finite in fp32");
   if (out) {
     check_rope_output(*out, "out", q);
     RAB_CHECK(rows_aligned(*out), "out must have rows aligned to 16 bytes");
@@ -737,7 +738,7 @@ std::tuple<torch::Tensor, OptTensor> tree_attention(torch::Tensor q, torch::Tens
     p.mask_stride = bits.stride(0);
     p.mask_w = static_cast<int>(bits.size(1));
   }
-  p.scale_log2 = static_cast<float>(sc * 1.4426950408889634074);
+  p.scale_log2 = scale_log2;
   p.timeout_ns = static_cast<uint64_t>(timeout_s * 1e9);
   const int64_t most = max_q ? std::min<int64_t>(*max_q, total) : (cu ? total : r.uniform);
   const TreePlan plan = tree_plan(e, p, static_cast<int>(most), flash_sm_count());

@@ -395,3 +395,9 @@ def test_outputs_that_overlap_are_refused(ext):
     for q, k, qo, ko, what in cases:
         with pytest.raises(RuntimeError, match=what or "CUDA"):
             apply_rotary(q, k, pos, inv, out=(qo, ko))
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e300, math.nan])
+def test_scales_beyond_fp32_are_refused(ext, scale):
+    with pytest.raises(RuntimeError, match="scale must be finite"):
+        apply_rotary(**_args(scale=scale))

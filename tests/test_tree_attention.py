@@ -756,3 +756,10 @@ def test_the_result_may_take_the_place_of_the_queries(ext, cuda_device, dtype, t
     ctx_t = torch.tensor(ctx, dtype=torch.int32).cuda()
     want = tree_attention(q, kp, vp, table, ctx_t)
     assert torch.equal(tree_attention(q, kp, vp, table, ctx_t, out=q), want) and torch.equal(q, want)
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e300, 3e38, math.inf])
+def test_scales_beyond_fp32_are_refused(ext, scale):
+    """Scores are scaled in fp32, in base-2 units; a scale that is infinite there gives NaN."""
+    with pytest.raises(RuntimeError, match="scale must be finite"):
+        tree_attention(**_args(scale=scale))
