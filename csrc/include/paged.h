@@ -35,6 +35,7 @@ struct RopeOperand {
 struct RopeParams {
   RopeOperand op[3];
   int n_op;
+  int sms;  // of the GPU, for the launch
   int tokens, dim, rotary_dim;
   int interleaved;       // pairs (2p, 2p+1); otherwise (p, p + rotary_dim/2)
   float scale;           // factor on the rotated elements

@@ -408,11 +408,11 @@ int rope_run(const RopeParams& p, cudaStream_t stream) {
     const int rows_step = kRopeThreads / tasks;
     int most = 1;
     for (int i = 0; i < p.n_op; ++i) most = p.op[i].heads > most ? p.op[i].heads : most;
-    if (2 * most < rows_step && p.tokens >= 148 * 16) {
+    if (2 * most < rows_step && p.tokens >= p.sms * 16) {
       int tb = rows_step / most;
       tb = tb < 16 ? 16 : (tb > kJointTokens ? kJointTokens : tb);
       while (tb > 8 && tb * p.rotary_dim * static_cast<int>(sizeof(float)) > kJointSmem) tb >>= 1;
-      while (tb > 8 && (p.tokens + tb - 1) / tb < 148 * 4) tb >>= 1;
+      while (tb > 8 && (p.tokens + tb - 1) / tb < p.sms * 4) tb >>= 1;
       const size_t smem = static_cast<size_t>(tb) * (p.rotary_dim / 2) * sizeof(float2);
       return launch_overlapped(rope_joint_kernel<T, VEC, kInter>, dim3((p.tokens + tb - 1) / tb),
                                kRopeThreads, smem, stream, &p, &tasks, &tb);
@@ -425,7 +425,7 @@ int rope_run(const RopeParams& p, cudaStream_t stream) {
   while (true) {
     gy = 0;
     for (int i = 0; i < p.n_op; ++i) gy += (p.op[i].heads + hc - 1) / hc;
-    if (tb == 1 || static_cast<int64_t>((p.tokens + tb - 1) / tb) * gy >= 148 * 8) break;
+    if (tb == 1 || static_cast<int64_t>((p.tokens + tb - 1) / tb) * gy >= p.sms * 8) break;
     tb >>= 1;
     if (tb == 1) hc = kRopeThreads / tasks;
   }

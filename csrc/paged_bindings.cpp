@@ -185,9 +185,8 @@ void set_positions(RopeParams& p, const torch::Tensor& positions, int64_t tokens
 }
 
 // vectors of 16 bytes fit the head, the rotated part and its halves or pairs
-bool rope_vectors(Elem e, int64_t dim, int rotary_dim, bool interleaved) {
+bool rope_vectors(Elem e, int64_t dim, int rotary_dim) {
   const int64_t v = 16 / elem_bytes(e);
-  (void)interleaved;
   return dim % v == 0 && rotary_dim % (2 * v) == 0;
 }
 
@@ -265,11 +264,12 @@ std::tuple<torch::Tensor, OptTensor> rotary(torch::Tensor q, OptTensor k, torch:
   torch::Tensor qo = q_out ? *q_out : fresh(q.sizes(), q.scalar_type(), q);
   OptTensor ko = k_out;
   if (k && !ko) ko = fresh(k->sizes(), k->scalar_type(), q);
+  p.sms = flash_sm_count();
   p.interleaved = interleaved;
   p.scale = static_cast<float>(scale);
   p.sign = inverse ? -1.f : 1.f;
   // an operand without heads has no rows: the kernels share their threads out by heads
-  bool vec = rope_vectors(e, q.size(2), p.rotary_dim, interleaved);
+  bool vec = rope_vectors(e, q.size(2), p.rotary_dim);
   if (q.size(1) > 0) {
     p.op[p.n_op++] = dense_operand(q, qo);
     vec = vec && rows_aligned(q) && rows_aligned(qo);
@@ -449,7 +449,7 @@ OptTensor append_kv(torch::Tensor k, torch::Tensor v, torch::Tensor k_pages, tor
   if (q_out) check_same(*q_out, "q_out", k);
   p.status = status_of(status, k);
   const c10::cuda::CUDAGuard guard(k.device());
-  bool vec = rope_vectors(e, dim, p.rotary_dim, interleaved) && rows_aligned(k) && rows_aligned(v);
+  bool vec = rope_vectors(e, dim, p.rotary_dim) && rows_aligned(k) && rows_aligned(v);
   OptTensor qo = q_out;
   if (q) {
     if (!qo) qo = fresh(q->sizes(), q->scalar_type(), k);
@@ -467,6 +467,7 @@ OptTensor append_kv(torch::Tensor k, torch::Tensor v, torch::Tensor k_pages, tor
     o.paged = 1;
     p.op[p.n_op++] = o;
   }
+  p.sms = flash_sm_count();
   p.interleaved = interleaved;
   p.scale = static_cast<float>(scale);
   p.sign = 1.f;

@@ -381,3 +381,34 @@ def test_pools_and_outputs_that_overlap_are_refused(ext):
             append_kv(**args, q_out=out)
     with pytest.raises(RuntimeError, match="q_out shares memory with q"):
         append_kv(**_append_args(inv_freq=inv, q=flat[:3]), q_out=flat[1:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("ctx, counts, Hk, D, page", [
+    ([5, 0, 31, 16], [1, 0, 3, 33], 2, 128, 16),
+    ([0, 9, 2, 700], [1200, 0, 1, 1700], 1, 64, 16),  # many tokens of few heads
+])
+def test_append_holds_each_element_to_its_own_bound(ext, cuda_device, dtype, inter, ctx, counts, Hk, D, page):
+    """K within its own element's bound where it was written, and every other row as it was."""
+    T = sum(counts)
+    g = torch.Generator().manual_seed(9)
+    k, v = (torch.randn(T, Hk, D, generator=g).to(dtype) for _ in "kv")
+    table, pages = _table([c + m for c, m in zip(ctx, counts)], page)
+    kp, vp = _pool(pages, Hk, page, D, dtype)
+    inv = rotary_frequencies(D // 2)[0]
+    kd, vd = kp.cuda(), vp.cuda()
+    append_kv(k.cuda(), v.cuda(), kd, vd, table.cuda(), torch.tensor(ctx, dtype=torch.int32).cuda(),
+              _cu(counts).cuda(), inv_freq=inv.cuda(), interleaved=inter)
+    pos = torch.cat([torch.arange(c, c + m) for c, m in zip(ctx, counts)])
+    req = torch.repeat_interleave(torch.arange(len(counts)), torch.tensor(counts))
+    page_of, off = table[req, pos // page].long(), pos % page
+    got, ref = kd.cpu(), O.rotate(k, pos, inv, inter)
+    bound = O.rotate_bound(k, inv, inter, 1.0, dtype, pos)
+    assert ((got[page_of, :, off].double() - ref).abs() <= bound).all()
+    assert torch.equal(vd.cpu()[page_of, :, off], v)
+    other = torch.ones(pages, page, dtype=torch.bool)
+    other[page_of, off] = False
+    for x, y in ((got, kp), (vd.cpu(), vp)):
+        assert torch.equal(x.transpose(1, 2)[other], y.transpose(1, 2)[other])
