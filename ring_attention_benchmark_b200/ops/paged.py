@@ -13,11 +13,16 @@ read nor written.
 
 What device tensors hold cannot be refused without waiting for the GPU.  A page
 id outside the pool, a place outside the table or a path that is not increasing
-is skipped and reported in ``status`` (int32[8], see `new_status` and
-`check_status` in `ops.attention`) when one is given.
+is not written to, and reported in ``status`` (int32[8], see `new_status` and
+`check_status` in `ops.attention`) when one is given; attention reads a page outside
+the pool as zeros, whose keys score 0 and take weight.  Other requests of the call
+are unaffected.  The word keeps its first report; later calls may be given it.
 
 All calls run on the current stream of the tensors' GPU, keep nothing from one
-call to the next, and can be captured into CUDA graphs.
+call to the next, and can be captured into CUDA graphs.  None has a gradient.  What
+they write counts as changed in place, and must not overlap what they read; ``q_out``
+may be ``q``, and ``out`` the queries.  New tokens must not be slices of the pages
+that a call writes.
 """
 from __future__ import annotations
 
@@ -82,7 +87,7 @@ def tree_mask(parents: torch.Tensor, cu_q: Optional[torch.Tensor] = None, *, max
     a root).  A token sees its ancestors and itself.
 
     Returns ``(mask, depth)``: int32 words of 32 bits ``[tokens, ceil(max_q / 32)]``
-    for `tree_attention`, and int32 depths (0 for a root), so that a token's
+    for `tree_attention` (ancestors behind the last column are left out), and int32 depths (0 for a root), so that a token's
     position is ``context + depth``.  One call serves every layer of a step.
     """
     return load().tree_mask(parents, cu_q, batch, max_q, status)
@@ -109,10 +114,15 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
 
     ``q`` is ``[tokens, heads, dim]`` with dim 64 or 128 and heads a multiple of
     the cache's; page sizes 16 to 256, powers of two.  ``max_q`` is the most new
-    tokens of any request where the caller knows it; it only steers the choice of
-    kernel.  ``timeout_s`` bounds the kernel's waits for its own loads and products;
-    one that runs out is reported in ``status``.  Returns ``out``, or ``(out, lse)`` with the natural-log sums
-    ``[tokens, heads]`` in fp32.
+    tokens of any request where the caller knows it.  Any value is right; it chooses the
+    kernel: with ``cu_q`` alone a request could hold all the tokens, and a batch of
+    decoding steps would run on tiles of 256 rows.  A bool mask is packed in every call;
+    layers share one packed by `pack_mask`.
+
+    ``timeout_s`` bounds the kernel's waits for its own loads and products; one that runs out
+    is reported in ``status``, and calls given the word end early until it is cleared.
+    Returns ``out``, or ``(out, lse)`` with the natural-log sums ``[tokens, heads]`` in
+    fp32.
     """
     o, lse = load().tree_attention(q, k_pages, v_pages, block_table, context_lens, cu_q, max_q,
                                    mask, scale, return_lse, out, status, timeout_s)
