@@ -81,10 +81,11 @@ struct Half<__nv_bfloat16> {
 template <>
 struct Half<__half> {
   static constexpr uint32_t kExp = 0x7c00u;
-  // Weights are formed 2^15 times larger: fp16 holds nothing below 2^-25, and a quarter
+  // Weights are formed 2^7 times larger: fp16 holds nothing below 2^-25, and a quarter
   // million keys of such weights add up to a percent.  The sums and the merge carry the
-  // factor in the maximum, lowered by it.
-  static constexpr float kLift = 15.f;
+  // factor in the maximum, lowered by it.  Below half of 16, so that the lowered maximum
+  // of scores past 2^24, where fp32 counts in steps of 2 to 16, leaves weights of 2^8 at most.
+  static constexpr float kLift = 7.f;
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));

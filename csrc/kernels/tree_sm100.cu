@@ -58,7 +58,8 @@ constexpr int kM = 128;  // rows of a chain
 constexpr uint32_t kCols = 512;
 constexpr float kRescale = 8.0f;  // the running maximum moves when it grows by 2^8
 // fp16 weights are formed 2^7 times larger, at most 2^15 until the maximum moves: fp16
-// holds nothing below 2^-25, and many such weights of a long context add up
+// holds nothing below 2^-25, and many such weights of a long context add up.  7 and not
+// more as in tree_few.cu.
 constexpr float kLiftF16 = 7.0f;
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr uint32_t kRegsLaunch = 168;
@@ -589,12 +590,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                 fmax3(pm[(k >> 1) & 7], __uint_as_float(sr[k]), __uint_as_float(sr[k + 1]));
           const float mx = fmaxf(fmax3(fmax3(pm[0], pm[1], pm[2]), fmax3(pm[3], pm[4], pm[5]),
                                        pm[6]),
-                                 pm[7]) * sl2 - (kBF16 ? 0.f : kLiftF16);
-          const bool need = mx > m_run + kRescale;
+                                 pm[7]) * sl2;
+          // by the difference, which is exact where it matters: m_run + 8 would be rounded
+          // to steps of 16 for scores past 2^27
+          constexpr float kLift = kBF16 ? 0.f : kLiftF16;
+          const bool need = mx - m_run > kRescale + kLift;
           float alpha = 1.f;
           if (need) {
-            alpha = m_run == -INFINITY ? 0.f : ex2_approx(m_run - mx);
-            m_run = mx;
+            const float top = mx - kLift;
+            alpha = m_run == -INFINITY ? 0.f : ex2_approx(m_run - top);
+            m_run = top;
             l_run *= alpha;
           }
           // the scores' commit covers this chain's products before them: O is at rest

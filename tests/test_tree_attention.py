@@ -763,3 +763,37 @@ def test_scales_beyond_fp32_are_refused(ext, scale):
     """Scores are scaled in fp32, in base-2 units; a scale that is infinite there gives NaN."""
     with pytest.raises(RuntimeError, match="scale must be finite"):
         tree_attention(**_args(scale=scale))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [1, 12, 20, 130])
+@pytest.mark.parametrize("step", [1, 2, 4, 8, 16])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_scores_that_fp32_holds_in_whole_steps(ext, cuda_device, dtype, step, tokens):
+    """Scores of 1.25 * 2^23 * step in base-2 units, which fp32 holds to a step, and 16 to 48
+    more from tile to tile: weights are powers of two whatever the running maximum.
+
+    The scores are exact, so are their distances; the exponential is good to 2^-21, the sums
+    to 2^-24 a term, and a weight that is 2^-16 of the largest or more is exact in every type.
+    """
+    D, page, n = 64, 128, 40 * 128
+    g = torch.Generator().manual_seed(step)
+    more = torch.randint(0, 4, (n // page,), generator=g) * 16
+    more[0], more[-1] = 0, 48
+    kp, vp = torch.zeros(n // page + 2, 1, page, D), torch.randn(n // page + 2, 1, page, D, generator=g)
+    kp[:-2, 0, :, 0], kp[:-2, 0, :, 1] = 2048.0 * step, more[:, None].float()
+    vp = vp.to(dtype)
+    q = torch.zeros(tokens, 1, D)
+    q[:, 0, 0], q[:, 0, 1] = 5120.0, 1.0
+    table = torch.arange(n // page + 2, dtype=torch.int32).view(1, -1)
+    out, lse = tree_attention(q.to(dtype).cuda(), kp.to(dtype).cuda(), vp.cuda(), table.cuda(),
+                              torch.tensor([n], dtype=torch.int32).cuda(), scale=math.log(2.0),
+                              mask=torch.zeros(tokens, 1, dtype=torch.bool, device="cuda"), return_lse=True)
+    w = torch.exp2((more - 48).double()).repeat_interleave(page)
+    v = vp[:-2, 0].reshape(n, D).double()
+    want, mag = w @ v / w.sum(), w @ v.abs() / w.sum()
+    tol = mag * (2.0 ** -20 + n * 2.0 ** -23) + O.half_step(dtype) * want.abs()
+    # weights 2^-32 and 2^-48 below the largest may vanish in 16 bits: their share is below 2^-31
+    assert ((out.cpu().double()[:, 0] - want).abs() <= tol + 2.0 ** -31 * 8).all()
+    ref = (5120.0 * 2048.0 * step + 48 + math.log2(w.sum().item())) * math.log(2.0)
+    assert (lse.cpu().double() - ref).abs().max().item() <= 2 * 2.0 ** -24 * ref + 2.0 ** -20
