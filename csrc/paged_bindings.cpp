@@ -42,8 +42,9 @@ void check_same(const torch::Tensor& t, const char* name, const torch::Tensor& r
 void check_int32(const torch::Tensor& t, const char* name, int64_t dims) {
   RAB_CHECK(t.scalar_type() == torch::kInt32, "%s must be int32", name);
   RAB_CHECK(t.dim() == dims, "%s must have %lld dimension(s)", name, ll(dims));
-  RAB_CHECK(t.numel() == 0 || t.stride(dims - 1) == 1, "%s must be contiguous in its last dimension",
-            name);
+  // (the stride of a single element is any: contiguous() leaves it as it is)
+  RAB_CHECK(t.size(dims - 1) <= 1 || t.stride(dims - 1) == 1,
+            "%s must be contiguous in its last dimension", name);
 }
 
 // [tokens, heads, dim] with adjacent elements of a row

@@ -362,3 +362,44 @@ def test_uploads_inside_a_capture_are_refused(ext, cuda_device):
     assert cache.table.pages(other) == () and cache.length(seq) == 0
     step.accept([[0]])  # still open
     assert cache.length(seq) == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("parents, path", [([-1, 0, 0, 1, 2, 2], [0, 2, 5]), ([-1, 0, 0], [0, 2]),
+                                           ([-1, -1], [1]), ([-1, 0], []), ([-1], [0])])
+def test_one_sequence_from_prompt_to_defragmentation(ext, cuda_device, parents, path):
+    """The whole course with a single sequence: a prompt, a drafted tree whose path is accepted,
+    single tokens, a fork, a free and a defragmentation; the cache holds what was kept."""
+    L, Hk, D, n = 2, 2, 64, 21
+    g = torch.Generator().manual_seed(len(parents))
+    rot = Rotary(D, device="cuda")
+    cache = PagedKVCache(L, 16, Hk, D, page_size=16)
+    seq = cache.new_sequence()
+    kept = [torch.zeros(0, Hk, D).bfloat16() for _ in range(L)]
+
+    def write(step, keep, mask=None, positions=None):
+        for layer in range(L):
+            q, k, v = (torch.randn(step.tokens, h, D, generator=g).bfloat16() for h in (4, Hk, Hk))
+            q = step.append(layer, k.cuda(), v.cuda(), rotary=rot, q=q.cuda(), positions=positions)
+            assert step.attend(layer, q, mask=mask).isfinite().all()
+            kept[layer] = torch.cat((kept[layer], v[keep]))
+
+    step = cache.step([seq], [n])
+    write(step, list(range(n)))
+    step.commit()
+    step = cache.step([seq], [len(parents)])
+    mask, depth = step.tree([parents])
+    write(step, path, mask, step.positions(depth))
+    step.accept([path])
+    for _ in range(3):
+        step = cache.step([seq], [1])
+        write(step, [0])
+        step.commit()
+    best = cache.fork(seq)
+    cache.free(seq)
+    assert cache.defragment() == len(cache.table.pages(best))
+    assert cache.length(best) == n + len(path) + 3
+    pages = cache.table.pages(best)
+    for layer in range(L):
+        held = torch.stack([cache.v[layer, pages[i // 16], :, i % 16] for i in range(cache.length(best))])
+        assert torch.equal(held.cpu(), kept[layer])

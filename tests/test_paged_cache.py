@@ -412,3 +412,27 @@ def test_append_holds_each_element_to_its_own_bound(ext, cuda_device, dtype, int
     other[page_of, off] = False
     for x, y in ((got, kp), (vd.cpu(), vp)):
         assert torch.equal(x.transpose(1, 2)[other], y.transpose(1, 2)[other])
+
+
+@pytest.mark.gpu
+def test_single_entries_of_any_stride(ext, cuda_device):
+    """One request's lengths, pages, borders and path may be slices of wider tensors: the stride
+    of a single element means nothing."""
+    from ring_attention_benchmark_b200.ops.paged import tree_attention
+
+    kp, vp = _pool(3, 1, 16, 64, torch.float32)
+    wide = torch.tensor([[2, 9], [1, 9], [1, 9]], dtype=torch.int32).cuda()
+    table, one = wide[:1, :1], wide[1:2, 0]  # page 2; one
+    ctx = torch.tensor([[5, 9]], dtype=torch.int32).cuda()[:, 0]
+    assert one.stride(0) == 2 and ctx.stride(0) == 2
+    k, v = torch.randn(2, 1, 64), torch.randn(2, 1, 64)
+    kd, vd = kp.cuda(), vp.cuda()
+    append_kv(k.cuda(), v.cuda(), kd, vd, table, ctx)
+    kp[2, 0, 5:7], vp[2, 0, 5:7] = k[:, 0], v[:, 0]
+    assert torch.equal(kd.cpu(), kp) and torch.equal(vd.cpu(), vp)
+    q = torch.randn(2, 1, 64).cuda()
+    assert torch.equal(tree_attention(q, kd, vd, table, ctx),
+                       tree_attention(q, kd, vd, table.contiguous().clone(), ctx.clone()))
+    compact_path(kd, vd, table, ctx, one.view(1, 1), one)
+    kp[2, 0, 5], vp[2, 0, 5] = k[1, 0], v[1, 0]
+    assert torch.equal(kd.cpu(), kp) and torch.equal(vd.cpu(), vp)
