@@ -62,9 +62,11 @@ torch::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const torch::Ten
 
 bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
 
+// every row begins on a 16-byte boundary (the stride of a single token or head is none)
 bool rows_aligned(const torch::Tensor& t) {
   const int64_t e = t.element_size();
-  return aligned16(t.data_ptr()) && t.stride(0) * e % 16 == 0 && t.stride(1) * e % 16 == 0;
+  return aligned16(t.data_ptr()) && (t.size(0) <= 1 || t.stride(0) * e % 16 == 0) &&
+         (t.size(1) <= 1 || t.stride(1) * e % 16 == 0);
 }
 
 // Strides and sizes in bytes of the dimensions that step through memory.

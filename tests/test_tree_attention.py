@@ -797,3 +797,30 @@ def test_scores_that_fp32_holds_in_whole_steps(ext, cuda_device, dtype, step, to
     assert ((out.cpu().double()[:, 0] - want).abs() <= tol + 2.0 ** -31 * 8).all()
     ref = (5120.0 * 2048.0 * step + 48 + math.log2(w.sum().item())) * math.log(2.0)
     assert (lse.cpu().double() - ref).abs().max().item() <= 2 * 2.0 ** -24 * ref + 2.0 ** -20
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_one_row_of_an_odd_stride(ext, cuda_device, dtype):
+    """A single token or head may be a slice of any width, queries and results alike."""
+    from ring_attention_benchmark_b200.ops.rotary import apply_rotary, rotary_frequencies
+
+    ctx, D = [40], 64
+    for T, H in ((1, 4), (3, 1), (1, 1)):
+        q, kp, vp, table = (x.cuda() for x in _case(ctx, [T], H, 1, D, 16, dtype, seed=44))
+        ctx_t = torch.tensor(ctx, dtype=torch.int32).cuda()
+        want = tree_attention(q, kp, vp, table, ctx_t)
+        pos, inv = torch.arange(T).cuda(), rotary_frequencies(D)[0].cuda()
+        turned = apply_rotary(q, None, pos, inv)
+        for st, sh in ((H * D + 1, D), (H * D + 8, D + 1)):
+            if (T > 1 and st % 8) or (H > 1 and sh % 8):
+                continue
+            flat_q, flat_o = (torch.full((T * st + 64 * H,), 3.0, dtype=dtype, device="cuda") for _ in "qo")
+            odd, out = (x.as_strided((T, H, D), (st, sh, 1)) for x in (flat_q, flat_o))
+            odd.copy_(q)
+            assert torch.equal(tree_attention(odd, kp, vp, table, ctx_t, out=out), want) and torch.equal(out, want)
+            apply_rotary(odd, None, pos, inv, out=(out, None))
+            assert torch.equal(out, turned)
+            left = torch.ones(flat_o.numel(), dtype=torch.bool, device="cuda")
+            left.as_strided((T, H, D), (st, sh, 1)).fill_(False)
+            assert (flat_o[left] == 3.0).all()
