@@ -403,3 +403,88 @@ def test_one_sequence_from_prompt_to_defragmentation(ext, cuda_device, parents, 
     for layer in range(L):
         held = torch.stack([cache.v[layer, pages[i // 16], :, i % 16] for i in range(cache.length(best))])
         assert torch.equal(held.cpu(), kept[layer])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seed", range(6))
+def test_a_random_course_of_a_cache(ext, cuda_device, seed):
+    """Steps (prompts, single tokens, trees, none), paths, forks, truncations, frees and
+    defragmentations at random: V of every sequence stays what was kept, K too, and every
+    attention is that of the rows that its sequence holds."""
+    rng, g = random.Random(seed), torch.Generator().manual_seed(seed)
+    D, L = rng.choice([(64, 2), (128, 1)])
+    Hk, group, page = rng.choice([1, 2, 3]), rng.choice([1, 2, 5]), rng.choice([16, 32])
+    dtype = [torch.bfloat16, torch.float16, torch.float32][seed % 3]
+    cache = PagedKVCache(L, 24, Hk, D, page_size=page, dtype=dtype)
+    held = {}
+
+    def rand(n, h):
+        return torch.randn(n, h, D, generator=g).to(dtype)
+
+    for _ in range(60):
+        op, seqs = rng.random(), cache.table.sequences()
+        if not seqs or op < 0.1:
+            held[cache.new_sequence()] = [[torch.zeros(0, Hk, D).to(dtype)] * 2] * L
+        elif op < 0.2:
+            s = rng.choice(seqs)
+            held[cache.fork(s)] = held[s]
+        elif op < 0.3 and len(seqs) > 2:
+            s = rng.choice(seqs)
+            cache.free(s)
+            del held[s]
+        elif op < 0.38:
+            s = rng.choice(seqs)
+            n = rng.randint(0, cache.length(s))
+            cache.truncate(s, n)
+            held[s] = [[x[:n] for x in kv] for kv in held[s]]
+        elif op < 0.45:
+            cache.defragment()
+        else:
+            some = rng.sample(seqs, rng.randint(1, len(seqs)))
+            counts = [rng.choice([0, 1, 1, 2, 7, 30]) for _ in some]
+            try:
+                step = cache.step(some, counts)
+            except OutOfPages:
+                continue
+            tree = rng.random() < 0.5
+            parents = [[-1 if i == 0 else rng.randint(-1, i - 1) for i in range(n)] for n in counts]
+            mask, depth = step.tree(parents) if tree else (None, None)
+            masks = [O.ancestors(p)[0] for p in parents] if tree else None
+            new = [[] for _ in some]
+            pad = rng.choice([0, 0, 3])
+            for layer in range(L):
+                q, k, v = rand(step.tokens + pad, Hk * group), rand(step.tokens + pad, Hk), rand(step.tokens + pad, Hk)
+                step.append(layer, k.cuda(), v.cuda())
+                m = mask if mask is None or not pad else torch.cat((mask, mask.new_zeros(pad, mask.shape[1])))
+                out, lse = step.attend(layer, q.cuda(), mask=m, return_lse=True)
+                at = 0
+                for b, (s, n) in enumerate(zip(some, counts)):
+                    rows, was = slice(at, at + n), held[s][layer]
+                    kk, vv = torch.cat((was[0], k[rows])), torch.cat((was[1], v[rows]))
+                    new[b].append((k[rows], v[rows]))
+                    at += n
+                    if n == 0:
+                        continue
+                    pool = [x.permute(1, 0, 2).reshape(1, Hk, len(x), D) for x in (kk, vv)]
+                    ref, rlse, mag, smax = O.attention(q[rows], *pool, torch.zeros(1, 1, dtype=torch.int32),
+                                                       [len(kk) - n], [n], masks and [masks[b]])
+                    bo, bl = O.attention_bound(ref, mag, smax, dtype, len(kk), D)
+                    assert ((out[rows].cpu().double() - ref).abs() <= bo).all()
+                    assert ((lse[rows].cpu().double() - rlse).abs() <= bl + 2.0 ** -22 * rlse.abs()).all()
+            if rng.random() < 0.15:
+                paths = [[] for _ in some]
+                step.cancel()
+            elif tree:
+                paths = [sorted(rng.sample(range(n), rng.randint(0, n))) for n in counts]
+                step.accept(paths)
+            else:
+                paths = [list(range(n)) for n in counts]
+                step.commit()
+            for s, kv, p in zip(some, new, paths):
+                held[s] = [[torch.cat((x, y[p])) for x, y in zip(held[s][layer], kv[layer])] for layer in range(L)]
+        for s in cache.table.sequences():
+            n, pages = cache.length(s), torch.tensor(cache.table.pages(s), dtype=torch.long)
+            i = torch.arange(n)
+            for layer in range(L):
+                for pool, rows in zip((cache.k, cache.v), held[s][layer]):
+                    assert torch.equal(pool[layer].cpu()[pages[i // page], :, i % page], rows)
